@@ -5,3 +5,4 @@ libgat_mi355.so (include/gat_mi355.h): hand-written HIP kernels only, no fallbac
 """
 from .layer import GATConv  # noqa: F401
 from .graph import GraphLayout, build_graph, cached_graph  # noqa: F401
+from .dense import dropout, embedding, group_norm_act, linear_act  # noqa: F401

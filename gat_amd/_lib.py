@@ -70,6 +70,17 @@ class Glue(C.Structure):
                 ("beta", C.c_void_p), ("running_mean", C.c_void_p), ("running_var", C.c_void_p)]
 
 
+class Linear(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("in_features", C.c_int32), ("out_features", C.c_int32),
+                ("dtype", C.c_int32), ("act", C.c_int32)]
+
+
+class GroupNorm(C.Structure):
+    _fields_ = [("batch", C.c_int64), ("length", C.c_int64), ("groups", C.c_int32), ("width", C.c_int32),
+                ("dtype", C.c_int32), ("act", C.c_int32), ("eps", C.c_float), ("_pad", C.c_int32),
+                ("weight", C.c_void_p), ("bias", C.c_void_p)]
+
+
 # name -> (restype, argtypes); every symbol include/gat_mi355.h declares
 SYMBOLS = {
     "gatmi_last_error": (C.c_char_p, []),
@@ -142,6 +153,23 @@ SYMBOLS = {
                                  C.c_void_p, C.c_size_t, C.c_void_p]),
     "gatmi_tail_bwd": (C.c_int, [C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                  C.c_void_p, C.c_void_p, C.c_void_p]),
+    "gatmi_linear_fwd": (C.c_int, [C.POINTER(Linear), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                   C.c_void_p, C.c_void_p, C.c_void_p]),
+    "gatmi_linear_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(Linear)]),
+    "gatmi_linear_bwd": (C.c_int, [C.POINTER(Linear), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "gatmi_group_norm_workspace_bytes": (C.c_size_t, [C.POINTER(GroupNorm)]),
+    "gatmi_group_norm_fwd": (C.c_int, [C.POINTER(GroupNorm), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                       C.c_void_p, C.c_size_t, C.c_void_p]),
+    "gatmi_group_norm_bwd": (C.c_int, [C.POINTER(GroupNorm), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                       C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "gatmi_embedding_fwd": (C.c_int, [C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_float, C.c_void_p,
+                                      C.c_void_p, C.c_void_p, C.c_void_p]),
+    "gatmi_embedding_bwd_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int64]),
+    "gatmi_embedding_bwd": (C.c_int, [C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_float, C.c_void_p,
+                                      C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "gatmi_dropout": (C.c_int, [C.c_int32, C.c_int64, C.c_int64, C.c_float, C.c_uint64, C.c_void_p,
+                                C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "gatmi_set_option": (C.c_int, [C.c_char_p, C.c_int]),
     "gatmi_knn_workspace_bytes": (C.c_size_t, [C.c_int64]),
     "gatmi_knn_graph": (C.c_int, [C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p,

@@ -1,0 +1,183 @@
+// Device-side building blocks of the dense operators (linear.hip, group_norm.hip, embedding.hip,
+// dropout.hip): element types, vector access at element alignment, activations.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+#include "../../include/gat_mi355.h"
+
+namespace gatmi {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+// V elements as one access.  The address only needs the element's own alignment: rows of odd widths and
+// sliced tensors start anywhere, and a global load or store of up to 16 bytes takes that as it is.
+template <class T, int V> struct __attribute__((packed, aligned(sizeof(T)))) RawVec { T e[V]; };
+
+template <int V> struct VecF { float e[V]; };
+
+template <class T, int V> __device__ __forceinline__ VecF<V> ldv(const T *p) {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    typedef vec uvec __attribute__((aligned(sizeof(T))));
+    VecF<V> r;
+    if constexpr (V == 1) {
+        r.e[0] = (float)p[0];
+    } else {
+        const vec v = *reinterpret_cast<const uvec *>(p);
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.e[i] = (float)v[i];
+    }
+    return r;
+}
+// f32 -> T rounds to nearest even, once
+template <class T, int V> __device__ __forceinline__ void stv(T *p, const VecF<V> &r) {
+    typedef T vec __attribute__((ext_vector_type(V)));
+    typedef vec uvec __attribute__((aligned(sizeof(T))));
+    if constexpr (V == 1) {
+        p[0] = (T)r.e[0];
+    } else {
+        vec v;
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = (T)r.e[i];
+        *reinterpret_cast<uvec *>(p) = v;
+    }
+}
+
+// Division of a 32-bit number by a divisor fixed at launch: one high multiply instead of a division
+// (round-up multiplier with the carry kept in the shift, exact for every 32-bit numerator).
+struct FastDiv {
+    uint32_t d, m, s;
+};
+inline FastDiv make_fast_div(uint32_t d) {
+    FastDiv f;
+    f.d = d;
+    uint32_t l = 0;
+    while (l < 32 && (1ull << l) < d) ++l;
+    f.m = (uint32_t)((((1ull << l) - d) << 32) / d + 1);
+    f.s = l;
+    return f;
+}
+__device__ __forceinline__ uint32_t fdiv(const FastDiv &f, uint32_t n) {
+    const uint32_t t = __umulhi(f.m, n);
+    return f.s == 0 ? n : (t + ((n - t) >> 1)) >> (f.s - 1);
+}
+
+// ---- activations: value and derivative at z, f32.  EXACT: the library's expm1 / exp / erf, for f32
+// tensors.  Otherwise (results are rounded to 16 bits) v_exp_f32 forms, whose error of a few 2^-22 is a
+// hundredth of that rounding.
+template <bool EXACT> __device__ __forceinline__ float act_exp(float v) {
+    if constexpr (EXACT) return expf(v);
+    return __builtin_amdgcn_exp2f(v * 1.44269502162933349609375f);
+}
+
+// exp(z) - 1 for z <= 0
+template <bool EXACT> __device__ __forceinline__ float act_expm1(float z) {
+    if constexpr (EXACT) return expm1f(z);
+    // next to 0 the subtraction would cancel: z + z^2/2 + z^3/6, off by z^3/24 relative (< 2^-20 there)
+    const float e = act_exp<false>(z) - 1.0f;
+    const float s = z * fmaf(z, fmaf(z, 0.16666667f, 0.5f), 1.0f);
+    return z > -0.03f ? s : e;
+}
+
+// The normal distribution function.  16-bit results: 1 - t(a1 + .. + a5 t^4) exp(-z^2/2) with
+// t = 1 / (1 + p |z| / sqrt 2) (Abramowitz and Stegun 7.1.26, absolute error 1.5e-7 of erf); the
+// lower tail is taken from the product itself, not from a difference.  `gauss` = exp(-z^2/2).
+template <bool EXACT> __device__ __forceinline__ float act_phi(float z, float &gauss) {
+    if constexpr (EXACT) {
+        gauss = expf(-0.5f * z * z);
+        return 0.5f * (1.0f + erff(z * 0.70710678118654752f));
+    }
+    gauss = act_exp<false>(-0.5f * z * z);
+    const float a = fabsf(z) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.0f));
+    float q = fmaf(t, 1.061405429f, -1.453152027f);
+    q = fmaf(t, q, 1.421413741f);
+    q = fmaf(t, q, -0.284496736f);
+    q = fmaf(t, q, 0.254829592f);
+    const float tail = 0.5f * q * t * gauss;
+    return z > 0.f ? 1.0f - tail : tail;
+}
+
+template <int ACT, bool EXACT> __device__ __forceinline__ float act_value(float z) {
+    if constexpr (ACT == GATMI_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
+    if constexpr (ACT == GATMI_ACT_ELU) return z > 0.f ? z : act_expm1<EXACT>(z);
+    if constexpr (ACT == GATMI_ACT_SILU) {
+        const float d = 1.0f + act_exp<EXACT>(-z);   // +inf for z far below 0: the quotient is -0
+        return EXACT ? z / d : z * __builtin_amdgcn_rcpf(d);
+    }
+    if constexpr (ACT == GATMI_ACT_GELU) {
+        float g;
+        return z * act_phi<EXACT>(z, g);
+    }
+    return z;
+}
+
+// (value, derivative)
+template <int ACT, bool EXACT> __device__ __forceinline__ float act_both(float z, float &d) {
+    if constexpr (ACT == GATMI_ACT_RELU) {
+        d = z > 0.f ? 1.f : (z != z ? z : 0.f);
+        return z > 0.f ? z : (z != z ? z : 0.f);
+    }
+    if constexpr (ACT == GATMI_ACT_ELU) {
+        const float e = act_expm1<EXACT>(z);
+        d = z > 0.f ? 1.f : (EXACT ? expf(z) : e + 1.f);
+        return z > 0.f ? z : e;
+    }
+    if constexpr (ACT == GATMI_ACT_SILU) {
+        const float q = 1.0f + act_exp<EXACT>(-z);
+        const float s = EXACT ? 1.0f / q : __builtin_amdgcn_rcpf(q);
+        d = s * (1.0f + z * (1.0f - s));
+        return EXACT ? z / q : z * s;
+    }
+    if constexpr (ACT == GATMI_ACT_GELU) {
+        float g;
+        const float phi = act_phi<EXACT>(z, g);
+        d = fmaf(z * 0.3989422804014327f, g, phi);
+        return z * phi;
+    }
+    d = 1.f;
+    return z;
+}
+
+template <class T> struct IsF32 { static constexpr bool value = false; };
+template <> struct IsF32<float> { static constexpr bool value = true; };
+
+// f(integral_constant V) for a vector of v elements: 16 bytes, or less where a row is shorter
+template <class T, class F> void with_vec(int v, F f) {
+    constexpr int VM = 16 / sizeof(T);
+    if (v == VM) f(std::integral_constant<int, VM>{});
+    else if (v == 1) f(std::integral_constant<int, 1>{});
+    else if (v == 2) f(std::integral_constant<int, 2>{});
+    else f(std::integral_constant<int, 4>{});
+}
+// the widest vector, in elements, that a row of n elements takes
+inline int vec_of(int dtype, long long n) {
+    int v = dtype == GATMI_F32 ? 4 : 8;
+    while (v > n) v >>= 1;
+    return v;
+}
+
+}  // namespace gatmi
+
+// Runs BODY with `T` bound to the element type of a GATMI_F32 / _BF16 / _F16 code (checked before).
+#define GATMI_WITH_TYPE(code, ...)                                                        \
+    do {                                                                                  \
+        if ((code) == GATMI_F32) { using T = float; __VA_ARGS__; }                        \
+        else if ((code) == GATMI_BF16) { using T = gatmi::bf16_t; __VA_ARGS__; }          \
+        else { using T = gatmi::f16_t; __VA_ARGS__; }                                     \
+    } while (0)
+
+// ... and with `ACT` bound to an activation code
+#define GATMI_WITH_ACT(code, ...)                                                         \
+    do {                                                                                  \
+        switch (code) {                                                                   \
+        case GATMI_ACT_RELU: { constexpr int ACT = GATMI_ACT_RELU; __VA_ARGS__; break; }  \
+        case GATMI_ACT_ELU: { constexpr int ACT = GATMI_ACT_ELU; __VA_ARGS__; break; }    \
+        case GATMI_ACT_SILU: { constexpr int ACT = GATMI_ACT_SILU; __VA_ARGS__; break; }  \
+        case GATMI_ACT_GELU: { constexpr int ACT = GATMI_ACT_GELU; __VA_ARGS__; break; }  \
+        default: { constexpr int ACT = GATMI_ACT_NONE; __VA_ARGS__; break; }              \
+        }                                                                                 \
+    } while (0)

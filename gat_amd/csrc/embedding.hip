@@ -1,0 +1,485 @@
+// Embedding lookup with scaling, and its gradient by sorted ids.
+//   forward   y[i, :] = scale * table[ids[i], :]            (a zero row where ids[i] is outside [0, vocab))
+//   backward  dtable[v, :] = scale * sum_{i : ids[i] = v} dy[i, :]
+//
+// The gradient is a segmented sum: a stable radix sort of (id, position) puts the rows of one table entry
+// side by side, in the order of the positions, and the sorted list is summed in fixed chunks of rows -- so
+// that one frequent id costs what many rare ones do -- whose unfinished ends are summed the same way, level
+// by level.  No float atomics: the order of every sum is fixed by the ids alone.
+#include "attn_device.h"
+#include "common.h"
+#include "dense_device.h"
+
+namespace gatmi {
+
+// ---- forward ---------------------------------------------------------------------------------
+constexpr int kEmbUnroll = 4;
+
+struct EmbArgs {
+    const int64_t *ids;
+    const void *table;
+    void *y;
+    long long n, vocab;
+    int dim, W, w_log;     // W lanes a row
+    float scale;
+};
+
+template <class T, int V> __global__ __launch_bounds__(256) void emb_fwd_kernel(const EmbArgs A) {
+    const int lane = threadIdx.x & (A.W - 1);
+    const int per_block = 256 >> A.w_log;
+    const T *table = static_cast<const T *>(A.table);
+    T *y = static_cast<T *>(A.y);
+    const long long first = (long long)blockIdx.x * (per_block * kEmbUnroll) + (threadIdx.x >> A.w_log);
+    long long id[kEmbUnroll];
+#pragma unroll
+    for (int u = 0; u < kEmbUnroll; ++u) {
+        const long long i = first + u * per_block;
+        id[u] = i < A.n ? A.ids[i] : -1;
+    }
+    for (int j0 = lane * V; j0 < A.dim; j0 += A.W * V) {
+        const int j = j0 + V <= A.dim ? j0 : A.dim - V;     // the last vector steps back (equal stores)
+        VecF<V> v[kEmbUnroll];
+#pragma unroll
+        for (int u = 0; u < kEmbUnroll; ++u) {
+            if (id[u] >= 0 && id[u] < A.vocab) {
+                v[u] = ldv<T, V>(table + id[u] * A.dim + j);
+            } else {
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[u].e[k] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kEmbUnroll; ++u) {
+            const long long i = first + u * per_block;
+            if (i >= A.n) continue;
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[u].e[k] *= A.scale;
+            stv<T, V>(y + i * A.dim + j, v[u]);
+        }
+    }
+}
+
+// ---- stable radix sort of (id, position), 8 bits a pass -----------------------------------------
+// A block owns kSortTile consecutive items; wave w of it the items [w * 64 * kSortItems, ..), 64 at a time.
+constexpr int kSortItems = 16, kSortTile = 256 * kSortItems;
+
+struct SortArgs {
+    const int64_t *ids;            // first pass: keys come from here, positions are the indices
+    const uint32_t *key_in, *pos_in;
+    uint32_t *key_out, *pos_out;
+    uint32_t *hist;                // [256][blocks]
+    uint32_t *total;               // [256]
+    long long n, vocab;
+    int blocks, shift;
+};
+
+// ids outside the table get the key `vocab`: they sort behind every row and are left out of the sums
+__device__ __forceinline__ uint32_t sort_key(const SortArgs &A, long long i) {
+    if (A.ids) {
+        const long long id = A.ids[i];
+        return (uint32_t)(id >= 0 && id < A.vocab ? id : A.vocab);
+    }
+    return A.key_in[i];
+}
+
+// Lanes of this wave whose digit equals this lane's (only lanes with `on` count)
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool on) {
+    uint64_t m = __ballot(on);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        const uint64_t bit = __ballot((digit >> b) & 1u);
+        m &= (digit >> b) & 1u ? bit : ~bit;
+    }
+    return m;
+}
+
+__global__ __launch_bounds__(256) void sort_count_kernel(const SortArgs A) {
+    __shared__ uint32_t h[256];
+    h[threadIdx.x] = 0;
+    __syncthreads();
+    const long long base = (long long)blockIdx.x * kSortTile;
+#pragma unroll 4
+    for (int k = 0; k < kSortItems; ++k) {
+        const long long i = base + k * 256 + threadIdx.x;
+        if (i < A.n) atomicAdd(&h[(sort_key(A, i) >> A.shift) & 255u], 1u);   // integers: any order
+    }
+    __syncthreads();
+    A.hist[(long long)threadIdx.x * A.blocks + blockIdx.x] = h[threadIdx.x];
+}
+
+// block d: exclusive scan of digit d's counts over the tiles; total[d]
+__global__ __launch_bounds__(256) void sort_scan_kernel(const SortArgs A) {
+    __shared__ uint32_t wsum[4];
+    uint32_t *row = A.hist + (long long)blockIdx.x * A.blocks;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t carry = 0;
+    for (int base = 0; base < A.blocks; base += 256) {
+        const int i = base + threadIdx.x;
+        const uint32_t v = i < A.blocks ? row[i] : 0;
+        uint32_t s = v;
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t up = __shfl_up(s, o, 64);
+            if (lane >= o) s += up;
+        }
+        if (lane == 63) wsum[wave] = s;
+        __syncthreads();
+        uint32_t before = carry;
+        for (int w = 0; w < wave; ++w) before += wsum[w];
+        const uint32_t all = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+        if (i < A.blocks) row[i] = before + s - v;
+        carry += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) A.total[blockIdx.x] = carry;
+}
+
+__global__ __launch_bounds__(256) void sort_scatter_kernel(const SortArgs A) {
+    // per wave and digit: items seen; then where they start.  volatile: lanes of a wave read each other's counts
+    __shared__ volatile uint32_t cnt[4][256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int w = 0; w < 4; ++w) cnt[w][threadIdx.x] = 0;
+    __syncthreads();
+    const long long base = (long long)blockIdx.x * kSortTile + (long long)wave * (64 * kSortItems) + lane;
+    uint32_t key[kSortItems], pos[kSortItems], rank[kSortItems];
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        const long long i = base + k * 64;
+        const bool on = i < A.n;
+        key[k] = on ? sort_key(A, i) : 0u;
+        pos[k] = on ? (A.ids ? (uint32_t)i : A.pos_in[i]) : 0u;
+    }
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        const bool on = base + k * 64 < A.n;
+        const uint32_t digit = (key[k] >> A.shift) & 255u;
+        const uint64_t m = same_digit(digit, on);
+        const uint32_t before = __popcll(m & ((1ull << lane) - 1ull));
+        // only this wave touches its row of counts; its lanes' LDS accesses are in order
+        const uint32_t seen = on ? cnt[wave][digit] : 0u;
+        rank[k] = seen + before;
+        if (on && before == 0) cnt[wave][digit] = seen + (uint32_t)__popcll(m);
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    {   // thread d: where digit d starts in the output, then each wave's share of this tile
+        __shared__ uint32_t wsum[4];
+        const uint32_t t = A.total[threadIdx.x];
+        uint32_t s = t;
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t up = __shfl_up(s, o, 64);
+            if (lane >= o) s += up;
+        }
+        if (lane == 63) wsum[wave] = s;
+        __syncthreads();
+        uint32_t at = s - t + A.hist[(long long)threadIdx.x * A.blocks + blockIdx.x];
+        for (int w = 0; w < wave; ++w) at += wsum[w];
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t c = cnt[w][threadIdx.x];
+            cnt[w][threadIdx.x] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k)
+        if (base + k * 64 < A.n) {
+            const uint32_t to = cnt[wave][(key[k] >> A.shift) & 255u] + rank[k];
+            A.key_out[to] = key[k];
+            A.pos_out[to] = pos[k];
+        }
+}
+
+// ---- segmented sum of the sorted rows -----------------------------------------------------------
+// One level: entries [0, n) in order, equal keys side by side; entry e stands for row `row(e)` of the
+// source (none: a key that only continues its neighbours).  A lane group walks a chunk of entries and
+// stores every segment that lies inside the chunk; the parts of segments that cross its ends go to
+// (first, last) entries of the next level.
+constexpr uint32_t kNoKey = 0xffffffffu;
+
+struct SegArgs {
+    const uint32_t *key, *pos;    // level 0: sorted keys and positions
+    const uint32_t *flag;         // level > 0: 1 where the entry carries a row
+    const void *src;              // level 0: dy; level > 0: f32 partial rows
+    void *out;                    // dtable
+    uint32_t *nkey, *nflag;       // next level's entries, two a chunk
+    float *nsrc;
+    long long n;
+    uint32_t vocab;
+    int dim, chunk, W, w_log;
+    float scale;
+};
+
+template <class T, class S, int V, bool LEAF>
+__global__ __launch_bounds__(256) void seg_sum_kernel(const SegArgs A) {
+    const int lane = threadIdx.x & (A.W - 1);
+    const long long c = (long long)blockIdx.x * (256 >> A.w_log) + (threadIdx.x >> A.w_log);
+    const long long e0 = c * A.chunk;
+    if (e0 >= A.n) return;
+    const long long e1 = e0 + A.chunk < A.n ? e0 + A.chunk : A.n;
+    const int j0 = (blockIdx.y * A.W + lane) * V;
+    const bool on = j0 < A.dim;
+    const int j = !on ? 0 : (j0 + V <= A.dim ? j0 : A.dim - V);
+    const S *src = static_cast<const S *>(A.src) + j;
+    T *out = static_cast<T *>(A.out) + j;
+    const uint32_t before = e0 > 0 ? A.key[e0 - 1] : kNoKey, after = e1 < A.n ? A.key[e1] : kNoKey;
+    const uint32_t head = A.key[e0], tail = A.key[e1 - 1];
+    const bool open_head = head < A.vocab && head == before;
+    const bool open_tail = tail < A.vocab && tail == after;
+    uint32_t k0 = kNoKey, k1 = kNoKey, f0 = 0, f1 = 0;
+    VecF<V> acc;
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc.e[k] = 0.f;
+    uint32_t cur = head;
+    bool first = true;      // the chunk's first segment
+    constexpr int U = 8;
+    for (long long e = e0; e < e1; e += U) {
+        uint32_t kk[U];
+        VecF<V> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool in = e + u < e1;
+            kk[u] = in ? A.key[e + u] : kNoKey;
+            const bool row = in && kk[u] < A.vocab && (LEAF || A.flag[e + u]);
+            if (row) {
+                const long long r = LEAF ? (long long)A.pos[e + u] : e + u;
+                v[u] = ldv<S, V>(src + r * A.dim);
+            } else {
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[u].e[k] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (e + u >= e1) break;
+            if (kk[u] != cur) {       // `cur` ends inside this chunk
+                if (cur < A.vocab) {
+                    if (first && open_head) {
+                        k0 = cur;
+                        f0 = 1;
+                        if (on) stv<float, V>(A.nsrc + (2 * c) * A.dim + j, acc);
+                    } else if (on) {
+#pragma unroll
+                        for (int k = 0; k < V; ++k) acc.e[k] *= A.scale;
+                        stv<T, V>(out + (long long)cur * A.dim, acc);
+                    }
+                }
+                first = false;
+                cur = kk[u];
+#pragma unroll
+                for (int k = 0; k < V; ++k) acc.e[k] = 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc.e[k] += v[u].e[k];
+        }
+    }
+    if (cur < A.vocab) {
+        if (first && open_head) {         // the whole chunk: one entry, continued to the right if it goes on
+            k0 = cur;
+            f0 = 1;
+            if (on) stv<float, V>(A.nsrc + (2 * c) * A.dim + j, acc);
+            if (open_tail) k1 = cur;
+        } else if (open_tail) {
+            k1 = cur;
+            f1 = 1;
+            if (on) stv<float, V>(A.nsrc + (2 * c + 1) * A.dim + j, acc);
+        } else if (on) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc.e[k] *= A.scale;
+            stv<T, V>(out + (long long)cur * A.dim, acc);
+        }
+    }
+    if (lane == 0 && blockIdx.y == 0 && A.nkey) {
+        A.nkey[2 * c] = k0;
+        A.nkey[2 * c + 1] = k1;
+        A.nflag[2 * c] = f0;
+        A.nflag[2 * c + 1] = f1;
+    }
+}
+
+__global__ __launch_bounds__(256) void emb_zero_kernel(uint4 *p16, long long n16, uint8_t *tail, int ntail) {
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n16; i += gridDim.x * 256ll) p16[i] = make_uint4(0, 0, 0, 0);
+    if (blockIdx.x == 0 && (int)threadIdx.x < ntail) tail[threadIdx.x] = 0;
+}
+
+constexpr int kMaxLevels = 8;
+struct EmbGeom {
+    long long n;
+    int blocks, passes, chunk, levels;
+    long long entries[kMaxLevels + 1];    // of each level; level 0 = n
+};
+
+static EmbGeom emb_geom(long long n, long long vocab) {
+    EmbGeom G;
+    memset(&G, 0, sizeof(G));
+    G.n = n;
+    G.blocks = (int)((n + kSortTile - 1) / kSortTile);
+    int bits = 1;
+    while (bits < 32 && (1ll << bits) <= vocab) ++bits;      // keys 0 .. vocab
+    G.passes = (bits + 7) / 8;
+    // long chunks leave fewer ends to sum again, short ones keep the chip busy when there are few rows
+    G.chunk = n >= (1 << 20) ? 64 : (n >= (1 << 17) ? 32 : 16);
+    G.entries[0] = n;
+    G.levels = 1;
+    while ((G.entries[G.levels - 1] + G.chunk - 1) / G.chunk > 1) {
+        G.entries[G.levels] = 2 * ((G.entries[G.levels - 1] + G.chunk - 1) / G.chunk);
+        ++G.levels;
+    }
+    return G;
+}
+
+static int emb_check(int32_t dtype, int64_t n, int64_t vocab, int64_t dim) {
+    GATMI_REQUIRE(dtype >= GATMI_F32 && dtype <= GATMI_F16, "embedding: unknown element type %d", dtype);
+    GATMI_REQUIRE(n >= 0 && n < (1ll << 31) && vocab >= 0 && vocab < (1ll << 31) && dim >= 1 && dim <= 65536,
+                  "embedding: %lld ids, %lld rows of %lld out of range", (long long)n, (long long)vocab, (long long)dim);
+    return GATMI_OK;
+}
+
+static int emb_lanes(int v, int64_t dim) {
+    const long long nv = (dim + v - 1) / v;
+    return nv >= 64 ? 64 : next_pow2((int)nv);
+}
+
+}  // namespace gatmi
+
+using namespace gatmi;
+
+extern "C" int gatmi_embedding_fwd(int32_t dtype, int64_t n, int64_t vocab, int64_t dim, float scale,
+                                   const int64_t *ids, const void *table, void *y, void *stream) {
+    if (int e = emb_check(dtype, n, vocab, dim)) return e;
+    if (n == 0) return GATMI_OK;
+    GATMI_REQUIRE(ids && (table || vocab == 0) && y, "embedding_fwd: null argument");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int v = vec_of(dtype, dim);
+    EmbArgs A{ids, table, y, n, vocab, (int)dim, emb_lanes(v, dim), 0, scale};
+    A.w_log = ilog2(A.W);
+    const long long per = (256 >> A.w_log) * kEmbUnroll;
+    ProfScope ps("embedding_fwd", st);
+    GATMI_WITH_TYPE(dtype, with_vec<T>(v, [&](auto V) {
+        hipLaunchKernelGGL((emb_fwd_kernel<T, decltype(V)::value>), dim3((unsigned)((n + per - 1) / per)), dim3(256), 0,
+                           st, A);
+    }));
+    GATMI_HIP(hipGetLastError());
+    return GATMI_OK;
+}
+
+struct EmbWs {
+    uint32_t *key[2], *pos[2], *hist, *total;
+    uint32_t *lkey[2], *lflag[2];
+    float *lsrc[2];
+    size_t bytes;
+};
+static EmbWs emb_carve(const EmbGeom &G, long long dim, void *ws) {
+    Carver cv(ws);
+    EmbWs w;
+    for (int i = 0; i < 2; ++i) {
+        w.key[i] = cv.take<uint32_t>(G.n);
+        w.pos[i] = cv.take<uint32_t>(G.n);
+    }
+    w.hist = cv.take<uint32_t>(256ll * G.blocks);
+    w.total = cv.take<uint32_t>(256);
+    for (int i = 0; i < 2; ++i) {        // levels 1, 3, .. and 2, 4, ..
+        const long long m = G.levels > 1 + i ? G.entries[1 + i] : 0;
+        w.lkey[i] = cv.take<uint32_t>(m);
+        w.lflag[i] = cv.take<uint32_t>(m);
+        w.lsrc[i] = cv.take<float>(m * dim);
+    }
+    w.bytes = cv.off + 256;
+    return w;
+}
+
+extern "C" size_t gatmi_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t dim) {
+    if (emb_check(GATMI_F32, n, vocab, dim)) return 0;
+    return emb_carve(emb_geom(n, vocab), dim, nullptr).bytes;
+}
+
+extern "C" int gatmi_embedding_bwd(int32_t dtype, int64_t n, int64_t vocab, int64_t dim, float scale,
+                                   const int64_t *ids, const void *grad_y, void *grad_table, void *ws,
+                                   size_t ws_bytes, void *stream) {
+    if (int e = emb_check(dtype, n, vocab, dim)) return e;
+    if (vocab == 0) return GATMI_OK;
+    GATMI_REQUIRE(grad_table && (n == 0 || (ids && grad_y)), "embedding_bwd: null argument");
+    const EmbGeom G = emb_geom(n, vocab);
+    const EmbWs w = emb_carve(G, dim, ws);
+    if (ws_bytes < w.bytes || !ws) {
+        set_error("embedding workspace too small: %zu < %zu", ws_bytes, w.bytes);
+        return GATMI_ERR_WS;
+    }
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    {   // every row, then the rows that have ids
+        ProfScope ps("embedding_zero", st);
+        const long long bytes = vocab * dim * (dtype == GATMI_F32 ? 4 : 2);
+        char *p = static_cast<char *>(grad_table);
+        const long long lead = (16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15;
+        // the aligned middle in 16-byte stores; the few bytes around it one by one
+        const long long head = lead < bytes ? lead : bytes, n16 = (bytes - head) / 16, rest = bytes - head - n16 * 16;
+        const long long b = (n16 + 1023) / 1024;
+        hipLaunchKernelGGL(emb_zero_kernel, dim3((unsigned)(b < 1 ? 1 : (b > 8192 ? 8192 : b))), dim3(256), 0, st,
+                           reinterpret_cast<uint4 *>(p + head), n16, reinterpret_cast<uint8_t *>(p + head + n16 * 16),
+                           (int)rest);
+        if (head)
+            hipLaunchKernelGGL(emb_zero_kernel, dim3(1), dim3(256), 0, st, nullptr, 0ll,
+                               reinterpret_cast<uint8_t *>(p), (int)head);
+        GATMI_HIP(hipGetLastError());
+    }
+    if (n == 0) return GATMI_OK;
+    {
+        ProfScope ps("embedding_sort", st);
+        SortArgs S;
+        memset(&S, 0, sizeof(S));
+        S.n = n;
+        S.vocab = vocab;
+        S.blocks = G.blocks;
+        S.hist = w.hist;
+        S.total = w.total;
+        for (int p = 0; p < G.passes; ++p) {
+            S.ids = p == 0 ? ids : nullptr;
+            S.key_in = w.key[(p + 1) & 1];
+            S.pos_in = w.pos[(p + 1) & 1];
+            S.key_out = w.key[p & 1];
+            S.pos_out = w.pos[p & 1];
+            S.shift = 8 * p;
+            hipLaunchKernelGGL(sort_count_kernel, dim3(G.blocks), dim3(256), 0, st, S);
+            hipLaunchKernelGGL(sort_scan_kernel, dim3(256), dim3(256), 0, st, S);
+            hipLaunchKernelGGL(sort_scatter_kernel, dim3(G.blocks), dim3(256), 0, st, S);
+        }
+        GATMI_HIP(hipGetLastError());
+    }
+    ProfScope ps("embedding_sum", st);
+    const int last = (G.passes - 1) & 1;
+    SegArgs A;
+    memset(&A, 0, sizeof(A));
+    A.vocab = (uint32_t)vocab;
+    A.dim = (int)dim;
+    A.chunk = G.chunk;
+    A.scale = scale;
+    A.out = grad_table;
+    for (int l = 0; l < G.levels; ++l) {
+        A.n = G.entries[l];
+        A.key = l == 0 ? w.key[last] : w.lkey[(l - 1) & 1];
+        A.pos = w.pos[last];
+        A.flag = l == 0 ? nullptr : w.lflag[(l - 1) & 1];
+        A.src = l == 0 ? grad_y : w.lsrc[(l - 1) & 1];
+        const bool more = l + 1 < G.levels;
+        A.nkey = more ? w.lkey[l & 1] : nullptr;
+        A.nflag = w.lflag[l & 1];
+        A.nsrc = w.lsrc[l & 1];
+        // f32 partial rows take vectors of their own width
+        const int v = l == 0 ? vec_of(dtype, dim) : vec_of(GATMI_F32, dim);
+        A.W = emb_lanes(v, dim);
+        A.w_log = ilog2(A.W);
+        const long long chunks = (A.n + A.chunk - 1) / A.chunk, per = 256 >> A.w_log;
+        const dim3 grid((unsigned)((chunks + per - 1) / per), (unsigned)((dim + (long long)A.W * v - 1) / ((long long)A.W * v)));
+        GATMI_WITH_TYPE(dtype, {
+            if (l == 0)
+                with_vec<T>(v, [&](auto V) {
+                    hipLaunchKernelGGL((seg_sum_kernel<T, T, decltype(V)::value, true>), grid, dim3(256), 0, st, A);
+                });
+            else
+                with_vec<float>(v, [&](auto V) {
+                    hipLaunchKernelGGL((seg_sum_kernel<T, float, decltype(V)::value, false>), grid, dim3(256), 0, st, A);
+                });
+        });
+        GATMI_HIP(hipGetLastError());
+    }
+    return GATMI_OK;
+}

@@ -451,6 +451,84 @@ int gatmi_knn_graph(const double *x, int64_t n, int32_t f, int32_t k, int64_t *e
 int gatmi_knn_graph_ties(const double *x, int64_t n, int32_t f, int32_t k, int64_t *edge_index,
                          uint8_t *tie_flags, void *ws, size_t ws_bytes, void *stream);
 
+/* ---- Dense operators around a layer (no counterpart in the reference, which has stock torch modules
+ * there): a linear layer with its epilogue, group normalisation with an activation, embedding lookup,
+ * dropout -- each with its gradient.  Tensors are contiguous and all of one element type; they may start
+ * at any address that is a multiple of an element.  Products, sums and statistics are f32 or wider, every
+ * result is rounded once, and no sum is made with float atomics: the same inputs give the same bits.
+ * All calls only launch kernels on `stream` (capturable in a HIP graph). */
+#define GATMI_F32 0
+#define GATMI_BF16 1
+#define GATMI_F16 2
+
+#define GATMI_ACT_NONE 0
+#define GATMI_ACT_RELU 1
+#define GATMI_ACT_ELU 2    /* alpha = 1 */
+#define GATMI_ACT_SILU 3
+#define GATMI_ACT_GELU 4   /* the exact form, by erf */
+
+/* y = act(x W^T + b) + residual.  f32 tensors multiply on the bf16 matrix cores as three exact bf16 pieces
+ * each, at f32 accuracy (csrc/linear.hip). */
+typedef struct gatmi_linear {
+    int64_t rows;          /* < 2^31 */
+    int32_t in_features;   /* 1 .. 65536 */
+    int32_t out_features;  /* 1 .. 65536 */
+    int32_t dtype;         /* GATMI_F32 / _BF16 / _F16 */
+    int32_t act;           /* GATMI_ACT_* */
+} gatmi_linear;
+/*   x [rows, in], weight [out, in], bias [out] or NULL, residual [rows, out] or NULL -> y [rows, out]
+ *   slope: NULL, or (act != NONE, a backward follows) the activation's derivative [rows, out]: float for
+ *   f32 tensors, else uint16 of a private coding */
+int gatmi_linear_fwd(const gatmi_linear *l, const void *x, const void *weight, const void *bias,
+                     const void *residual, void *y, void *slope, void *stream);
+/*   slope: what the forward wrote (NULL when act == NONE);  grad_y [rows, out]
+ *   -> grad_x [rows, in], grad_weight [out, in], grad_bias [out], each NULL to skip.  The residual's
+ *   gradient is grad_y itself. */
+size_t gatmi_linear_bwd_workspace_bytes(const gatmi_linear *l);
+int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void *weight, const void *slope,
+                     const void *grad_y, void *grad_x, void *grad_weight, void *grad_bias, void *ws,
+                     size_t ws_bytes, void *stream);
+
+/* y = act(group_norm(x)), channels last: x [batch, length, groups * width]; mean and (biased) variance over
+ * the length * width values of a sample's group; weight, bias [groups * width].  length = 1: one row per
+ * sample, e.g. a node's channels normalised head by head. */
+#define GATMI_GROUP_NORM_MAX_CHANNELS 8192
+typedef struct gatmi_group_norm {
+    int64_t batch;         /* < 2^31; at most 65535 when length > 1 or width > 2048 (f32) / 4096 */
+    int64_t length;        /* 1 .. 2^31 - 1 */
+    int32_t groups, width;
+    int32_t dtype, act;
+    float eps;
+    int32_t _pad;
+    const void *weight, *bias;
+} gatmi_group_norm;
+size_t gatmi_group_norm_workspace_bytes(const gatmi_group_norm *g);
+/*   mean, rstd: float [batch, groups], for the backward (both NULL: not saved; length = 1 only) */
+int gatmi_group_norm_fwd(const gatmi_group_norm *g, const void *x, void *y, float *mean, float *rstd,
+                         void *ws, size_t ws_bytes, void *stream);
+int gatmi_group_norm_bwd(const gatmi_group_norm *g, const void *x, const void *grad_y, const float *mean,
+                         const float *rstd, void *grad_x, void *grad_weight, void *grad_bias, void *ws,
+                         size_t ws_bytes, void *stream);
+
+/* y[i, :] = scale * table[ids[i], :], a zero row where ids[i] is outside [0, vocab) (which takes no
+ * gradient).  n, vocab < 2^31, dim <= 65536.  The gradient is summed over the ids sorted by value, in the
+ * order of i. */
+int gatmi_embedding_fwd(int32_t dtype, int64_t n, int64_t vocab, int64_t dim, float scale,
+                        const int64_t *ids, const void *table, void *y, void *stream);
+size_t gatmi_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t dim);
+/*   grad_y [n, dim] -> grad_table [vocab, dim], every row written */
+int gatmi_embedding_bwd(int32_t dtype, int64_t n, int64_t vocab, int64_t dim, float scale,
+                        const int64_t *ids, const void *grad_y, void *grad_table, void *ws, size_t ws_bytes,
+                        void *stream);
+
+/* y = keep(seed, row, column) ? x / (1 - p) : 0, + residual (NULL: none); keep is the mask gatmi_glue_mask
+ * writes out for the same seed and p.  The gradient with respect to x is the same call on grad_y without a
+ * residual.  seed_on_device != NULL: the seed is read from there.  seed_used != NULL receives the seed, for a
+ * backward that must not see the caller's seed move on.  rows < 2^32, cols < 2^31. */
+int gatmi_dropout(int32_t dtype, int64_t rows, int64_t cols, float dropout_p, uint64_t seed,
+                  const uint64_t *seed_on_device, uint64_t *seed_used, const void *x, const void *residual,
+                  void *y, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
