@@ -153,8 +153,9 @@ SYMBOLS = {
                                  C.c_void_p, C.c_size_t, C.c_void_p]),
     "gatmi_tail_bwd": (C.c_int, [C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                  C.c_void_p, C.c_void_p, C.c_void_p]),
+    "gatmi_linear_fwd_workspace_bytes": (C.c_size_t, [C.POINTER(Linear)]),
     "gatmi_linear_fwd": (C.c_int, [C.POINTER(Linear), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
-                                   C.c_void_p, C.c_void_p, C.c_void_p]),
+                                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "gatmi_linear_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(Linear)]),
     "gatmi_linear_bwd": (C.c_int, [C.POINTER(Linear), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),

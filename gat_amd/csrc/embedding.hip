@@ -59,133 +59,212 @@ template <class T, int V> __global__ __launch_bounds__(256) void emb_fwd_kernel(
     }
 }
 
-// ---- stable radix sort of (id, position), 8 bits a pass -----------------------------------------
-// A block owns kSortTile consecutive items; wave w of it the items [w * 64 * kSortItems, ..), 64 at a time.
-constexpr int kSortItems = 16, kSortTile = 256 * kSortItems;
+// ---- stable radix sort of (id, position) ---------------------------------------------------------
+// `bits` (at most 11) of the key a pass, so that up to 4 M table entries take two passes.  A block owns a
+// tile of 256 * ITEMS consecutive items; wave w of it the items [w * 64 * ITEMS, ..), 64 at a time: an
+// item's rank is what came before it in (tile, wave, step, lane) order, which is the order of the items.
+constexpr int kSortMaxBits = 11, kSmallSort = 4096;
 
 struct SortArgs {
     const int64_t *ids;            // first pass: keys come from here, positions are the indices
     const uint32_t *key_in, *pos_in;
     uint32_t *key_out, *pos_out;
-    uint32_t *hist;                // [256][blocks]
-    uint32_t *total;               // [256]
+    uint32_t *hist;                // [bins][blocks]
+    uint32_t *total;               // [bins]
     long long n, vocab;
-    int blocks, shift;
+    int blocks, shift, bits, passes;
 };
 
 // ids outside the table get the key `vocab`: they sort behind every row and are left out of the sums
+__device__ __forceinline__ uint32_t id_key(int64_t id, long long vocab) {
+    return (uint32_t)(id >= 0 && id < vocab ? id : vocab);
+}
 __device__ __forceinline__ uint32_t sort_key(const SortArgs &A, long long i) {
-    if (A.ids) {
-        const long long id = A.ids[i];
-        return (uint32_t)(id >= 0 && id < A.vocab ? id : A.vocab);
-    }
-    return A.key_in[i];
+    return A.ids ? id_key(A.ids[i], A.vocab) : A.key_in[i];
 }
 
 // Lanes of this wave whose digit equals this lane's (only lanes with `on` count)
-__device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool on) {
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool on) {
     uint64_t m = __ballot(on);
-#pragma unroll
-    for (int b = 0; b < 8; ++b) {
+    for (int b = 0; b < bits; ++b) {
         const uint64_t bit = __ballot((digit >> b) & 1u);
         m &= (digit >> b) & 1u ? bit : ~bit;
     }
     return m;
 }
 
-__global__ __launch_bounds__(256) void sort_count_kernel(const SortArgs A) {
-    __shared__ uint32_t h[256];
-    h[threadIdx.x] = 0;
+// Ranks this wave's items among the wave's equal digits: rank[k], and the wave's counts in `cnt` [bins],
+// zero before.  volatile: lanes read each other's counts; a wave's LDS accesses are in order.
+template <int ITEMS>
+__device__ __forceinline__ void wave_ranks(volatile uint32_t *cnt, const uint32_t (&digit)[ITEMS], int have, int bits,
+                                           int lane, uint32_t (&rank)[ITEMS]) {
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const bool on = k * 64 + lane < have;
+        const uint64_t m = same_digit(digit[k], bits, on);
+        const uint32_t before = __popcll(m & ((1ull << lane) - 1ull));
+        const uint32_t seen = on ? cnt[digit[k]] : 0u;
+        rank[k] = seen + before;
+        if (on && before == 0) cnt[digit[k]] = seen + (uint32_t)__popcll(m);
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// Exclusive scan over the block's 256 threads
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *wsum, uint32_t *all = nullptr) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint32_t s = v;
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t up = __shfl_up(s, o, 64);
+        if (lane >= o) s += up;
+    }
+    if (lane == 63) wsum[wave] = s;
     __syncthreads();
-    const long long base = (long long)blockIdx.x * kSortTile;
-#pragma unroll 4
-    for (int k = 0; k < kSortItems; ++k) {
+    uint32_t before = 0;
+    for (int w = 0; w < wave; ++w) before += wsum[w];
+    if (all) *all = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+    __syncthreads();
+    return before + s - v;
+}
+
+template <int ITEMS> __global__ __launch_bounds__(256) void sort_count_kernel(const SortArgs A) {
+    extern __shared__ uint32_t h[];
+    const int bins = 1 << A.bits;
+    for (int d = threadIdx.x; d < bins; d += 256) h[d] = 0;
+    __syncthreads();
+    const long long base = (long long)blockIdx.x * (256 * ITEMS);
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
         const long long i = base + k * 256 + threadIdx.x;
-        if (i < A.n) atomicAdd(&h[(sort_key(A, i) >> A.shift) & 255u], 1u);   // integers: any order
+        if (i < A.n) atomicAdd(&h[(sort_key(A, i) >> A.shift) & (bins - 1)], 1u);   // integers: any order
     }
     __syncthreads();
-    A.hist[(long long)threadIdx.x * A.blocks + blockIdx.x] = h[threadIdx.x];
+    for (int d = threadIdx.x; d < bins; d += 256) A.hist[(long long)d * A.blocks + blockIdx.x] = h[d];
 }
 
 // block d: exclusive scan of digit d's counts over the tiles; total[d]
 __global__ __launch_bounds__(256) void sort_scan_kernel(const SortArgs A) {
     __shared__ uint32_t wsum[4];
     uint32_t *row = A.hist + (long long)blockIdx.x * A.blocks;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t carry = 0;
     for (int base = 0; base < A.blocks; base += 256) {
         const int i = base + threadIdx.x;
         const uint32_t v = i < A.blocks ? row[i] : 0;
-        uint32_t s = v;
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t up = __shfl_up(s, o, 64);
-            if (lane >= o) s += up;
-        }
-        if (lane == 63) wsum[wave] = s;
-        __syncthreads();
-        uint32_t before = carry;
-        for (int w = 0; w < wave; ++w) before += wsum[w];
-        const uint32_t all = wsum[0] + wsum[1] + wsum[2] + wsum[3];
-        if (i < A.blocks) row[i] = before + s - v;
+        uint32_t all;
+        const uint32_t before = block_scan(v, wsum, &all);
+        if (i < A.blocks) row[i] = carry + before;
         carry += all;
-        __syncthreads();
     }
     if (threadIdx.x == 0) A.total[blockIdx.x] = carry;
 }
 
-__global__ __launch_bounds__(256) void sort_scatter_kernel(const SortArgs A) {
-    // per wave and digit: items seen; then where they start.  volatile: lanes of a wave read each other's counts
-    __shared__ volatile uint32_t cnt[4][256];
+// thread t owns the bins / 256 digits from t * that on (bins < 256: one each): turns the counts of
+// the tile's four waves in cnt [4][bins] into where their items start, `start(d)` being the digit's first
+// place for this tile and `total(d)` its items in all
+template <class S, class C>
+__device__ __forceinline__ void digit_starts(volatile uint32_t *cnt, int bins, uint32_t *wsum, S place, C total) {
+    const int per = bins > 256 ? bins / 256 : 1;
+    const int d0 = threadIdx.x * per;
+    uint32_t sum = 0;
+    for (int q = 0; q < per; ++q)
+        if (d0 + q < bins) sum += total(d0 + q);
+    uint32_t at = block_scan(sum, wsum);
+    for (int q = 0; q < per; ++q) {
+        const int d = d0 + q;
+        if (d >= bins) break;
+        uint32_t to = at + place(d);
+        at += total(d);
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t c = cnt[w * bins + d];
+            cnt[w * bins + d] = to;
+            to += c;
+        }
+    }
+}
+
+template <int ITEMS> __global__ __launch_bounds__(256) void sort_scatter_kernel(const SortArgs A) {
+    extern __shared__ uint32_t smem[];
+    __shared__ uint32_t wsum[4];
+    volatile uint32_t *cnt = smem;       // [4][bins]
+    const int bins = 1 << A.bits;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int w = 0; w < 4; ++w) cnt[w][threadIdx.x] = 0;
+    for (int d = threadIdx.x; d < 4 * bins; d += 256) cnt[d] = 0;
     __syncthreads();
-    const long long base = (long long)blockIdx.x * kSortTile + (long long)wave * (64 * kSortItems) + lane;
-    uint32_t key[kSortItems], pos[kSortItems], rank[kSortItems];
+    const long long base = (long long)blockIdx.x * (256 * ITEMS) + wave * (64 * ITEMS);
+    const long long left = A.n - base;
+    const int have = left < 0 ? 0 : (left < 64 * ITEMS ? (int)left : 64 * ITEMS);
+    uint32_t key[ITEMS], pos[ITEMS], digit[ITEMS], rank[ITEMS];
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
-        const long long i = base + k * 64;
-        const bool on = i < A.n;
+    for (int k = 0; k < ITEMS; ++k) {
+        const long long i = base + k * 64 + lane;
+        const bool on = k * 64 + lane < have;
         key[k] = on ? sort_key(A, i) : 0u;
         pos[k] = on ? (A.ids ? (uint32_t)i : A.pos_in[i]) : 0u;
+        digit[k] = (key[k] >> A.shift) & (bins - 1);
     }
-#pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
-        const bool on = base + k * 64 < A.n;
-        const uint32_t digit = (key[k] >> A.shift) & 255u;
-        const uint64_t m = same_digit(digit, on);
-        const uint32_t before = __popcll(m & ((1ull << lane) - 1ull));
-        // only this wave touches its row of counts; its lanes' LDS accesses are in order
-        const uint32_t seen = on ? cnt[wave][digit] : 0u;
-        rank[k] = seen + before;
-        if (on && before == 0) cnt[wave][digit] = seen + (uint32_t)__popcll(m);
-        __builtin_amdgcn_wave_barrier();
-    }
+    wave_ranks<ITEMS>(cnt + wave * bins, digit, have, A.bits, lane, rank);
     __syncthreads();
-    {   // thread d: where digit d starts in the output, then each wave's share of this tile
-        __shared__ uint32_t wsum[4];
-        const uint32_t t = A.total[threadIdx.x];
-        uint32_t s = t;
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t up = __shfl_up(s, o, 64);
-            if (lane >= o) s += up;
-        }
-        if (lane == 63) wsum[wave] = s;
-        __syncthreads();
-        uint32_t at = s - t + A.hist[(long long)threadIdx.x * A.blocks + blockIdx.x];
-        for (int w = 0; w < wave; ++w) at += wsum[w];
-        for (int w = 0; w < 4; ++w) {
-            const uint32_t c = cnt[w][threadIdx.x];
-            cnt[w][threadIdx.x] = at;
-            at += c;
-        }
-    }
+    digit_starts(cnt, bins, wsum, [&](int d) { return A.hist[(long long)d * A.blocks + blockIdx.x]; },
+                 [&](int d) { return A.total[d]; });
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k)
-        if (base + k * 64 < A.n) {
-            const uint32_t to = cnt[wave][(key[k] >> A.shift) & 255u] + rank[k];
+    for (int k = 0; k < ITEMS; ++k)
+        if (k * 64 + lane < have) {
+            const uint32_t to = cnt[wave * bins + digit[k]] + rank[k];
             A.key_out[to] = key[k];
             A.pos_out[to] = pos[k];
+        }
+}
+
+// at most kSmallSort items: all passes in one block, through LDS
+__global__ __launch_bounds__(256) void sort_small_kernel(const SortArgs A) {
+    constexpr int ITEMS = kSmallSort / 256;
+    __shared__ uint32_t skey[kSmallSort], spos[kSmallSort], scnt[4 * 256], wsum[4];
+    volatile uint32_t *cnt = scnt;
+    constexpr int bins = 256;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = (int)A.n;
+    const int base = wave * (64 * ITEMS);
+    const int have = n - base < 0 ? 0 : (n - base < 64 * ITEMS ? n - base : 64 * ITEMS);
+    uint32_t key[ITEMS], pos[ITEMS], digit[ITEMS], rank[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const int i = base + k * 64 + lane;
+        const bool on = k * 64 + lane < have;
+        key[k] = on ? id_key(A.ids[i], A.vocab) : 0u;
+        pos[k] = (uint32_t)i;
+    }
+    for (int p = 0; p < A.passes; ++p) {
+        for (int d = threadIdx.x; d < 4 * bins; d += 256) cnt[d] = 0;
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k) digit[k] = (key[k] >> (8 * p)) & (bins - 1);
+        __syncthreads();
+        wave_ranks<ITEMS>(cnt + wave * bins, digit, have, 8, lane, rank);
+        __syncthreads();
+        uint32_t mine = 0;      // thread d: the tile is all there is, its counts are the totals
+        for (int w = 0; w < 4; ++w) mine += cnt[w * bins + threadIdx.x];
+        digit_starts(cnt, bins, wsum, [&](int) { return 0u; }, [&](int) { return mine; });
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k)
+            if (k * 64 + lane < have) {
+                const uint32_t to = cnt[wave * bins + digit[k]] + rank[k];
+                skey[to] = key[k];
+                spos[to] = pos[k];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < ITEMS; ++k)
+            if (k * 64 + lane < have) {
+                key[k] = skey[base + k * 64 + lane];
+                pos[k] = spos[base + k * 64 + lane];
+            }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+        if (k * 64 + lane < have) {
+            A.key_out[base + k * 64 + lane] = key[k];
+            A.pos_out[base + k * 64 + lane] = pos[k];
         }
 }
 
@@ -231,23 +310,29 @@ __global__ __launch_bounds__(256) void seg_sum_kernel(const SegArgs A) {
     for (int k = 0; k < V; ++k) acc.e[k] = 0.f;
     uint32_t cur = head;
     bool first = true;      // the chunk's first segment
+    // Every entry names a row that exists, so rows are loaded without a test (past the end: the last entry
+    // again) and the keys and positions of the next batch travel while this one's rows do.
     constexpr int U = 8;
+    uint32_t kk[U], pp[U], kn[U], pn[U];
+    auto entries = [&](long long e, uint32_t (&k_)[U], uint32_t (&p_)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long i = e + u < e1 ? e + u : e1 - 1;
+            k_[u] = A.key[i];
+            p_[u] = LEAF ? A.pos[i] : A.flag[i];
+        }
+    };
+    entries(e0, kn, pn);
     for (long long e = e0; e < e1; e += U) {
-        uint32_t kk[U];
         VecF<V> v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const bool in = e + u < e1;
-            kk[u] = in ? A.key[e + u] : kNoKey;
-            const bool row = in && kk[u] < A.vocab && (LEAF || A.flag[e + u]);
-            if (row) {
-                const long long r = LEAF ? (long long)A.pos[e + u] : e + u;
-                v[u] = ldv<S, V>(src + r * A.dim);
-            } else {
-#pragma unroll
-                for (int k = 0; k < V; ++k) v[u].e[k] = 0.f;
-            }
+            kk[u] = kn[u];
+            pp[u] = pn[u];
+            const long long r = LEAF ? (long long)pp[u] : (e + u < e1 ? e + u : e1 - 1);
+            v[u] = ldv<S, V>(src + r * A.dim);
         }
+        entries(e + U, kn, pn);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (e + u >= e1) break;
@@ -268,8 +353,9 @@ __global__ __launch_bounds__(256) void seg_sum_kernel(const SegArgs A) {
 #pragma unroll
                 for (int k = 0; k < V; ++k) acc.e[k] = 0.f;
             }
+            if (LEAF || pp[u])        // a node entry without a row holds nothing that was written
 #pragma unroll
-            for (int k = 0; k < V; ++k) acc.e[k] += v[u].e[k];
+                for (int k = 0; k < V; ++k) acc.e[k] += v[u].e[k];
         }
     }
     if (cur < A.vocab) {
@@ -301,10 +387,10 @@ __global__ __launch_bounds__(256) void emb_zero_kernel(uint4 *p16, long long n16
     if (blockIdx.x == 0 && (int)threadIdx.x < ntail) tail[threadIdx.x] = 0;
 }
 
-constexpr int kMaxLevels = 8;
+constexpr int kMaxLevels = 10;
 struct EmbGeom {
     long long n;
-    int blocks, passes, chunk, levels;
+    int blocks, passes, bits, items, chunk0, chunk, levels;
     long long entries[kMaxLevels + 1];    // of each level; level 0 = n
 };
 
@@ -312,16 +398,21 @@ static EmbGeom emb_geom(long long n, long long vocab) {
     EmbGeom G;
     memset(&G, 0, sizeof(G));
     G.n = n;
-    G.blocks = (int)((n + kSortTile - 1) / kSortTile);
     int bits = 1;
     while (bits < 32 && (1ll << bits) <= vocab) ++bits;      // keys 0 .. vocab
-    G.passes = (bits + 7) / 8;
+    const bool small = n <= kSmallSort;
+    G.passes = small ? (bits + 7) / 8 : (bits + kSortMaxBits - 1) / kSortMaxBits;
+    G.bits = small ? 8 : (bits + G.passes - 1) / G.passes;
+    // tiles of 4096 items, of 1024 where those would leave compute units idle
+    G.items = n >= (1 << 20) ? 16 : 4;
+    G.blocks = (int)((n + 256ll * G.items - 1) / (256ll * G.items));
     // long chunks leave fewer ends to sum again, short ones keep the chip busy when there are few rows
-    G.chunk = n >= (1 << 20) ? 64 : (n >= (1 << 17) ? 32 : 16);
+    G.chunk0 = n >= (1 << 20) ? 64 : (n >= (1 << 17) ? 32 : 16);
+    G.chunk = 32;
     G.entries[0] = n;
     G.levels = 1;
-    while ((G.entries[G.levels - 1] + G.chunk - 1) / G.chunk > 1) {
-        G.entries[G.levels] = 2 * ((G.entries[G.levels - 1] + G.chunk - 1) / G.chunk);
+    for (long long c = (n + G.chunk0 - 1) / G.chunk0; c > 1; c = (2 * c + G.chunk - 1) / G.chunk) {
+        G.entries[G.levels] = 2 * c;
         ++G.levels;
     }
     return G;
@@ -375,8 +466,8 @@ static EmbWs emb_carve(const EmbGeom &G, long long dim, void *ws) {
         w.key[i] = cv.take<uint32_t>(G.n);
         w.pos[i] = cv.take<uint32_t>(G.n);
     }
-    w.hist = cv.take<uint32_t>(256ll * G.blocks);
-    w.total = cv.take<uint32_t>(256);
+    w.hist = cv.take<uint32_t>((1ll << G.bits) * G.blocks);
+    w.total = cv.take<uint32_t>(1ll << G.bits);
     for (int i = 0; i < 2; ++i) {        // levels 1, 3, .. and 2, 4, ..
         const long long m = G.levels > 1 + i ? G.entries[1 + i] : 0;
         w.lkey[i] = cv.take<uint32_t>(m);
@@ -431,16 +522,27 @@ extern "C" int gatmi_embedding_bwd(int32_t dtype, int64_t n, int64_t vocab, int6
         S.blocks = G.blocks;
         S.hist = w.hist;
         S.total = w.total;
-        for (int p = 0; p < G.passes; ++p) {
+        S.bits = G.bits;
+        S.passes = G.passes;
+        if (n <= kSmallSort) {
+            S.ids = ids;
+            S.key_out = w.key[(G.passes - 1) & 1];
+            S.pos_out = w.pos[(G.passes - 1) & 1];
+            hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(256), 0, st, S);
+        }
+        for (int p = 0; n > kSmallSort && p < G.passes; ++p) {
+            const size_t bins = (size_t)1 << G.bits;
             S.ids = p == 0 ? ids : nullptr;
             S.key_in = w.key[(p + 1) & 1];
             S.pos_in = w.pos[(p + 1) & 1];
             S.key_out = w.key[p & 1];
             S.pos_out = w.pos[p & 1];
-            S.shift = 8 * p;
-            hipLaunchKernelGGL(sort_count_kernel, dim3(G.blocks), dim3(256), 0, st, S);
-            hipLaunchKernelGGL(sort_scan_kernel, dim3(256), dim3(256), 0, st, S);
-            hipLaunchKernelGGL(sort_scatter_kernel, dim3(G.blocks), dim3(256), 0, st, S);
+            S.shift = G.bits * p;
+            auto count = G.items == 16 ? sort_count_kernel<16> : sort_count_kernel<4>;
+            auto scatter = G.items == 16 ? sort_scatter_kernel<16> : sort_scatter_kernel<4>;
+            hipLaunchKernelGGL(count, dim3(G.blocks), dim3(256), bins * 4, st, S);
+            hipLaunchKernelGGL(sort_scan_kernel, dim3((unsigned)bins), dim3(256), 0, st, S);
+            hipLaunchKernelGGL(scatter, dim3(G.blocks), dim3(256), bins * 16, st, S);
         }
         GATMI_HIP(hipGetLastError());
     }
@@ -450,11 +552,11 @@ extern "C" int gatmi_embedding_bwd(int32_t dtype, int64_t n, int64_t vocab, int6
     memset(&A, 0, sizeof(A));
     A.vocab = (uint32_t)vocab;
     A.dim = (int)dim;
-    A.chunk = G.chunk;
     A.scale = scale;
     A.out = grad_table;
     for (int l = 0; l < G.levels; ++l) {
         A.n = G.entries[l];
+        A.chunk = l == 0 ? G.chunk0 : G.chunk;
         A.key = l == 0 ? w.key[last] : w.lkey[(l - 1) & 1];
         A.pos = w.pos[last];
         A.flag = l == 0 ? nullptr : w.lflag[(l - 1) & 1];

@@ -19,7 +19,7 @@ namespace gatmi {
 
 constexpr int kGnMaxT = 8;         // vectors per lane of the segment kernels
 constexpr int kGnFwdBlocks = 4096, kGnBwdBlocks = 1024;
-constexpr int kGnChunks = 2048;    // blocks of the length > 1 form, over all samples
+constexpr int kGnChunks = 1536;    // blocks of the length > 1 form, over all samples
 constexpr int kGnSlabs = 64;       // row slabs of the column sums
 
 struct GnArgs {
@@ -248,7 +248,7 @@ template <class T, int V> __global__ __launch_bounds__(256) void gn_stats_kernel
 #pragma unroll
         for (int k = 0; k < V; ++k)
             if (k >= L.skip) {
-                p[k] = sh.e[k] + s1.e[k] / n;
+                p[k] = sh.e[k] + s1.e[k] / n;                  // a chunk without rows: zeros
                 p[A.C + k] = fmaxf(s2.e[k] - s1.e[k] * s1.e[k] / n, 0.f);
             }
     }
@@ -266,6 +266,22 @@ __device__ __forceinline__ double block_sum(double v, double *red) {
     return r;
 }
 
+// Threads of a block over a [chunks][width] array: thread -> (channel, first chunk); a block takes `step`
+// chunks at once, or several channels a thread when a group is wider than the block.
+struct GnWalk {
+    int j, c, step, jstep;
+};
+__device__ __forceinline__ GnWalk gn_walk(int width) {
+    GnWalk w;
+    const int lanes = width < 256 ? width : 256;
+    w.step = 256 / lanes;
+    w.j = threadIdx.x % lanes;
+    w.c = threadIdx.x / lanes;
+    w.jstep = lanes;
+    if (w.c >= w.step) w.j = width;      // left over: nothing
+    return w;
+}
+
 // one block per (group, sample): Chan over the group's channels and chunks, in double
 __global__ __launch_bounds__(256) void gn_finalize_kernel(const GnArgs A) {
     __shared__ double red[256];
@@ -276,24 +292,20 @@ __global__ __launch_bounds__(256) void gn_finalize_kernel(const GnArgs A) {
         const long long r0 = c * per, r1 = r0 + per < A.length ? r0 + per : A.length;
         return r1 > r0 ? (double)(r1 - r0) : 0.0;
     };
-    const int n = A.chunks * A.width;
+    const GnWalk w = gn_walk(A.width);
     double s = 0.0;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const int c = i / A.width, j = i - c * A.width;
-        const double m = rows(c);
-        if (m > 0.0) s += m * p[(long long)c * 2 * A.C + j];
-    }
+    for (int j = w.j; j < A.width; j += w.jstep)
+#pragma unroll 8
+        for (int c = w.c; c < A.chunks; c += w.step) s += rows(c) * p[(long long)c * 2 * A.C + j];
     const double count = (double)A.length * A.width;
     const double mean = block_sum(s, red) / count;
     s = 0.0;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const int c = i / A.width, j = i - c * A.width;
-        const double m = rows(c);
-        if (m > 0.0) {
+    for (int j = w.j; j < A.width; j += w.jstep)
+#pragma unroll 8
+        for (int c = w.c; c < A.chunks; c += w.step) {
             const double d = p[(long long)c * 2 * A.C + j] - mean;
-            s += p[(long long)c * 2 * A.C + A.C + j] + m * d * d;
+            s += p[(long long)c * 2 * A.C + A.C + j] + rows(c) * d * d;
         }
-    }
     const double var = block_sum(s, red) / count;
     if (threadIdx.x == 0) {
         A.mean[(long long)blockIdx.y * A.groups + g] = (float)mean;
@@ -387,13 +399,15 @@ template <class T> __global__ __launch_bounds__(256) void gn_coef_kernel(const G
     const int g = blockIdx.x;
     const float *p = A.part + (long long)blockIdx.y * A.chunks * 2 * A.C + g * A.width;
     const T *w = static_cast<const T *>(A.w) + g * A.width;
-    const int n = A.chunks * A.width;
+    const GnWalk k = gn_walk(A.width);
     double s1 = 0.0, s2 = 0.0;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const int c = i / A.width, j = i - c * A.width;
+    for (int j = k.j; j < A.width; j += k.jstep) {
         const double wj = (float)w[j];
-        s1 += wj * p[(long long)c * 2 * A.C + j];
-        s2 += wj * p[(long long)c * 2 * A.C + A.C + j];
+#pragma unroll 8
+        for (int c = k.c; c < A.chunks; c += k.step) {
+            s1 += wj * p[(long long)c * 2 * A.C + j];
+            s2 += wj * p[(long long)c * 2 * A.C + A.C + j];
+        }
     }
     const double count = (double)A.length * A.width;
     const double m1 = block_sum(s1, red) / count, m2 = block_sum(s2, red) / count;
@@ -445,6 +459,7 @@ __global__ __launch_bounds__(256) void colsum_slab_kernel(const float *in, long 
     const long long r0 = blockIdx.y * per, r1 = r0 + per < rows ? r0 + per : rows;
     float s = 0.f;
     if (c < cols)
+#pragma unroll 8
         for (long long r = r0 + rg; r < r1; r += 8) s += in[blockIdx.z * set + r * ld + c];
     red[threadIdx.x] = s;
     __syncthreads();
@@ -455,13 +470,19 @@ __global__ __launch_bounds__(256) void colsum_slab_kernel(const float *in, long 
 }
 template <class T>
 __global__ __launch_bounds__(256) void colsum_final_kernel(const float *slab, int nslab, int cols, T *out0, T *out1) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= 2 * cols) return;
-    const int k = i / cols, c = i - k * cols;
+    __shared__ double red[256];
+    const int i = blockIdx.x * 32 + (threadIdx.x & 31), rg = threadIdx.x >> 5;     // i over [2][cols]
     double s = 0.0;
-    for (int q = 0; q < nslab; ++q) s += slab[((long long)q * 2 + k) * cols + c];
-    T *o = k == 0 ? out0 : out1;
-    if (o) o[c] = (T)(float)s;
+    if (i < 2 * cols)
+#pragma unroll 8
+        for (int q = rg; q < nslab; q += 8) s += slab[(long long)q * 2 * cols + i];
+    red[threadIdx.x] = s;
+    __syncthreads();
+    if (rg == 0 && i < 2 * cols) {
+        for (int q = 1; q < 8; ++q) s += red[threadIdx.x + q * 32];
+        T *o = i < cols ? out0 + i : out1 + (i - cols);
+        *o = (T)(float)s;
+    }
 }
 
 // a group that fits the registers of one wave and is contiguous
@@ -687,7 +708,7 @@ extern "C" int gatmi_group_norm_bwd(const gatmi_group_norm *g, const void *x, co
     if (slabs > 0)
         hipLaunchKernelGGL(colsum_slab_kernel, dim3((C + 31) / 32, slabs, 2), dim3(256), 0, st, A.part, rows, ld, set,
                            C, slab);
-    GATMI_WITH_TYPE(g->dtype, hipLaunchKernelGGL((colsum_final_kernel<T>), dim3((2 * C + 255) / 256), dim3(256), 0, st,
+    GATMI_WITH_TYPE(g->dtype, hipLaunchKernelGGL((colsum_final_kernel<T>), dim3((2 * C + 31) / 32), dim3(256), 0, st,
                                                  slab, slabs, C, static_cast<T *>(out0), static_cast<T *>(out1)));
     GATMI_HIP(hipGetLastError());
     return GATMI_OK;

@@ -19,19 +19,15 @@ namespace gatmi {
 typedef __bf16 bf16x8v __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8v __attribute__((ext_vector_type(8)));
 typedef float f32x16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));   // 16 bytes from any element on
 
 // act'(z) in 16 bits: round(d * 2^15) + 2^13, i.e. [-0.25, 1.75); 65535 stands for NaN
 __device__ __forceinline__ uint16_t pack_slope(float d) {
     return d != d ? (uint16_t)65535 : (uint16_t)(int)rintf(fmaf(d, 32768.f, 8192.f));
 }
-__device__ __forceinline__ float unpack_slope(uint16_t q) {
-    return q == 65535 ? __uint_as_float(0x7fc00000u) : ((float)(int)q - 8192.f) * (1.0f / 32768.f);
-}
 template <class T> struct SlopeOf { typedef uint16_t type; };
 template <> struct SlopeOf<float> { typedef float type; };
-__device__ __forceinline__ float slope_in(float d) { return d; }
-__device__ __forceinline__ float slope_in(uint16_t d) { return unpack_slope(d); }
 template <class T> __device__ __forceinline__ typename SlopeOf<T>::type slope_out(float d) {
     if constexpr (IsF32<T>::value) return d;
     else return pack_slope(d);
@@ -41,40 +37,73 @@ template <class T> __device__ __forceinline__ typename SlopeOf<T>::type slope_ou
 template <class T> struct Mul;
 template <> struct Mul<bf16_t> {
     static constexpr int PIECES = 1, BK = 64;
-    static __device__ __forceinline__ f32x16v mma(uint4 a, uint4 b, f32x16v c) {
+    static __device__ __forceinline__ f32x16v mma(u32x4 a, u32x4 b, f32x16v c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8v, a), __builtin_bit_cast(bf16x8v, b), c, 0, 0, 0);
     }
 };
 template <> struct Mul<f16_t> {
     static constexpr int PIECES = 1, BK = 64;
-    static __device__ __forceinline__ f32x16v mma(uint4 a, uint4 b, f32x16v c) {
+    static __device__ __forceinline__ f32x16v mma(u32x4 a, u32x4 b, f32x16v c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8v, a), __builtin_bit_cast(f16x8v, b), c, 0, 0, 0);
     }
 };
 template <> struct Mul<float> {
     static constexpr int PIECES = 3, BK = 32;
-    static __device__ __forceinline__ f32x16v mma(uint4 a, uint4 b, f32x16v c) { return Mul<bf16_t>::mma(a, b, c); }
+    static __device__ __forceinline__ f32x16v mma(u32x4 a, u32x4 b, f32x16v c) { return Mul<bf16_t>::mma(a, b, c); }
 };
 
-// Eight consecutive elements of a row as they lie in memory; `left` of them exist, the rest read as zero
+// Eight consecutive elements of a row as they lie in memory.  The loads of the main loops have no branch
+// around them -- a load under a condition is waited for where the paths join, not where it is used -- so a
+// granule that would run over the end of its row starts at the row's last eight elements instead and `drop`
+// zeroes, on the way into LDS, the ones that belong to the granule before it.
 template <class T> struct Gran {
     uint32_t w[2 * sizeof(T)];
 };
-template <class T> __device__ __forceinline__ Gran<T> ld_gran(const T *p, int left) {
+template <class T> __device__ __forceinline__ Gran<T> ld_gran(const void *base, uint32_t bytes) {
     Gran<T> g;
-    if (left >= 8) {
+    const u32x4u *p = reinterpret_cast<const u32x4u *>(static_cast<const char *>(base) + bytes);
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-            const u32x4u v = reinterpret_cast<const u32x4u *>(p)[i];
-            g.w[4 * i] = v[0]; g.w[4 * i + 1] = v[1]; g.w[4 * i + 2] = v[2]; g.w[4 * i + 3] = v[3];
-        }
-    } else {
-        T e[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = i < left ? p[i] : (T)0.f;
-        __builtin_memcpy(g.w, e, sizeof(e));
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+        const u32x4u v = p[i];
+        g.w[4 * i] = v[0]; g.w[4 * i + 1] = v[1]; g.w[4 * i + 2] = v[2]; g.w[4 * i + 3] = v[3];
     }
     return g;
+}
+// rows of fewer than eight elements: `left` of them exist
+template <class T> __device__ __forceinline__ Gran<T> ld_gran_short(const void *base, uint32_t bytes, int left) {
+    Gran<T> g;
+    const T *p = reinterpret_cast<const T *>(static_cast<const char *>(base) + bytes);
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = i < left ? p[i] : (T)0.f;
+    __builtin_memcpy(g.w, e, sizeof(e));
+    return g;
+}
+template <class T> __device__ __forceinline__ void drop(Gran<T> &g, int first) {
+#pragma unroll
+    for (int i = 0; i < (int)(2 * sizeof(T)); ++i) {
+        if constexpr (sizeof(T) == 4) g.w[i] = i < first ? 0u : g.w[i];
+        else g.w[i] &= 2 * i + 1 < first ? 0u : (2 * i < first ? 0xffff0000u : 0xffffffffu);
+    }
+}
+
+// A granule that was loaded `over` elements early, moved to its place; zeros follow
+template <class T> __device__ __forceinline__ void shift_down(uint32_t (&w)[2 * sizeof(T)], int over) {
+    constexpr int W = 2 * sizeof(T);
+    if constexpr (sizeof(T) == 2)
+        if (over & 1)
+#pragma unroll
+            for (int i = 0; i < W; ++i) w[i] = (w[i] >> 16) | (i + 1 < W ? w[i + 1 < W ? i + 1 : i] << 16 : 0u);
+#pragma unroll
+    for (int b = sizeof(T) == 2 ? 2 : 1; b < 8; b <<= 1) {
+        const int by = sizeof(T) == 2 ? b / 2 : b;
+        if (over & b)
+#pragma unroll
+            for (int i = 0; i < W; ++i) w[i] = i + by < W ? w[i + by < W ? i + by : i] : 0u;
+    }
+    if (over >= 8)
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = 0u;
 }
 
 // (a, b) -> the pair's three bf16 pieces, low half first
@@ -99,7 +128,7 @@ template <class T, int R> struct Tile {
     }
     static __device__ __forceinline__ void put(char *lds, int row, int g, const Gran<T> &v) {
         if constexpr (P == 1) {
-            *reinterpret_cast<uint4 *>(lds + at(row, g)) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+            *reinterpret_cast<u32x4 *>(lds + at(row, g)) = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
         } else {
             uint32_t q[3][4];
 #pragma unroll
@@ -107,138 +136,319 @@ template <class T, int R> struct Tile {
                 cut3(__uint_as_float(v.w[2 * i]), __uint_as_float(v.w[2 * i + 1]), q[0][i], q[1][i], q[2][i]);
 #pragma unroll
             for (int p = 0; p < 3; ++p)
-                *reinterpret_cast<uint4 *>(lds + p * PLANE + at(row, g)) = make_uint4(q[p][0], q[p][1], q[p][2], q[p][3]);
+                *reinterpret_cast<u32x4 *>(lds + p * PLANE + at(row, g)) = u32x4{q[p][0], q[p][1], q[p][2], q[p][3]};
         }
     }
-    // two contraction steps (2m, 2m + 1) of eight rows row0 .. row0 + 7: the transposing store of dW
-    static __device__ __forceinline__ void put_pair(char *lds, int row0, int m2, const Gran<T> &lo, const Gran<T> &hi) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int a = at(row0 + i, m2 >> 2) + (m2 & 3) * 4;
-            if constexpr (P == 1) {
-                const uint32_t l = i & 1 ? lo.w[i / 2] >> 16 : lo.w[i / 2] & 0xffffu;
-                const uint32_t h = i & 1 ? hi.w[i / 2] & 0xffff0000u : hi.w[i / 2] << 16;
-                *reinterpret_cast<uint32_t *>(lds + a) = l | h;
-            } else {
-                uint32_t q[3];
-                cut3(__uint_as_float(lo.w[i]), __uint_as_float(hi.w[i]), q[0], q[1], q[2]);
-#pragma unroll
-                for (int p = 0; p < 3; ++p) *reinterpret_cast<uint32_t *>(lds + p * PLANE + a) = q[p];
-            }
-        }
-    }
-    static __device__ __forceinline__ uint4 frag(const char *lds, int p, int row, int g) {
-        return *reinterpret_cast<const uint4 *>(lds + p * PLANE + at(row, g));
+    static __device__ __forceinline__ u32x4 frag(const char *lds, int p, int row, int g) {
+        return *reinterpret_cast<const u32x4 *>(lds + p * PLANE + at(row, g));
     }
 };
 
+constexpr int kBM = 128, kBN = 128;      // tiles of dW
+
 struct LinArgs {
-    const void *A, *B;        // [M, K] and [N, K], rows of K elements
+    const void *A, *B;        // [M, K] and [N, K], rows of K elements (B: of ldb)
+    const void *plain;        // f32: the weights as they are ([N, K], or [K, N] when A is dy)
+    const void *aslope;       // A is multiplied by this slope on its way in (dz = dy act'(z))
     const void *bias, *res;
     void *C;                  // [M, N]
     void *slope;              // forward: act'(z) out
-    float *part;              // dW: [splits][N][K] slabs
+    float *part, *dbpart;     // dW: [splits][N][K] slabs, [splits][N] column sums
     long long M;
-    int N, K;
+    int N, K, ldb, act;
     long long tiles_n, tiles;
     long long per_split;      // dW: rows of one split
 };
 
-constexpr int kBM = 128, kBN = 128;
+// Granule of A as it enters the products: dy * slope, rounded to the tensor's type
+template <class T> struct SlopeGran {
+    uint32_t w[2 * sizeof(T)];
+};
+template <class T> __device__ __forceinline__ SlopeGran<T> ld_slope(const void *base, uint32_t bytes) {
+    SlopeGran<T> s;
+    const u32x4u *p = reinterpret_cast<const u32x4u *>(static_cast<const char *>(base) + bytes);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(typename SlopeOf<T>::type) / 2; ++i) {
+        const u32x4u v = p[i];
+        s.w[4 * i] = v[0]; s.w[4 * i + 1] = v[1]; s.w[4 * i + 2] = v[2]; s.w[4 * i + 3] = v[3];
+    }
+    return s;
+}
+template <class T> __device__ __forceinline__ SlopeGran<T> ld_slope_short(const void *base, uint32_t bytes, int left) {
+    typedef typename SlopeOf<T>::type ST;
+    SlopeGran<T> s;
+    const ST *p = reinterpret_cast<const ST *>(static_cast<const char *>(base) + bytes);
+    ST e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = i < left ? p[i] : (ST)0;
+    __builtin_memcpy(s.w, e, sizeof(e));
+    return s;
+}
+// the eight values of a granule in f32
+template <class T> __device__ __forceinline__ VecF<8> gran_values(const Gran<T> &g) {
+    VecF<8> v;
+    T e[8];
+    __builtin_memcpy(e, g.w, sizeof(e));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.e[i] = (float)e[i];
+    return v;
+}
+template <class T> __device__ __forceinline__ VecF<8> with_slope(const Gran<T> &g, const SlopeGran<T> &s) {
+    VecF<8> v = gran_values<T>(g);
+    if constexpr (IsF32<T>::value) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v.e[i] *= __uint_as_float(s.w[i]);
+    } else {
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 top = __builtin_bit_cast(u16x2, s.w[0]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, s.w[i]));
+            v.e[2 * i] *= fmaf((float)(s.w[i] & 0xffffu), 1.0f / 32768.f, -0.25f);
+            v.e[2 * i + 1] *= fmaf((float)(s.w[i] >> 16), 1.0f / 32768.f, -0.25f);
+        }
+        if (top[0] == 65535 || top[1] == 65535)      // a NaN among the eight
+            for (int i = 0; i < 8; ++i)
+                if (((s.w[i / 2] >> (16 * (i & 1))) & 0xffffu) == 65535u) v.e[i] = __uint_as_float(0x7fc00000u);
+    }
+    return v;
+}
+template <class T> __device__ __forceinline__ Gran<T> to_gran(const VecF<8> &v) {
+    Gran<T> g;
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = (T)v.e[i];
+    __builtin_memcpy(g.w, e, sizeof(e));
+    return g;
+}
 
-// acc (32x32 blocks of a wave's 64 x 64) += A-tile rows ra.. x B-tile rows rb..
-template <class T> __device__ __forceinline__ void tile_mma(const char *la, const char *lb, int ra, int rb, int lane,
-                                                            f32x16v (&acc)[2][2]) {
-    typedef Tile<T, kBM> TA;
-    typedef Tile<T, kBN> TB;
+// acc (32x32 blocks of a wave) += one contraction step of 16, all pieces
+template <class T, int MI, int NI>
+__device__ __forceinline__ void mma_pieces(const u32x4 (&a)[MI][Mul<T>::PIECES], const u32x4 (&b)[NI][Mul<T>::PIECES],
+                                           f32x16v (&acc)[MI][NI]) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+            if constexpr (Mul<T>::PIECES == 1) {
+                acc[i][j] = Mul<T>::mma(a[i][0], b[j][0], acc[i][j]);
+            } else {   // the small products first
+                acc[i][j] = Mul<T>::mma(a[i][0], b[j][2], acc[i][j]);
+                acc[i][j] = Mul<T>::mma(a[i][2], b[j][0], acc[i][j]);
+                acc[i][j] = Mul<T>::mma(a[i][1], b[j][1], acc[i][j]);
+                acc[i][j] = Mul<T>::mma(a[i][0], b[j][1], acc[i][j]);
+                acc[i][j] = Mul<T>::mma(a[i][1], b[j][0], acc[i][j]);
+                acc[i][j] = Mul<T>::mma(a[i][0], b[j][0], acc[i][j]);
+            }
+        }
+}
+
+// acc += A-tile rows ra.. x B-tile rows rb..
+template <class T, int BM, int BN, int MI, int NI>
+__device__ __forceinline__ void tile_mma(const char *la, const char *lb, int ra, int rb, int lane,
+                                         f32x16v (&acc)[MI][NI]) {
+    typedef Tile<T, BM> TA;
+    typedef Tile<T, BN> TB;
     const int r = lane & 31, half = lane >> 5;
 #pragma unroll
     for (int s = 0; s < TA::BK / 16; ++s) {
-        uint4 a[2][TA::P], b[2][TA::P];
+        u32x4 a[MI][TA::P], b[NI][TA::P];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int p = 0; p < TA::P; ++p) {
 #pragma unroll
-            for (int p = 0; p < TA::P; ++p) {
-                a[i][p] = TA::frag(la, p, ra + i * 32 + r, 2 * s + half);
-                b[i][p] = TB::frag(lb, p, rb + i * 32 + r, 2 * s + half);
-            }
+            for (int i = 0; i < MI; ++i) a[i][p] = TA::frag(la, p, ra + i * 32 + r, 2 * s + half);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                if constexpr (TA::P == 1) {
-                    acc[i][j] = Mul<T>::mma(a[i][0], b[j][0], acc[i][j]);
-                } else {   // the small products first
-                    acc[i][j] = Mul<T>::mma(a[i][0], b[j][2], acc[i][j]);
-                    acc[i][j] = Mul<T>::mma(a[i][2], b[j][0], acc[i][j]);
-                    acc[i][j] = Mul<T>::mma(a[i][1], b[j][1], acc[i][j]);
-                    acc[i][j] = Mul<T>::mma(a[i][0], b[j][1], acc[i][j]);
-                    acc[i][j] = Mul<T>::mma(a[i][1], b[j][0], acc[i][j]);
-                    acc[i][j] = Mul<T>::mma(a[i][0], b[j][0], acc[i][j]);
-                }
-            }
+            for (int j = 0; j < NI; ++j) b[j][p] = TB::frag(lb, p, rb + j * 32 + r, 2 * s + half);
+        }
+        mma_pieces<T, MI, NI>(a, b, acc);
     }
 }
 
 // row of accumulator register q in a 32 x 32 block (its column is lane & 31)
 __device__ __forceinline__ int acc_row(int q, int half) { return (q >> 2) * 8 + half * 4 + (q & 3); }
 
-// C[m][n] = epilogue(sum_k A[m][k] B[n][k]); FWD: bias, activation, residual, slope
-template <class T, int ACT, bool FWD>
-__global__ __launch_bounds__(256, 2) void lin_nt_kernel(const LinArgs A) {
-    typedef Tile<T, kBM> TA;
-    typedef Tile<T, kBN> TB;
-    constexpr int kLoop = TA::BYTES + TB::BYTES, kEpi = 4 * 32 * 68 * 4;
+// eight columns of one row on their way out: bias, activation, residual, slope
+template <class T, int ACT> __device__ __forceinline__ void epi_values(float (&v)[8], const float (&bias)[8],
+                                                                     typename SlopeOf<T>::type (&sl)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        float d;
+        v[k] = act_both<ACT, IsF32<T>::value>(v[k] + bias[k], d);
+        sl[k] = slope_out<T>(d);
+    }
+}
+template <class T, bool FWD>
+__device__ __forceinline__ void epi_piece(const LinArgs &A, long long m, int n, int have, float (&v)[8],
+                                          const float (&bias)[8]) {
+    typedef typename SlopeOf<T>::type ST;
+    const long long at = m * A.N + n;
+    T *out = static_cast<T *>(A.C) + at;
+    ST sl[8];
+    if constexpr (FWD) {
+        const T *res = A.res ? static_cast<const T *>(A.res) + at : nullptr;
+        VecF<8> rr;
+        if (res) {
+            if (have >= 8) rr = ldv<T, 8>(res);
+            else
+                for (int k = 0; k < 8; ++k) rr.e[k] = k < have ? (float)res[k] : 0.f;
+        }
+        GATMI_WITH_ACT(A.act, epi_values<T, ACT>(v, bias, sl));
+        if (A.slope) {
+            ST *so = static_cast<ST *>(A.slope) + at;
+            if (have >= 8) {
+#pragma unroll
+                for (int w = 0; w < (int)sizeof(ST) / 2; ++w) {
+                    u32x4u t;
+                    __builtin_memcpy(&t, sl + w * (16 / sizeof(ST)), 16);
+                    reinterpret_cast<u32x4u *>(so)[w] = t;
+                }
+            } else {
+                for (int k = 0; k < 8; ++k)
+                    if (k < have) so[k] = sl[k];
+            }
+        }
+        if (res)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] += rr.e[k];
+    }
+    if (have >= 8) {
+        VecF<8> o;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o.e[k] = v[k];
+        stv<T, 8>(out, o);
+    } else {
+        for (int k = 0; k < 8; ++k)
+            if (k < have) out[k] = (T)v[k];
+    }
+}
+
+// the sum in plain f32, an element at a time: what the pieces cannot say (f32 only)
+template <bool FWD> __device__ __forceinline__ float plain_dot(const LinArgs &A, long long m, int n) {
+    const float *a = static_cast<const float *>(A.A) + m * A.K;
+    const float *sl = FWD || !A.aslope ? nullptr : static_cast<const float *>(A.aslope) + m * A.K;
+    const float *w = static_cast<const float *>(A.plain) + (FWD ? (long long)n * A.K : n);
+    const long long step = FWD ? 1 : A.N;
+    float s = 0.f;
+#pragma unroll 1
+    for (int k = 0; k < A.K; ++k) s = fmaf(sl ? a[k] * sl[k] : a[k], w[k * step], s);
+    return s;
+}
+
+// C[m][n] = epilogue(sum_k A[m][k] B[n][k]).  FWD: bias, activation, residual, slope; else A = dy * aslope
+// when given.  CUT (f32): B comes as three planes of bf16 pieces, rows of ldb (a multiple of 8, zeros behind K).
+// SHORT: K < 8.
+template <class T, int BM, int BN, int WM, int WN, bool FWD, bool CUT, bool SHORT>
+__global__ __launch_bounds__(WM * WN * 64) void lin_nt_kernel(const LinArgs A) {
+    typedef Tile<T, BM> TA;
+    typedef Tile<T, BN> TB;
+    constexpr int THREADS = WM * WN * 64, MI = BM / WM / 32, NI = BN / WN / 32;
+    constexpr int LD = NI * 32 + 4;
+    constexpr int kLoop = TA::BYTES + TB::BYTES, kEpi = WM * WN * 16 * LD * 4;
     __shared__ __attribute__((aligned(16))) char smem[kLoop > kEpi ? kLoop : kEpi];
     char *la = smem, *lb = smem + TA::BYTES;
     // consecutive tiles share rows of A: give each XCD (block index mod 8) a contiguous range of them
     const long long tile = (long long)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     if (tile >= A.tiles) return;
-    const long long m0 = tile / A.tiles_n * kBM;
-    const int n0 = (int)(tile % A.tiles_n) * kBN;
-    const T *pa = static_cast<const T *>(A.A), *pb = static_cast<const T *>(A.B);
+    const long long m0 = tile / A.tiles_n * BM;
+    const int n0 = (int)(tile % A.tiles_n) * BN;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    constexpr int G = TA::G, NA = kBM * G / 256, NB = kBN * G / 256;
-    Gran<T> ga[NA], gb[NB];
+    const int wm = (wave / WN) * (MI * 32), wn = (wave % WN) * (NI * 32);
+    constexpr int G = TA::G, RP = THREADS / G, NA = BM / RP, NB = (BN + RP - 1) / RP;
+    static_assert(BM % RP == 0 && (BN % RP == 0 || BN < RP), "whole tiles a pass");
+    typedef typename SlopeOf<T>::type ST;
+    Gran<T> ga[NA];
+    SlopeGran<T> gs[FWD ? 1 : NA];
+    Gran<T> gb[CUT ? 1 : NB];
+    u32x4 gc[CUT ? NB : 1][3];
     const int g = threadIdx.x % G, row = threadIdx.x / G;
+    const bool sloped = !FWD && A.aslope;
+    // wave-uniform tile bases, 32-bit offsets from there (a tile spans at most 256 rows of 256 KB); rows behind
+    // the matrix repeat its last one, their results are not stored
+    const T *ba = static_cast<const T *>(A.A) + m0 * A.K;
+    const ST *bs = static_cast<const ST *>(A.aslope) + m0 * A.K;
+    const char *bb = static_cast<const char *>(A.B) + (long long)n0 * A.ldb * (CUT ? 2 : (int)sizeof(T));
+    const long long plane = (long long)A.N * A.ldb * 2;
+    uint32_t ra[NA], rb[NB];        // row offsets in elements
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+        const long long left = A.M - 1 - m0;
+        const int r = row + i * RP;
+        ra[i] = (uint32_t)(r < left ? r : (int)left) * (uint32_t)A.K;
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const int left = A.N - 1 - n0, r = row + i * RP;
+        rb[i] = (uint32_t)(r < left ? r : left) * (uint32_t)A.ldb;
+    }
+    const int last = CUT ? A.ldb - 8 : A.K - 8;     // B's last whole granule
     auto fetch = [&](int k0) {
-        const int k = k0 + g * 8;
+        const int k = k0 + g * 8, ka = SHORT ? k : (k < A.K - 8 ? k : A.K - 8), kb = SHORT && !CUT ? k : (k < last ? k : last);
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
-            long long m = m0 + row + i * (256 / G);
-            if (m >= A.M) m = A.M - 1;             // its results are not stored
-            ga[i] = ld_gran<T>(pa + m * A.K + k, A.K - k);
+            if constexpr (SHORT) {
+                ga[i] = ld_gran_short<T>(ba, (ra[i] + ka) * (uint32_t)sizeof(T), A.K - k);
+                if (!FWD && sloped) gs[i] = ld_slope_short<T>(bs, (ra[i] + ka) * (uint32_t)sizeof(ST), A.K - k);
+            } else {
+                ga[i] = ld_gran<T>(ba, (ra[i] + ka) * (uint32_t)sizeof(T));
+                if (!FWD && sloped) gs[i] = ld_slope<T>(bs, (ra[i] + ka) * (uint32_t)sizeof(ST));
+            }
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-            int n = n0 + row + i * (256 / G);
-            if (n >= A.N) n = A.N - 1;
-            gb[i] = ld_gran<T>(pb + (long long)n * A.K + k, A.K - k);
+            if constexpr (CUT) {
+#pragma unroll
+                for (int p = 0; p < 3; ++p)
+                    gc[i][p] = *reinterpret_cast<const u32x4 *>(bb + p * plane + (rb[i] + kb) * 2u);
+            } else if constexpr (SHORT) {
+                gb[i] = ld_gran_short<T>(bb, (rb[i] + kb) * (uint32_t)sizeof(T), A.K - k);
+            } else {
+                gb[i] = ld_gran<T>(bb, (rb[i] + kb) * (uint32_t)sizeof(T));
+            }
         }
     };
-    f32x16v acc[2][2];
+    f32x16v acc[MI][NI];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
     fetch(0);
     for (int k0 = 0; k0 < A.K; k0 += TA::BK) {
+        // the row's last, partial step: what a granule holds of the one before it is dropped.  An image has
+        // zeros behind K instead of a step back, in its place: A must line up, so it is moved down there.
+        const bool end = !SHORT && k0 + TA::BK > A.K;
+        const int k = k0 + g * 8, over = k > A.K - 8 ? k - (A.K - 8) : 0;
 #pragma unroll
-        for (int i = 0; i < NA; ++i) TA::put(la, row + i * (256 / G), g, ga[i]);
+        for (int i = 0; i < NA; ++i) {
+            if (!FWD && sloped) ga[i] = to_gran<T>(with_slope<T>(ga[i], gs[i]));
+            if (end) {
+                if constexpr (CUT) shift_down<T>(ga[i].w, over);
+                else drop(ga[i], over);
+            }
+            TA::put(la, row + i * RP, g, ga[i]);
+        }
 #pragma unroll
-        for (int i = 0; i < NB; ++i) TB::put(lb, row + i * (256 / G), g, gb[i]);
+        for (int i = 0; i < NB; ++i) {
+            if (BN < RP && row >= BN) continue;
+            if constexpr (CUT) {
+#pragma unroll
+                for (int p = 0; p < 3; ++p)
+                    *reinterpret_cast<u32x4 *>(lb + p * TB::PLANE + TB::at(row + i * RP, g)) = gc[i][p];
+            } else {
+                if (end) drop(gb[i], over);
+                TB::put(lb, row + i * RP, g, gb[i]);
+            }
+        }
         __syncthreads();
         if (k0 + TA::BK < A.K) fetch(k0 + TA::BK);
-        tile_mma<T>(la, lb, wm, wn, lane, acc);
+        tile_mma<T, BM, BN, MI, NI>(la, lb, wm, wn, lane, acc);
         __syncthreads();
     }
-    // epilogue: a wave turns its blocks 32 rows at a time through LDS of its own into row pieces of 8
-    constexpr int LD = 68;
-    float *le = reinterpret_cast<float *>(smem) + wave * 32 * LD;
-    const int half = lane >> 5, c8 = (lane & 7) * 8, r8 = lane >> 3;
+    // epilogue: a wave turns its blocks 16 rows at a time through LDS of its own into row pieces of 8
+    float *le = reinterpret_cast<float *>(smem) + wave * 16 * LD;
+    constexpr int PR = NI * 4, RI = 64 / PR;        // pieces a row, rows at once
+    const int half = lane >> 5, c8 = (lane % PR) * 8, rr = lane / PR;
     const int n = n0 + wn + c8;
     const int have = A.N - n;                       // columns of this piece that exist
     float bias[8];
@@ -246,107 +456,133 @@ __global__ __launch_bounds__(256, 2) void lin_nt_kernel(const LinArgs A) {
     for (int k = 0; k < 8; ++k)
         bias[k] = FWD && A.bias && k < have ? (float)static_cast<const T *>(A.bias)[n + k] : 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        __syncthreads();
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int h = 0; h < 2; ++h) {
+            // the wave's own LDS, in order: what it stored before is read before it stores again
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-            for (int q = 0; q < 16; ++q) le[acc_row(q, half) * LD + j * 32 + (lane & 31)] = acc[i][j][q];
-        __syncthreads();
+            for (int j = 0; j < NI; ++j)
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const long long m = m0 + wm + i * 32 + p * 8 + r8;
-            if (m >= A.M || have <= 0) continue;
-            float v[8];
+                for (int q = 0; q < 8; ++q) le[acc_row(q, half) * LD + j * 32 + (lane & 31)] = acc[i][j][h * 8 + q];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = le[(p * 8 + r8) * LD + c8 + k];
-            if constexpr (IsF32<T>::value) {        // see the head of this file
-                bool fine = true;
+            for (int p = 0; p < 16 / RI; ++p) {
+                const long long m = m0 + wm + i * 32 + h * 16 + p * RI + rr;
+                if (m >= A.M || have <= 0) continue;
+                float v[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) fine = fine && fabsf(v[k]) < INFINITY;
-                if (!fine)
-                    for (int k = 0; k < 8; ++k) {
-                        if (k >= have || fabsf(v[k]) < INFINITY) continue;
-                        float s = 0.f;
-                        for (int kk = 0; kk < A.K; ++kk)
-                            s = fmaf((float)pa[m * A.K + kk], (float)pb[(long long)(n + k) * A.K + kk], s);
-                        v[k] = s;
-                    }
-            }
-            const long long at = m * A.N + n;
-            T *out = static_cast<T *>(A.C) + at;
-            const T *res = static_cast<const T *>(A.res) + at;
-            typedef typename SlopeOf<T>::type ST;
-            ST *so = static_cast<ST *>(A.slope) + at;
-            if (have >= 8) {
-                VecF<8> o, rr;
-                ST sl[8];
-                if (FWD && A.res) rr = ldv<T, 8>(res);
+                for (int k = 0; k < 8; ++k) v[k] = le[(p * RI + rr) * LD + c8 + k];
+                if constexpr (IsF32<T>::value) {        // see the head of this file
+                    bool fine = true;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    float y = v[k];
-                    if constexpr (FWD) {
-                        float d;
-                        y = act_both<ACT, IsF32<T>::value>(y + bias[k], d);
-                        sl[k] = slope_out<T>(d);
-                        if (A.res) y += rr.e[k];
-                    }
-                    o.e[k] = y;
-                }
-                stv<T, 8>(out, o);
-                if (FWD && ACT != GATMI_ACT_NONE && A.slope) {
+                    for (int k = 0; k < 8; ++k) fine = fine && fabsf(v[k]) < INFINITY;
+                    if (!fine) {
+                        float *row = le + (p * RI + rr) * LD + c8;      // this lane's own eight
+#pragma unroll 1
+                        for (int k = 0; k < 8; ++k)
+                            if (k < have && !(fabsf(row[k]) < INFINITY)) row[k] = plain_dot<FWD>(A, m, n + k);
 #pragma unroll
-                    for (int w = 0; w < (int)sizeof(ST) / 2; ++w) {
-                        u32x4u t;
-                        __builtin_memcpy(&t, sl + w * (16 / sizeof(ST)), 16);
-                        reinterpret_cast<u32x4u *>(so)[w] = t;
+                        for (int k = 0; k < 8; ++k) v[k] = row[k];
                     }
                 }
-            } else {
-                for (int k = 0; k < 8; ++k) {
-                    if (k >= have) break;
-                    float y = v[k];
-                    if constexpr (FWD) {
-                        float d;
-                        y = act_both<ACT, IsF32<T>::value>(y + bias[k], d);
-                        if (ACT != GATMI_ACT_NONE && A.slope) so[k] = slope_out<T>(d);
-                        if (A.res) y += (float)res[k];
-                    }
-                    out[k] = (T)y;
-                }
+                epi_piece<T, FWD>(A, m, n, have, v, bias);
             }
         }
-    }
 }
 
-// dW slabs: part[split][n][k] = sum over the split's rows of A[m][n] B[m][k]  (A = dz [M, N], B = x [M, K])
-template <class T> __global__ __launch_bounds__(256, 2) void lin_tn_kernel(const LinArgs A) {
-    typedef Tile<T, kBM> TA;
-    typedef Tile<T, kBN> TB;
+// A tile of the transposed product in LDS, as it lies in memory: contraction steps (rows of the matrix) by
+// C channels, PIECES planes.  Fragments are read with the transposing LDS load: 16 lanes fetch a block of
+// 4 steps x 16 channels, four channels each, and every lane comes back with one channel's four steps.  Rows are
+// 64 bytes apart from a multiple of 256, so that the four rows of a block lie in different banks.
+template <class T, int C> struct TileT {
+    static constexpr int BK = Mul<T>::BK, P = Mul<T>::PIECES;
+    static constexpr int STRIDE = C * 2 + 64, PLANE = BK * STRIDE, BYTES = PLANE * P;
+    static __device__ __forceinline__ void put(char *lds, int row, int col, const Gran<T> &v) {
+        char *at = lds + row * STRIDE + col * 2;
+        if constexpr (P == 1) {
+            *reinterpret_cast<u32x4 *>(at) = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
+        } else {
+            uint32_t q[3][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                cut3(__uint_as_float(v.w[2 * i]), __uint_as_float(v.w[2 * i + 1]), q[0][i], q[1][i], q[2][i]);
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+                *reinterpret_cast<u32x4 *>(at + p * PLANE) = u32x4{q[p][0], q[p][1], q[p][2], q[p][3]};
+        }
+    }
+    // channels col0 .. col0 + 31, steps 16 s + 8 half .. + 7 of this lane's channel
+    static __device__ __forceinline__ u32x4 frag(const char *lds, int p, int s, int col0, int lane) {
+        typedef short v4s __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) v4s *lds_ptr;
+        const int row = 16 * s + (lane >> 5) * 8 + ((lane & 15) >> 2), col = col0 + (lane & 16) + (lane & 3) * 4;
+        const char *at = lds + p * PLANE + row * STRIDE + col * 2;
+        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at));
+        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 4 * STRIDE));
+        typedef short v8s __attribute__((ext_vector_type(8)));
+        return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+};
+
+// dW slabs: part[split][n][k] = sum over the split's rows of dz[m][n] x[m][k], dz = A (* aslope) [M, N],
+// x = B [M, K]; the blocks of the first column of tiles also leave dz's column sums.  SHORT: N or K < 8.
+template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void lin_tn_kernel(const LinArgs A) {
+    typedef TileT<T, kBM> TA;
+    typedef TileT<T, BN> TB;
+    constexpr int THREADS = 2 * BN, WN = BN / 64, GA = kBM / 8, GB = BN / 8;
+    constexpr int RA = THREADS / GA, RB = THREADS / GB, NA = TA::BK / RA, NB = TA::BK / RB;
     __shared__ __attribute__((aligned(16))) char smem[TA::BYTES + TB::BYTES];
+    static_assert(TA::BYTES + TB::BYTES >= RA * kBM * 4, "the column sums fit");
     char *la = smem, *lb = smem + TA::BYTES;
     const long long split = blockIdx.x / A.tiles;
     const int tile = (int)(blockIdx.x - split * A.tiles);
-    const int n0 = tile / (int)A.tiles_n * kBM, k0 = tile % (int)A.tiles_n * kBN;
+    const int n0 = tile / (int)A.tiles_n * kBM, k0 = tile % (int)A.tiles_n * BN;
     const long long r0 = split * A.per_split, r1 = r0 + A.per_split < A.M ? r0 + A.per_split : A.M;
     const T *pa = static_cast<const T *>(A.A), *pb = static_cast<const T *>(A.B);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    // a thread's pieces: contraction pair (2 * pr, + 1), eight channels ch ..
-    constexpr int PAIRS = TA::BK / 2, GC = 256 / PAIRS, NP = kBM / 8 / GC;
-    const int pr = threadIdx.x % PAIRS, cg = threadIdx.x / PAIRS;
-    Gran<T> ga[NP][2], gb[NP][2];
+    const int wm = (wave / WN) * 64, wn = (wave % WN) * 64;
+    typedef typename SlopeOf<T>::type ST;
+    const bool sloped = A.aslope, sums = A.dbpart && k0 == 0;
+    Gran<T> ga[NA], gb[NB];
+    SlopeGran<T> gs[NA];
+    VecF<8> db;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) db.e[k] = 0.f;
+    // a thread's pieces: eight channels, rows ta + i * RA (tb + i * RB).  A piece that would run over the last
+    // channel is loaded from the last eight and moved to its place.
+    const int ta = threadIdx.x / GA, ja = threadIdx.x % GA * 8, tb = threadIdx.x / GB, jb = threadIdx.x % GB * 8;
+    const bool edge_a = !SHORT && n0 + kBM > A.N, edge_b = !SHORT && k0 + BN > A.K;
+    int ca = n0 + ja, cb = k0 + jb, over_a = 0, over_b = 0;
+    if (!SHORT && ca > A.N - 8) {
+        over_a = ca - (A.N - 8);
+        ca = A.N - 8;
+    }
+    if (!SHORT && cb > A.K - 8) {
+        over_b = cb - (A.K - 8);
+        cb = A.K - 8;
+    }
     auto fetch = [&](long long r) {
+        const T *ra = pa + r * A.N, *rb = pb + r * A.K;
+        const ST *rs = static_cast<const ST *>(A.aslope) + r * A.N;
+        const int left = (int)(r1 - 1 - r < TA::BK ? r1 - 1 - r : TA::BK);      // rows behind the last repeat it
 #pragma unroll
-        for (int i = 0; i < NP; ++i)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const long long m = r + 2 * pr + u;
-                const bool in = m < r1;
-                const int ca = n0 + (cg + i * GC) * 8, cb = k0 + (cg + i * GC) * 8;
-                ga[i][u] = ld_gran<T>(pa + (in ? m : r0) * A.N + (ca < A.N ? ca : 0), in ? A.N - ca : 0);
-                gb[i][u] = ld_gran<T>(pb + (in ? m : r0) * A.K + (cb < A.K ? cb : 0), in ? A.K - cb : 0);
+        for (int i = 0; i < NA; ++i) {
+            const uint32_t m = ta + i * RA < left ? ta + i * RA : left, at = m * (uint32_t)A.N + ca;
+            if constexpr (SHORT) {
+                ga[i] = ld_gran_short<T>(ra, at * (uint32_t)sizeof(T), A.N - ca);
+                if (sloped) gs[i] = ld_slope_short<T>(rs, at * (uint32_t)sizeof(ST), A.N - ca);
+            } else {
+                ga[i] = ld_gran<T>(ra, at * (uint32_t)sizeof(T));
+                if (sloped) gs[i] = ld_slope<T>(rs, at * (uint32_t)sizeof(ST));
             }
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const uint32_t m = tb + i * RB < left ? tb + i * RB : left, at = m * (uint32_t)A.K + cb;
+            if constexpr (SHORT) gb[i] = ld_gran_short<T>(rb, at * (uint32_t)sizeof(T), A.K - cb);
+            else gb[i] = ld_gran<T>(rb, at * (uint32_t)sizeof(T));
+        }
     };
     f32x16v acc[2][2];
 #pragma unroll
@@ -357,15 +593,62 @@ template <class T> __global__ __launch_bounds__(256, 2) void lin_tn_kernel(const
             for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
     if (r0 < r1) fetch(r0);
     for (long long r = r0; r < r1; r += TA::BK) {
+        const bool end = r + TA::BK > r1;
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            TA::put_pair(la, (cg + i * GC) * 8, pr, ga[i][0], ga[i][1]);
-            TB::put_pair(lb, (cg + i * GC) * 8, pr, gb[i][0], gb[i][1]);
+        for (int i = 0; i < NA; ++i) {
+            if (edge_a) {
+                shift_down<T>(ga[i].w, over_a);
+                if (sloped) shift_down<T>(gs[i].w, over_a);
+            }
+            if (end && r + ta + i * RA >= r1) {        // no such row: zeros, slope and all
+                shift_down<T>(ga[i].w, 8);
+                if (sloped) shift_down<T>(gs[i].w, 8);
+            }
+            if (sloped) {
+                const VecF<8> v = with_slope<T>(ga[i], gs[i]);
+                if (sums)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) db.e[k] += v.e[k];     // before the rounding
+                ga[i] = to_gran<T>(v);
+            } else if (sums) {
+                const VecF<8> v = gran_values<T>(ga[i]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) db.e[k] += v.e[k];
+            }
+            TA::put(la, ta + i * RA, ja, ga[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            if (edge_b) shift_down<T>(gb[i].w, over_b);
+            if (end && r + tb + i * RB >= r1) shift_down<T>(gb[i].w, 8);
+            TB::put(lb, tb + i * RB, jb, gb[i]);
         }
         __syncthreads();
         if (r + TA::BK < r1) fetch(r + TA::BK);
-        tile_mma<T>(la, lb, wm, wn, lane, acc);
+#pragma unroll
+        for (int s = 0; s < TA::BK / 16; ++s) {
+            u32x4 a[2][TA::P], b[2][TA::P];
+#pragma unroll
+            for (int p = 0; p < TA::P; ++p)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    a[i][p] = TA::frag(la, p, s, wm + i * 32, lane);
+                    b[i][p] = TB::frag(lb, p, s, wn + i * 32, lane);
+                }
+            mma_pieces<T, 2, 2>(a, b, acc);
+        }
         __syncthreads();
+    }
+    if (sums) {      // [RA][128] partial sums, added in order
+        float *red = reinterpret_cast<float *>(smem);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) red[ta * kBM + ja + k] = db.e[k];
+        __syncthreads();
+        if (threadIdx.x < kBM && n0 + (int)threadIdx.x < A.N) {
+            float s = 0.f;
+            for (int q = 0; q < RA; ++q) s += red[q * kBM + threadIdx.x];
+            A.dbpart[split * A.N + n0 + threadIdx.x] = s;
+        }
     }
     float *part = A.part + split * (long long)A.N * A.K;
 #pragma unroll
@@ -379,66 +662,83 @@ template <class T> __global__ __launch_bounds__(256, 2) void lin_tn_kernel(const
                 float v = acc[i][j][q];
                 if (IsF32<T>::value && !(fabsf(v) < INFINITY)) {
                     v = 0.f;
-                    for (long long m = r0; m < r1; ++m) v = fmaf((float)pa[m * A.N + n], (float)pb[m * A.K + k], v);
+                    for (long long m = r0; m < r1; ++m) {
+                        float d = (float)pa[m * A.N + n];
+                        if (sloped) d *= static_cast<const float *>(A.aslope)[m * A.N + n];
+                        v = fmaf(d, (float)pb[m * A.K + k], v);
+                    }
                 }
                 part[(long long)n * A.K + k] = v;
             }
 }
 
-// dW = sum of the slabs, in order
-template <class T> __global__ __launch_bounds__(256) void lin_slabs_kernel(const float *part, int splits, long long size, T *out) {
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < size; i += gridDim.x * 256ll) {
-        float s = 0.f;
-        for (int q = 0; q < splits; ++q) s += part[q * size + i];
-        out[i] = (T)s;
+// A few rows (serving): one wave a column of y, lanes along the contraction, f32 multiply-adds whatever the
+// type.  The weights are read once, by as many waves as there are columns.
+template <class T, int MR> __global__ __launch_bounds__(256) void lin_rows_kernel(const LinArgs A) {
+    constexpr int V = 16 / sizeof(T);
+    const int lane = threadIdx.x & 63;
+    const int n = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (n >= A.N) return;
+    const T *w = static_cast<const T *>(A.B) + (long long)n * A.K, *x = static_cast<const T *>(A.A);
+    const int M = (int)A.M;
+    float acc[MR];
+#pragma unroll
+    for (int r = 0; r < MR; ++r) acc[r] = 0.f;
+    const int whole = A.K / V * V;
+#pragma unroll 2
+    for (int k = lane * V; k < whole; k += 64 * V) {
+        const VecF<V> wv = ldv<T, V>(w + k);
+#pragma unroll
+        for (int r = 0; r < MR; ++r) {
+            const VecF<V> xv = ldv<T, V>(x + (long long)(r < M ? r : M - 1) * A.K + k);
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[r] = fmaf(xv.e[i], wv.e[i], acc[r]);
+        }
     }
+    if (whole + lane < A.K) {
+        const float wl = (float)w[whole + lane];
+#pragma unroll
+        for (int r = 0; r < MR; ++r) acc[r] = fmaf((float)x[(long long)(r < M ? r : M - 1) * A.K + whole + lane], wl, acc[r]);
+    }
+    float z = 0.f;
+#pragma unroll
+    for (int r = 0; r < MR; ++r) {
+        const float s = head_sum<64>(acc[r], 64);
+        if (lane == r) z = s;      // lane r ends with row r
+    }
+    if (lane >= M) return;
+    const long long at = (long long)lane * A.N + n;
+    z += A.bias ? (float)static_cast<const T *>(A.bias)[n] : 0.f;
+    float d = 1.f, y = z;
+    GATMI_WITH_ACT(A.act, y = (act_both<ACT, IsF32<T>::value>(z, d)));
+    if (A.slope) static_cast<typename SlopeOf<T>::type *>(A.slope)[at] = slope_out<T>(d);
+    if (A.res) y += (float)static_cast<const T *>(A.res)[at];
+    static_cast<T *>(A.C)[at] = (T)y;
 }
 
-// dz = dy * act'(z) (DZ: written), and its column sums per block (part [blocks][N], when part)
-template <class T, int V, bool DZ>
-__global__ __launch_bounds__(256) void lin_dz_kernel(const T *dy, const typename SlopeOf<T>::type *slope, T *dz,
-                                                     float *part, long long rows, int N) {
-    __shared__ VecF<V> red[256];
-    const int nslot = (N + V - 1) / V, first = blockIdx.y * 256;
-    const int slots = nslot - first < 256 ? nslot - first : 256;
-    const int rpp = 256 / slots, s = threadIdx.x % slots, rsub = threadIdx.x / slots;
-    const int j = (first + s) * V, off = j + V <= N ? j : N - V, skip = j - off;
-    const long long per = (rows + gridDim.x - 1) / gridDim.x, r0 = blockIdx.x * per, r1 = r0 + per < rows ? r0 + per : rows;
-    VecF<V> sum;
-#pragma unroll
-    for (int k = 0; k < V; ++k) sum.e[k] = 0.f;
-    if (rsub < rpp)
-#pragma unroll 4
-        for (long long r = r0 + rsub; r < r1; r += rpp) {
-            VecF<V> g = ldv<T, V>(dy + r * N + off);
-            if (DZ) {
-                typename SlopeOf<T>::type q[V];
-                __builtin_memcpy(q, slope + r * N + off, sizeof(q));
-#pragma unroll
-                for (int k = 0; k < V; ++k) g.e[k] *= slope_in(q[k]);
-                stv<T, V>(dz + r * N + off, g);
-            }
-#pragma unroll
-            for (int k = 0; k < V; ++k) sum.e[k] += g.e[k];
-        }
-    if (!part) return;
-    red[threadIdx.x] = sum;
+// dW = sum of the slabs, in order.  64 values by 4 groups of slabs a block: few values and hundreds of slabs
+// still make many loads
+template <class T> __global__ __launch_bounds__(256) void lin_slabs_kernel(const float *part, int splits, long long size, T *out) {
+    __shared__ float red[256];
+    const int lane = threadIdx.x & 63, grp = threadIdx.x >> 6;
+    const long long i = blockIdx.x * 64ll + lane;
+    float s = 0.f;
+    if (i < size)
+#pragma unroll 8
+        for (int q = grp; q < splits; q += 4) s += part[q * size + i];
+    red[threadIdx.x] = s;
     __syncthreads();
-    if ((int)threadIdx.x < slots) {
-        for (int q = 1; q < rpp; ++q)
-#pragma unroll
-            for (int k = 0; k < V; ++k) sum.e[k] += red[threadIdx.x + q * slots].e[k];
-#pragma unroll
-        for (int k = 0; k < V; ++k)
-            if (k >= skip) part[(long long)blockIdx.x * N + off + k] = sum.e[k];
-    }
+    if (grp == 0 && i < size) out[i] = (T)(((s + red[64 + lane]) + red[128 + lane]) + red[192 + lane]);
 }
-template <class T> __global__ __launch_bounds__(256) void lin_db_kernel(const float *part, int blocks, int N, T *db) {
+
+// db = sum of the splits' column sums, in order
+template <class T> __global__ __launch_bounds__(256) void lin_db_kernel(const float *part, int splits, int N, T *db) {
     __shared__ double red[256];
     const int c = blockIdx.x * 8 + (threadIdx.x & 7), rg = threadIdx.x >> 3;
     double s = 0.0;
     if (c < N)
-        for (int b = rg; b < blocks; b += 32) s += part[(long long)b * N + c];
+#pragma unroll 4
+        for (int b = rg; b < splits; b += 32) s += part[(long long)b * N + c];
     red[threadIdx.x] = s;
     __syncthreads();
     if (rg == 0 && c < N) {
@@ -447,15 +747,33 @@ template <class T> __global__ __launch_bounds__(256) void lin_db_kernel(const fl
     }
 }
 
-// out[k][n] = w[n][k]
-template <class T> __global__ __launch_bounds__(256) void lin_transpose_kernel(const T *w, int N, int K, T *out) {
+// The weights as the products take them: rows of `ld` (a multiple of 8, zeros behind the end), the matrix
+// itself (TR: transposed, out[k][n] = w[n][k]), f32 as three planes of bf16 pieces
+template <class T, bool TR> __global__ __launch_bounds__(256) void lin_image_kernel(const T *w, int N, int K, int ld, void *out) {
     __shared__ T t[32][33];
-    const int k0 = blockIdx.x * 32, n0 = blockIdx.y * 32, x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    for (int i = y; i < 32; i += 8)
-        if (n0 + i < N && k0 + x < K) t[i][x] = w[(long long)(n0 + i) * K + k0 + x];
+    const int R = TR ? K : N, S = TR ? N : K;       // rows and columns of the image
+    const int s0 = blockIdx.x * 32, r0 = blockIdx.y * 32, x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    for (int i = y; i < 32; i += 8) {
+        const int n = TR ? s0 + i : r0 + i, k = TR ? r0 + x : s0 + x;
+        t[TR ? x : i][TR ? i : x] = n < N && k < K ? w[(long long)n * K + k] : (T)0.f;
+    }
     __syncthreads();
-    for (int i = y; i < 32; i += 8)
-        if (k0 + i < K && n0 + x < N) out[(long long)(k0 + i) * N + n0 + x] = t[x][i];
+    for (int i = y; i < 32; i += 8) {
+        if (r0 + i >= R || s0 + x >= ld) continue;
+        const long long at = (long long)(r0 + i) * ld + s0 + x;
+        if constexpr (IsF32<T>::value) {
+            uint32_t p0, p1, p2;
+            cut3(t[i][x], 0.f, p0, p1, p2);
+            uint16_t *o = static_cast<uint16_t *>(out);
+            const long long plane = (long long)R * ld;
+            o[at] = (uint16_t)p0;
+            o[plane + at] = (uint16_t)p1;
+            o[2 * plane + at] = (uint16_t)p2;
+        } else {
+            static_cast<T *>(out)[at] = t[i][x];
+        }
+    }
+    (void)S;
 }
 
 static int lin_check(const gatmi_linear *l) {
@@ -468,17 +786,21 @@ static int lin_check(const gatmi_linear *l) {
     return GATMI_OK;
 }
 
-constexpr int kDzBlocks = 2048;
 struct LinGeom {
-    int dz_blocks, splits;
+    int splits;
     long long per_split;
-    size_t dz, wt, part, slabs;     // bytes
+    int ldf, ldb;                   // row lengths of the weight images, forward and transposed
+    size_t image_f, image_b, slabs, dbpart;     // bytes
+    bool image_fwd;                 // the forward takes an image
 };
+// From this many rows on the f32 forward reads its weights as pieces cut once, not by every block
+constexpr long long kCutRows = 2048;
+constexpr int kFewRows = 16;
+
 static LinGeom lin_geom(const gatmi_linear *l) {
     LinGeom G;
-    const size_t el = l->dtype == GATMI_F32 ? 4 : 2;
-    const long long b = (l->rows + 31) / 32;
-    G.dz_blocks = (int)(b < 1 ? 1 : (b > kDzBlocks ? kDzBlocks : b));
+    memset(&G, 0, sizeof(G));
+    const size_t el = l->dtype == GATMI_F32 ? 6 : 2;
     const long long tiles = ((l->out_features + kBM - 1ll) / kBM) * ((l->in_features + kBN - 1ll) / kBN);
     // enough splits of the rows for two blocks a CU, at least 256 rows each
     long long s = (2ll * device_cus() + tiles - 1) / tiles;
@@ -490,47 +812,85 @@ static LinGeom lin_geom(const gatmi_linear *l) {
     if (G.per_split < bk) G.per_split = bk;
     G.splits = (int)((l->rows + G.per_split - 1) / G.per_split);
     if (G.splits < 1) G.splits = 1;
-    G.dz = align_up((size_t)l->rows * l->out_features * el);
-    G.wt = align_up((size_t)l->in_features * l->out_features * el);
-    G.part = align_up((size_t)G.dz_blocks * l->out_features * 4);
+    G.ldf = (l->in_features + 7) / 8 * 8;
+    G.ldb = (l->out_features + 7) / 8 * 8;
+    G.image_fwd = l->dtype == GATMI_F32 && l->rows >= kCutRows;
+    G.image_f = G.image_fwd ? align_up((size_t)l->out_features * G.ldf * el) : 0;
+    G.image_b = align_up((size_t)l->in_features * G.ldb * el);
     G.slabs = align_up((size_t)G.splits * l->in_features * l->out_features * 4);
+    G.dbpart = align_up((size_t)G.splits * l->out_features * 4);
     return G;
 }
 
-template <class T> static void lin_launch_nt(LinArgs A, bool fwd, int act, hipStream_t st) {
-    A.tiles_n = (A.N + kBN - 1) / kBN;
-    A.tiles = (A.M + kBM - 1) / kBM * A.tiles_n;
+template <class T, int BM, int BN, int WM, int WN, bool FWD, bool CUT, bool SHORT = false> static void lin_go(LinArgs &A, hipStream_t st) {
+    A.tiles_n = (A.N + BN - 1) / BN;
+    A.tiles = (A.M + BM - 1) / BM * A.tiles_n;
     const unsigned grid = (unsigned)((A.tiles + 7) / 8 * 8);
-    if (!fwd) {
-        hipLaunchKernelGGL((lin_nt_kernel<T, GATMI_ACT_NONE, false>), dim3(grid), dim3(256), 0, st, A);
-        return;
-    }
-    GATMI_WITH_ACT(act, hipLaunchKernelGGL((lin_nt_kernel<T, ACT, true>), dim3(grid), dim3(256), 0, st, A));
+    hipLaunchKernelGGL((lin_nt_kernel<T, BM, BN, WM, WN, FWD, CUT, SHORT>), dim3(grid), dim3(WM * WN * 64), 0, st, A);
+}
+// The tile: narrow ones for narrow results; 64 x 64 while larger ones would leave compute units idle
+template <class T, bool FWD, bool CUT> static void lin_launch_nt(LinArgs A, hipStream_t st) {
+    const long long big = (A.M + 127) / 128 * ((A.N + 127) / 128);
+    if (A.K < 8) lin_go<T, 64, 64, 2, 2, FWD, CUT, true>(A, st);
+    else if (A.N <= 32) lin_go<T, 128, 32, 4, 1, FWD, CUT>(A, st);
+    else if (big < device_cus()) lin_go<T, 64, 64, 2, 2, FWD, CUT>(A, st);
+    else if (A.N <= 64) lin_go<T, 128, 64, 4, 1, FWD, CUT>(A, st);
+#ifndef LIN_WIDE
+#define LIN_WIDE 1
+#endif
+    else if (!LIN_WIDE || A.N <= 128 || big < 4 * device_cus()) lin_go<T, 128, 128, 2, 2, FWD, CUT>(A, st);
+    else lin_go<T, 128, 256, 2, 4, FWD, CUT>(A, st);
 }
 
 }  // namespace gatmi
 
 using namespace gatmi;
 
+extern "C" size_t gatmi_linear_fwd_workspace_bytes(const gatmi_linear *l) {
+    if (lin_check(l)) return 0;
+    return lin_geom(l).image_f;
+}
+
 extern "C" int gatmi_linear_fwd(const gatmi_linear *l, const void *x, const void *weight, const void *bias,
-                                const void *residual, void *y, void *slope, void *stream) {
+                                const void *residual, void *y, void *slope, void *ws, size_t ws_bytes, void *stream) {
     if (int e = lin_check(l)) return e;
     if (l->rows == 0) return GATMI_OK;
     GATMI_REQUIRE(x && weight && y, "linear_fwd: null argument");
+    const LinGeom G = lin_geom(l);
+    if (ws_bytes < G.image_f || (G.image_f && !ws)) {
+        set_error("linear workspace too small: %zu < %zu", ws_bytes, G.image_f);
+        return GATMI_ERR_WS;
+    }
     hipStream_t st = static_cast<hipStream_t>(stream);
     LinArgs A;
     memset(&A, 0, sizeof(A));
     A.A = x;
-    A.B = weight;
+    A.B = A.plain = weight;
     A.bias = bias;
     A.res = residual;
     A.C = y;
-    A.slope = slope;
+    A.slope = l->act == GATMI_ACT_NONE ? nullptr : slope;
+    A.act = l->act;
     A.M = l->rows;
     A.N = l->out_features;
-    A.K = l->in_features;
+    A.K = A.ldb = l->in_features;
     ProfScope ps("linear_fwd", st);
-    GATMI_WITH_TYPE(l->dtype, lin_launch_nt<T>(A, true, l->act, st));
+    if (l->rows <= kFewRows) {
+        GATMI_WITH_TYPE(l->dtype, {
+            auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((A.N + 3) / 4), dim3(256), 0, st, A); };
+            if (A.M == 1) go(lin_rows_kernel<T, 1>);
+            else if (A.M <= 4) go(lin_rows_kernel<T, 4>);
+            else go(lin_rows_kernel<T, kFewRows>);
+        });
+    } else if (G.image_fwd) {
+        hipLaunchKernelGGL((lin_image_kernel<float, false>), dim3((G.ldf + 31) / 32, (A.N + 31) / 32), dim3(256), 0, st,
+                           static_cast<const float *>(weight), A.N, A.K, G.ldf, ws);
+        A.B = ws;
+        A.ldb = G.ldf;
+        lin_launch_nt<float, true, true>(A, st);
+    } else {
+        GATMI_WITH_TYPE(l->dtype, (lin_launch_nt<T, true, false>(A, st)));
+    }
     GATMI_HIP(hipGetLastError());
     return GATMI_OK;
 }
@@ -538,7 +898,7 @@ extern "C" int gatmi_linear_fwd(const gatmi_linear *l, const void *x, const void
 extern "C" size_t gatmi_linear_bwd_workspace_bytes(const gatmi_linear *l) {
     if (lin_check(l)) return 0;
     const LinGeom G = lin_geom(l);
-    return G.dz + G.wt + G.part + G.slabs + 256;
+    return G.image_b + G.slabs + G.dbpart;
 }
 
 extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void *weight, const void *slope,
@@ -548,84 +908,60 @@ extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void
     GATMI_REQUIRE(l->rows == 0 || (x && weight && grad_y), "linear_bwd: null argument");
     GATMI_REQUIRE(l->act == GATMI_ACT_NONE || slope || l->rows == 0, "linear_bwd: the activation's slope is missing");
     const LinGeom G = lin_geom(l);
-    if (!ws || ws_bytes < G.dz + G.wt + G.part + G.slabs) {
-        set_error("linear workspace too small: %zu < %zu", ws_bytes, G.dz + G.wt + G.part + G.slabs);
+    if (!ws || ws_bytes < G.image_b + G.slabs + G.dbpart) {
+        set_error("linear workspace too small: %zu < %zu", ws_bytes, G.image_b + G.slabs + G.dbpart);
         return GATMI_ERR_WS;
     }
     hipStream_t st = static_cast<hipStream_t>(stream);
-    char *base = static_cast<char *>(ws);
+    char *image = static_cast<char *>(ws);
+    float *slabs = reinterpret_cast<float *>(image + G.image_b), *dbpart = reinterpret_cast<float *>(image + G.image_b + G.slabs);
     const int N = l->out_features, K = l->in_features;
-    const bool has_act = l->act != GATMI_ACT_NONE;
-    float *part = reinterpret_cast<float *>(base + G.dz + G.wt), *slabs = reinterpret_cast<float *>(base + G.dz + G.wt + G.part);
-    const void *dz = has_act ? base : grad_y;
-    if (l->rows > 0 && (has_act || grad_bias)) {
-        ProfScope ps("linear_dz", st);
-        GATMI_WITH_TYPE(l->dtype, {
-            constexpr int VM = 16 / sizeof(T);
-            const int v = N >= VM ? VM : (N >= 4 && VM == 8 ? 4 : (N >= 2 ? 2 : 1));
-            const dim3 grid(G.dz_blocks, ((N + v - 1) / v + 255) / 256);
-            auto go = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, static_cast<const T *>(grad_y),
-                                   static_cast<const typename SlopeOf<T>::type *>(slope), reinterpret_cast<T *>(base),
-                                   grad_bias ? part : nullptr, (long long)l->rows, N);
-            };
-            if (has_act) {
-                if (v == VM) go(lin_dz_kernel<T, VM, true>);
-                else if (v == 4) go(lin_dz_kernel<T, 4, true>);
-                else if (v == 2) go(lin_dz_kernel<T, 2, true>);
-                else go(lin_dz_kernel<T, 1, true>);
-            } else {
-                if (v == VM) go(lin_dz_kernel<T, VM, false>);
-                else if (v == 4) go(lin_dz_kernel<T, 4, false>);
-                else if (v == 2) go(lin_dz_kernel<T, 2, false>);
-                else go(lin_dz_kernel<T, 1, false>);
-            }
-        });
-        GATMI_HIP(hipGetLastError());
-    }
-    if (grad_bias) {
-        ProfScope ps("linear_db", st);
-        GATMI_WITH_TYPE(l->dtype, hipLaunchKernelGGL((lin_db_kernel<T>), dim3((N + 7) / 8), dim3(256), 0, st, part,
-                                                     l->rows > 0 ? G.dz_blocks : 0, N, static_cast<T *>(grad_bias)));
-        GATMI_HIP(hipGetLastError());
-    }
+    LinArgs A;
+    memset(&A, 0, sizeof(A));
+    A.A = grad_y;
+    A.aslope = l->act == GATMI_ACT_NONE ? nullptr : slope;
+    A.M = l->rows;
     if (grad_x && l->rows > 0) {
         ProfScope ps("linear_dx", st);
+        A.plain = weight;
+        A.B = image;
+        A.C = grad_x;
+        A.N = K;
+        A.K = N;
+        A.ldb = G.ldb;
         GATMI_WITH_TYPE(l->dtype, {
-            T *wt = reinterpret_cast<T *>(base + G.dz);
-            hipLaunchKernelGGL((lin_transpose_kernel<T>), dim3((K + 31) / 32, (N + 31) / 32), dim3(256), 0, st,
-                               static_cast<const T *>(weight), N, K, wt);
-            LinArgs A;
-            memset(&A, 0, sizeof(A));
-            A.A = dz;
-            A.B = wt;
-            A.C = grad_x;
-            A.M = l->rows;
-            A.N = K;
-            A.K = N;
-            lin_launch_nt<T>(A, false, GATMI_ACT_NONE, st);
+            hipLaunchKernelGGL((lin_image_kernel<T, true>), dim3((G.ldb + 31) / 32, (K + 31) / 32), dim3(256), 0, st,
+                               static_cast<const T *>(weight), N, K, G.ldb, ws);
+            lin_launch_nt<T, false, IsF32<T>::value>(A, st);
         });
         GATMI_HIP(hipGetLastError());
     }
-    if (grad_weight) {
+    if (grad_weight || grad_bias) {
         ProfScope ps("linear_dw", st);
+        A.plain = nullptr;
+        A.B = x;
+        A.N = N;
+        A.K = K;
+        A.part = slabs;
+        A.dbpart = grad_bias ? dbpart : nullptr;
+        A.per_split = G.per_split;
         GATMI_WITH_TYPE(l->dtype, {
-            LinArgs A;
-            memset(&A, 0, sizeof(A));
-            A.A = dz;
-            A.B = x;
-            A.M = l->rows;
-            A.N = N;
-            A.K = K;
-            A.part = slabs;
-            A.tiles_n = (K + kBN - 1) / kBN;
+#ifndef TN_WIDE
+#define TN_WIDE 1
+#endif
+            const bool wide = TN_WIDE && K > 128;
+            A.tiles_n = (K + (wide ? 255 : 127)) / (wide ? 256 : 128);
             A.tiles = (long long)((N + kBM - 1) / kBM) * A.tiles_n;
-            A.per_split = G.per_split;
-            hipLaunchKernelGGL((lin_tn_kernel<T>), dim3((unsigned)(A.tiles * G.splits)), dim3(256), 0, st, A);
+            auto tn = N < 8 || K < 8 ? (wide ? lin_tn_kernel<T, 256, true> : lin_tn_kernel<T, 128, true>)
+                                     : (wide ? lin_tn_kernel<T, 256, false> : lin_tn_kernel<T, 128, false>);
+            hipLaunchKernelGGL(tn, dim3((unsigned)(A.tiles * G.splits)), dim3(wide ? 512 : 256), 0, st, A);
             const long long size = (long long)N * K;
-            const long long b = (size + 255) / 256;
-            hipLaunchKernelGGL((lin_slabs_kernel<T>), dim3((unsigned)(b > 4096 ? 4096 : b)), dim3(256), 0, st, slabs,
-                               G.splits, size, static_cast<T *>(grad_weight));
+            if (grad_weight)
+                hipLaunchKernelGGL((lin_slabs_kernel<T>), dim3((unsigned)((size + 63) / 64)), dim3(256), 0, st, slabs,
+                                   G.splits, size, static_cast<T *>(grad_weight));
+            if (grad_bias)
+                hipLaunchKernelGGL((lin_db_kernel<T>), dim3((N + 7) / 8), dim3(256), 0, st, dbpart, G.splits, N,
+                                   static_cast<T *>(grad_bias));
         });
         GATMI_HIP(hipGetLastError());
     }

@@ -50,23 +50,49 @@ def _act(name: str, act: str) -> int:
     return code
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream      # the current stream's handle, without a Stream object
+_current = torch._C._cuda_getDevice
+
+
 class _on:
-    """The tensor's device made current, when it is not (a context manager costs more than a small kernel)."""
-    __slots__ = ("dev", "prev")
+    """The tensor's device made current when it is not, and its stream (torch's own context manager and
+    Stream object cost more than a small kernel)."""
+    __slots__ = ("index", "prev")
 
     def __init__(self, dev: torch.device):
-        self.dev = dev
+        self.index = dev.index
 
     def __enter__(self):
-        cur = torch.cuda.current_device()
-        self.prev = cur if cur != self.dev.index else None
+        prev = _current()
+        self.prev = prev if prev != self.index else None
         if self.prev is not None:
-            torch.cuda.set_device(self.dev)
-        return torch.cuda.current_stream(self.dev).cuda_stream
+            torch.cuda.set_device(self.index)
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc):
         if self.prev is not None:
             torch.cuda.set_device(self.prev)
+
+
+def _once(backward):
+    """A backward that cannot itself be differentiated.  Without create_graph nothing could, and the guard
+    (which costs as much as the call) is left out."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, grad_y):
+        return guarded(ctx, grad_y) if torch.is_grad_enabled() else backward(ctx, grad_y)
+    return staticmethod(run)
+
+
+class _NoCtx:
+    """Stands for autograd's context where nothing needs a gradient"""
+
+    def save_for_backward(self, *tensors):
+        pass
+
+
+def _apply(fn, needs_grad: bool, *args):
+    return fn.apply(*args) if needs_grad else fn.forward(_NoCtx(), *args)
 
 
 def _ptr(t: Optional[Tensor]):
@@ -88,14 +114,16 @@ class _LinearFn(torch.autograd.Function):
             slope = None
             if keep and act:
                 slope = torch.empty(y.shape, dtype=torch.float32 if dtype == 0 else torch.int16, device=dev)
+            need = lib.gatmi_linear_fwd_workspace_bytes(C.byref(desc))
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
             _lib.check(lib.gatmi_linear_fwd(C.byref(desc), x.data_ptr(), weight.data_ptr(), _ptr(bias),
-                                            _ptr(residual), y.data_ptr(), _ptr(slope), st), "gatmi_linear_fwd")
+                                            _ptr(residual), y.data_ptr(), _ptr(slope), _ptr(ws), need, st),
+                       "gatmi_linear_fwd")
         ctx.save_for_backward(x, weight, slope)
         ctx.desc = desc
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_y):
         x, weight, slope = ctx.saved_tensors
         lib, dev, desc = _lib.lib(), x.device, ctx.desc
@@ -130,9 +158,10 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: st
     if residual is not None and residual.shape != x.shape[:-1] + (weight.size(0),):
         raise ValueError(f"linear_act: residual must be {tuple(x.shape[:-1]) + (weight.size(0),)}, "
                          f"got {tuple(residual.shape)}")
-    keep = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
-                                        (bias is not None and bias.requires_grad))
-    return _LinearFn.apply(x, weight, bias, residual, dtype, code, keep)
+    grad = torch.is_grad_enabled()
+    keep = grad and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
+    needs = keep or (grad and residual is not None and residual.requires_grad)
+    return _apply(_LinearFn, needs, x, weight, bias, residual, dtype, code, keep)
 
 
 # ---- group norm ------------------------------------------------------------------------------
@@ -165,8 +194,7 @@ class _GroupNormFn(torch.autograd.Function):
         ctx.cfg = (groups, dtype, act, eps)
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_y):
         x, weight, bias, stats = ctx.saved_tensors
         lib, dev = _lib.lib(), x.device
@@ -203,7 +231,7 @@ def group_norm_act(x: Tensor, groups: int, weight: Tensor, bias: Tensor, eps: fl
     if not eps >= 0.0:
         raise ValueError(f"group_norm_act: eps must not be negative, got {eps}")
     keep = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias.requires_grad)
-    return _GroupNormFn.apply(x, weight, bias, groups, dtype, code, float(eps), keep)
+    return _apply(_GroupNormFn, keep, x, weight, bias, groups, dtype, code, float(eps), keep)
 
 
 # ---- embedding -------------------------------------------------------------------------------
@@ -221,8 +249,7 @@ class _EmbeddingFn(torch.autograd.Function):
         ctx.cfg = (dtype, vocab, dim, scale)
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_y):
         (ids,) = ctx.saved_tensors
         dtype, vocab, dim, scale = ctx.cfg
@@ -247,7 +274,7 @@ def embedding(ids: Tensor, table: Tensor, scale: float = 1.0) -> Tensor:
         raise TypeError(f"embedding: ids must be int64, got {ids.dtype}")
     if table.dim() != 2 or table.size(1) < 1:
         raise ValueError(f"embedding: table must be [entries, dim], got {tuple(table.shape)}")
-    return _EmbeddingFn.apply(ids, table, float(scale), dtype)
+    return _apply(_EmbeddingFn, torch.is_grad_enabled() and table.requires_grad, ids, table, float(scale), dtype)
 
 
 # ---- dropout ---------------------------------------------------------------------------------
@@ -271,8 +298,7 @@ class _DropoutFn(torch.autograd.Function):
         ctx.cfg = (p, seed if used is None else 0, dtype, residual is not None)
         return y
 
-    @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_y):
         (used,) = ctx.saved_tensors
         p, seed, dtype, _ = ctx.cfg
@@ -312,4 +338,5 @@ def dropout(x: Tensor, p: float, training: bool = True, seed=None, residual: Opt
         seed = int(torch.empty((), dtype=torch.int64).random_().item())
     else:
         seed = int(seed) & 0xFFFFFFFFFFFFFFFF
-    return _DropoutFn.apply(x, residual, float(p), seed, dtype)
+    needs = torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))
+    return _apply(_DropoutFn, needs, x, residual, float(p), seed, dtype)

@@ -479,8 +479,9 @@ typedef struct gatmi_linear {
 /*   x [rows, in], weight [out, in], bias [out] or NULL, residual [rows, out] or NULL -> y [rows, out]
  *   slope: NULL, or (act != NONE, a backward follows) the activation's derivative [rows, out]: float for
  *   f32 tensors, else uint16 of a private coding */
+size_t gatmi_linear_fwd_workspace_bytes(const gatmi_linear *l);   /* may be 0 (then ws may be NULL) */
 int gatmi_linear_fwd(const gatmi_linear *l, const void *x, const void *weight, const void *bias,
-                     const void *residual, void *y, void *slope, void *stream);
+                     const void *residual, void *y, void *slope, void *ws, size_t ws_bytes, void *stream);
 /*   slope: what the forward wrote (NULL when act == NONE);  grad_y [rows, out]
  *   -> grad_x [rows, in], grad_weight [out, in], grad_bias [out], each NULL to skip.  The residual's
  *   gradient is grad_y itself. */

@@ -28,7 +28,7 @@ def test_linear_refusals(fields, word):
     d = _lib.Linear(4, 8, 8, 0, 0)
     for k, v in fields.items():
         setattr(d, k, v)
-    for code in (lib.gatmi_linear_fwd(C.byref(d), 256, 256, None, None, 256, None, None),
+    for code in (lib.gatmi_linear_fwd(C.byref(d), 256, 256, None, None, 256, None, 256, 1 << 30, None),
                  lib.gatmi_linear_bwd(C.byref(d), 256, 256, None, 256, None, None, None, 256, 1 << 30, None)):
         code, msg = rc(code)
         assert code == 1 and word in msg
@@ -38,14 +38,17 @@ def test_linear_refusals(fields, word):
 def test_linear_null_and_workspace():
     lib = _lib.lib()
     d = _lib.Linear(4, 8, 8, 0, 2)
-    assert rc(lib.gatmi_linear_fwd(C.byref(d), None, 256, None, None, 256, None, None))[0] == 1
-    assert rc(lib.gatmi_linear_fwd(None, 256, 256, None, None, 256, None, None))[0] == 1
+    assert rc(lib.gatmi_linear_fwd(C.byref(d), None, 256, None, None, 256, None, None, 0, None))[0] == 1
+    assert rc(lib.gatmi_linear_fwd(None, 256, 256, None, None, 256, None, None, 0, None))[0] == 1
     code, msg = rc(lib.gatmi_linear_bwd(C.byref(d), 256, 256, None, 256, 256, 256, 256, 256, 1 << 30, None))
     assert code == 1 and "slope" in msg
     code, msg = rc(lib.gatmi_linear_bwd(C.byref(d), 256, 256, 256, 256, 256, 256, 256, 256, 16, None))
     assert code == 4 and "workspace" in msg
     d.rows = 0
-    assert lib.gatmi_linear_fwd(C.byref(d), None, None, None, None, None, None, None) == 0
+    assert lib.gatmi_linear_fwd(C.byref(d), None, None, None, None, None, None, None, 0, None) == 0
+    d.rows = 1 << 20
+    code, msg = rc(lib.gatmi_linear_fwd(C.byref(d), 256, 256, None, None, 256, None, None, 0, None))
+    assert code == 4 and "workspace" in msg
 
 
 @pytest.mark.parametrize("fields,word", [
