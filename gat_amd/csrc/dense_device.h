@@ -7,6 +7,7 @@
 #include <type_traits>
 
 #include "../../include/gat_mi355.h"
+#include "attn_device.h"
 
 namespace gatmi {
 
@@ -69,17 +70,28 @@ __device__ __forceinline__ uint32_t fdiv(const FastDiv &f, uint32_t n) {
 // tensors.  Otherwise (results are rounded to 16 bits) v_exp_f32 forms, whose error of a few 2^-22 is a
 // hundredth of that rounding.
 template <bool EXACT> __device__ __forceinline__ float act_exp(float v) {
-    if constexpr (EXACT) return expf(v);
+    if constexpr (EXACT) return expf(v);   // of either sign
     return __builtin_amdgcn_exp2f(v * 1.44269502162933349609375f);
 }
 
 // exp(z) - 1 for z <= 0
 template <bool EXACT> __device__ __forceinline__ float act_expm1(float z) {
-    if constexpr (EXACT) return expm1f(z);
+    if constexpr (EXACT) {
+        // above -0.35 the series to z^8 / 8! (what follows is below 2^-30 of the sum); below it exp(z) <= 0.705
+        // and the subtraction leaves an error of exp's own 1.5 steps of at most 2^-24 against 0.295 or more
+        float s = fmaf(z, 2.4801587e-5f, 1.9841270e-4f);
+        s = fmaf(z, s, 1.3888889e-3f);
+        s = fmaf(z, s, 8.3333333e-3f);
+        s = fmaf(z, s, 4.1666668e-2f);
+        s = fmaf(z, s, 1.6666667e-1f);
+        s = fmaf(z, s, 0.5f);
+        s = fmaf(z * z, s, z);
+        return z < -0.35f ? exp_fast(z) - 1.0f : s;      // NaN: s
+    }
     // next to 0 the subtraction would cancel: z + z^2/2 + z^3/6, off by z^3/24 relative (< 2^-20 there)
     const float e = act_exp<false>(z) - 1.0f;
     const float s = z * fmaf(z, fmaf(z, 0.16666667f, 0.5f), 1.0f);
-    return z > -0.03f ? s : e;
+    return z < -0.03f ? e : s;
 }
 
 // The normal distribution function.  16-bit results: 1 - t(a1 + .. + a5 t^4) exp(-z^2/2) with
@@ -123,7 +135,7 @@ template <int ACT, bool EXACT> __device__ __forceinline__ float act_both(float z
     }
     if constexpr (ACT == GATMI_ACT_ELU) {
         const float e = act_expm1<EXACT>(z);
-        d = z > 0.f ? 1.f : (EXACT ? expf(z) : e + 1.f);
+        d = z > 0.f ? 1.f : e + 1.f;      // exp(z), to a step of 1
         return z > 0.f ? z : e;
     }
     if constexpr (ACT == GATMI_ACT_SILU) {

@@ -279,19 +279,12 @@ template <class T, int ACT> __device__ __forceinline__ void epi_values(float (&v
 }
 template <class T, bool FWD>
 __device__ __forceinline__ void epi_piece(const LinArgs &A, long long m, int n, int have, float (&v)[8],
-                                          const float (&bias)[8]) {
+                                          const float (&bias)[8], const Gran<T> &res) {
     typedef typename SlopeOf<T>::type ST;
     const long long at = m * A.N + n;
     T *out = static_cast<T *>(A.C) + at;
     ST sl[8];
     if constexpr (FWD) {
-        const T *res = A.res ? static_cast<const T *>(A.res) + at : nullptr;
-        VecF<8> rr;
-        if (res) {
-            if (have >= 8) rr = ldv<T, 8>(res);
-            else
-                for (int k = 0; k < 8; ++k) rr.e[k] = k < have ? (float)res[k] : 0.f;
-        }
         GATMI_WITH_ACT(A.act, epi_values<T, ACT>(v, bias, sl));
         if (A.slope) {
             ST *so = static_cast<ST *>(A.slope) + at;
@@ -307,9 +300,11 @@ __device__ __forceinline__ void epi_piece(const LinArgs &A, long long m, int n, 
                     if (k < have) so[k] = sl[k];
             }
         }
-        if (res)
+        if (A.res) {
+            const VecF<8> rr = gran_values<T>(res);
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] += rr.e[k];
+        }
     }
     if (have >= 8) {
         VecF<8> o;
@@ -336,9 +331,9 @@ template <bool FWD> __device__ __forceinline__ float plain_dot(const LinArgs &A,
 
 // C[m][n] = epilogue(sum_k A[m][k] B[n][k]).  FWD: bias, activation, residual, slope; else A = dy * aslope
 // when given.  CUT (f32): B comes as three planes of bf16 pieces, rows of ldb (a multiple of 8, zeros behind K).
-// SHORT: K < 8.
-template <class T, int BM, int BN, int WM, int WN, bool FWD, bool CUT, bool SHORT>
-__global__ __launch_bounds__(WM * WN * 64) void lin_nt_kernel(const LinArgs A) {
+// SHORT: K < 8; SHORT_N: N < 8.
+template <class T, int BM, int BN, int WM, int WN, bool FWD, bool CUT, bool SHORT, bool SHORT_N>
+__global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void lin_nt_kernel(const LinArgs A) {
     typedef Tile<T, BM> TA;
     typedef Tile<T, BN> TB;
     constexpr int THREADS = WM * WN * 64, MI = BM / WM / 32, NI = BN / WN / 32;
@@ -451,12 +446,31 @@ __global__ __launch_bounds__(WM * WN * 64) void lin_nt_kernel(const LinArgs A) {
     const int half = lane >> 5, c8 = (lane % PR) * 8, rr = lane / PR;
     const int n = n0 + wn + c8;
     const int have = A.N - n;                       // columns of this piece that exist
+    // the residual's pieces of a 32-row block are on their way before the first of them is used
+    constexpr int PP = 16 / RI;
+    Gran<T> res[2][PP];
+    auto fetch_res = [&](int i) {
+        const T *br = static_cast<const T *>(A.res) + (m0 + wm) * A.N;
+        const long long left = A.M - 1 - (m0 + wm);
+        const int nc = SHORT_N || n <= A.N - 8 ? n : A.N - 8;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int p = 0; p < PP; ++p) {
+                const int r = i * 32 + h * 16 + p * RI + rr;
+                // a wave whose rows all lie behind the matrix reads the row before them
+                const long long at = (r < left ? r : left) * (long long)A.N + nc;
+                if constexpr (SHORT_N) res[h][p] = ld_gran_short<T>(br + at, 0, have);
+                else res[h][p] = ld_gran<T>(br + at, 0);
+            }
+    };
     float bias[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k)
         bias[k] = FWD && A.bias && k < have ? (float)static_cast<const T *>(A.bias)[n + k] : 0.f;
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+    for (int i = 0; i < MI; ++i) {
+        if (FWD && A.res) fetch_res(i);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             // the wave's own LDS, in order: what it stored before is read before it stores again
@@ -486,9 +500,11 @@ __global__ __launch_bounds__(WM * WN * 64) void lin_nt_kernel(const LinArgs A) {
                         for (int k = 0; k < 8; ++k) v[k] = row[k];
                     }
                 }
-                epi_piece<T, FWD>(A, m, n, have, v, bias);
+                if (FWD && !SHORT_N && have < 8 && A.res) shift_down<T>(res[h][p].w, 8 - have);
+                epi_piece<T, FWD>(A, m, n, have, v, bias, res[h][p]);
             }
         }
+    }
 }
 
 // A tile of the transposed product in LDS, as it lies in memory: contraction steps (rows of the matrix) by
@@ -822,24 +838,23 @@ static LinGeom lin_geom(const gatmi_linear *l) {
     return G;
 }
 
-template <class T, int BM, int BN, int WM, int WN, bool FWD, bool CUT, bool SHORT = false> static void lin_go(LinArgs &A, hipStream_t st) {
+template <class T, int BM, int BN, int WM, int WN, bool FWD, bool CUT, bool SHORT = false, bool SHORT_N = false>
+static void lin_go(LinArgs &A, hipStream_t st) {
     A.tiles_n = (A.N + BN - 1) / BN;
     A.tiles = (A.M + BM - 1) / BM * A.tiles_n;
     const unsigned grid = (unsigned)((A.tiles + 7) / 8 * 8);
-    hipLaunchKernelGGL((lin_nt_kernel<T, BM, BN, WM, WN, FWD, CUT, SHORT>), dim3(grid), dim3(WM * WN * 64), 0, st, A);
+    hipLaunchKernelGGL((lin_nt_kernel<T, BM, BN, WM, WN, FWD, CUT, SHORT, SHORT_N>), dim3(grid), dim3(WM * WN * 64), 0, st, A);
 }
 // The tile: narrow ones for narrow results; 64 x 64 while larger ones would leave compute units idle
 template <class T, bool FWD, bool CUT> static void lin_launch_nt(LinArgs A, hipStream_t st) {
     const long long big = (A.M + 127) / 128 * ((A.N + 127) / 128);
-    if (A.K < 8) lin_go<T, 64, 64, 2, 2, FWD, CUT, true>(A, st);
+    if (A.K < 8) lin_go<T, 64, 64, 2, 2, FWD, CUT, true, true>(A, st);
+    else if (A.N < 8) lin_go<T, 128, 32, 4, 1, FWD, CUT, false, true>(A, st);
     else if (A.N <= 32) lin_go<T, 128, 32, 4, 1, FWD, CUT>(A, st);
     else if (big < device_cus()) lin_go<T, 64, 64, 2, 2, FWD, CUT>(A, st);
     else if (A.N <= 64) lin_go<T, 128, 64, 4, 1, FWD, CUT>(A, st);
-#ifndef LIN_WIDE
-#define LIN_WIDE 1
-#endif
-    else if (!LIN_WIDE || A.N <= 128 || big < 4 * device_cus()) lin_go<T, 128, 128, 2, 2, FWD, CUT>(A, st);
-    else lin_go<T, 128, 256, 2, 4, FWD, CUT>(A, st);
+    else if (A.N <= 64) lin_go<T, 128, 64, 4, 1, FWD, CUT>(A, st);
+    else lin_go<T, 128, 128, 2, 2, FWD, CUT>(A, st);
 }
 
 }  // namespace gatmi
@@ -946,10 +961,7 @@ extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void
         A.dbpart = grad_bias ? dbpart : nullptr;
         A.per_split = G.per_split;
         GATMI_WITH_TYPE(l->dtype, {
-#ifndef TN_WIDE
-#define TN_WIDE 1
-#endif
-            const bool wide = TN_WIDE && K > 128;
+            const bool wide = K > 128;      // dz is made once for twice the columns of x
             A.tiles_n = (K + (wide ? 255 : 127)) / (wide ? 256 : 128);
             A.tiles = (long long)((N + kBM - 1) / kBM) * A.tiles_n;
             auto tn = N < 8 || K < 8 ? (wide ? lin_tn_kernel<T, 256, true> : lin_tn_kernel<T, 128, true>)
