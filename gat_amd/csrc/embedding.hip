@@ -60,15 +60,16 @@ template <class T, int V> __global__ __launch_bounds__(256) void emb_fwd_kernel(
 }
 
 // ---- stable radix sort of (id, position) ---------------------------------------------------------
-// `bits` (at most 11) of the key a pass, so that up to 4 M table entries take two passes.  A block owns a
+// `bits` (at most 9) of the key a pass: with more, a tile's runs of equal digits get shorter than a cache
+// line and the scattered stores cost more than the pass saved.  A block owns a
 // tile of 256 * ITEMS consecutive items; wave w of it the items [w * 64 * ITEMS, ..), 64 at a time: an
 // item's rank is what came before it in (tile, wave, step, lane) order, which is the order of the items.
-constexpr int kSortMaxBits = 11, kSmallSort = 4096;
+constexpr int kSortMaxBits = 9, kSmallSort = 4096;
 
 struct SortArgs {
     const int64_t *ids;            // first pass: keys come from here, positions are the indices
-    const uint32_t *key_in, *pos_in;
-    uint32_t *key_out, *pos_out;
+    const uint2 *in;               // later ones: (key, position)
+    uint2 *out;
     uint32_t *hist;                // [bins][blocks]
     uint32_t *total;               // [bins]
     long long n, vocab;
@@ -80,7 +81,7 @@ __device__ __forceinline__ uint32_t id_key(int64_t id, long long vocab) {
     return (uint32_t)(id >= 0 && id < vocab ? id : vocab);
 }
 __device__ __forceinline__ uint32_t sort_key(const SortArgs &A, long long i) {
-    return A.ids ? id_key(A.ids[i], A.vocab) : A.key_in[i];
+    return A.ids ? id_key(A.ids[i], A.vocab) : A.in[i].x;
 }
 
 // Lanes of this wave whose digit equals this lane's (only lanes with `on` count)
@@ -158,30 +159,6 @@ __global__ __launch_bounds__(256) void sort_scan_kernel(const SortArgs A) {
     if (threadIdx.x == 0) A.total[blockIdx.x] = carry;
 }
 
-// thread t owns the bins / 256 digits from t * that on (bins < 256: one each): turns the counts of
-// the tile's four waves in cnt [4][bins] into where their items start, `start(d)` being the digit's first
-// place for this tile and `total(d)` its items in all
-template <class S, class C>
-__device__ __forceinline__ void digit_starts(volatile uint32_t *cnt, int bins, uint32_t *wsum, S place, C total) {
-    const int per = bins > 256 ? bins / 256 : 1;
-    const int d0 = threadIdx.x * per;
-    uint32_t sum = 0;
-    for (int q = 0; q < per; ++q)
-        if (d0 + q < bins) sum += total(d0 + q);
-    uint32_t at = block_scan(sum, wsum);
-    for (int q = 0; q < per; ++q) {
-        const int d = d0 + q;
-        if (d >= bins) break;
-        uint32_t to = at + place(d);
-        at += total(d);
-        for (int w = 0; w < 4; ++w) {
-            const uint32_t c = cnt[w * bins + d];
-            cnt[w * bins + d] = to;
-            to += c;
-        }
-    }
-}
-
 template <int ITEMS> __global__ __launch_bounds__(256) void sort_scatter_kernel(const SortArgs A) {
     extern __shared__ uint32_t smem[];
     __shared__ uint32_t wsum[4];
@@ -198,22 +175,51 @@ template <int ITEMS> __global__ __launch_bounds__(256) void sort_scatter_kernel(
     for (int k = 0; k < ITEMS; ++k) {
         const long long i = base + k * 64 + lane;
         const bool on = k * 64 + lane < have;
-        key[k] = on ? sort_key(A, i) : 0u;
-        pos[k] = on ? (A.ids ? (uint32_t)i : A.pos_in[i]) : 0u;
+        uint2 e = make_uint2(0u, 0u);
+        if (on) e = A.ids ? make_uint2(id_key(A.ids[i], A.vocab), (uint32_t)i) : A.in[i];
+        key[k] = e.x;
+        pos[k] = e.y;
         digit[k] = (key[k] >> A.shift) & (bins - 1);
     }
     wave_ranks<ITEMS>(cnt + wave * bins, digit, have, A.bits, lane, rank);
     __syncthreads();
-    digit_starts(cnt, bins, wsum, [&](int d) { return A.hist[(long long)d * A.blocks + blockIdx.x]; },
-                 [&](int d) { return A.total[d]; });
+    // the tile's own order first, in LDS: neighbours in it go to neighbouring places, and the stores of a wave
+    // become runs instead of 64 separate ones
+    uint2 *tile = reinterpret_cast<uint2 *>(smem + 5 * bins);
+    uint32_t *shift = smem + 4 * bins;       // [bins]: a digit's place in the output less its place in the tile
+    {
+        const int per = bins > 256 ? bins / 256 : 1, d0 = threadIdx.x * per;
+        uint32_t mine = 0, all = 0;
+        for (int q = 0; q < per; ++q)
+            if (d0 + q < bins) {
+                for (int w = 0; w < 4; ++w) mine += cnt[w * bins + d0 + q];
+                all += A.total[d0 + q];
+            }
+        uint32_t here = block_scan(mine, wsum), there = block_scan(all, wsum);
+        for (int q = 0; q < per; ++q) {
+            const int d = d0 + q;
+            if (d >= bins) break;
+            shift[d] = there + A.hist[(long long)d * A.blocks + blockIdx.x] - here;
+            there += A.total[d];
+            for (int w = 0; w < 4; ++w) {
+                const uint32_t c = cnt[w * bins + d];
+                cnt[w * bins + d] = here;
+                here += c;
+            }
+        }
+    }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k)
-        if (k * 64 + lane < have) {
-            const uint32_t to = cnt[wave * bins + digit[k]] + rank[k];
-            A.key_out[to] = key[k];
-            A.pos_out[to] = pos[k];
-        }
+        if (k * 64 + lane < have) tile[cnt[wave * bins + digit[k]] + rank[k]] = make_uint2(key[k], pos[k]);
+    __syncthreads();
+    const long long first = (long long)blockIdx.x * (256 * ITEMS);
+    const int n = A.n - first < 256 * ITEMS ? (int)(A.n - first) : 256 * ITEMS;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const uint2 e = tile[i];
+        A.out[i + shift[(e.x >> A.shift) & (bins - 1)]] = e;
+    }
 }
 
 // at most kSmallSort items: all passes in one block, through LDS
@@ -240,9 +246,14 @@ __global__ __launch_bounds__(256) void sort_small_kernel(const SortArgs A) {
         __syncthreads();
         wave_ranks<ITEMS>(cnt + wave * bins, digit, have, 8, lane, rank);
         __syncthreads();
-        uint32_t mine = 0;      // thread d: the tile is all there is, its counts are the totals
+        uint32_t mine = 0;      // thread d: digit d
         for (int w = 0; w < 4; ++w) mine += cnt[w * bins + threadIdx.x];
-        digit_starts(cnt, bins, wsum, [&](int) { return 0u; }, [&](int) { return mine; });
+        uint32_t at = block_scan(mine, wsum);
+        for (int w = 0; w < 4; ++w) {
+            const uint32_t c = cnt[w * bins + threadIdx.x];
+            cnt[w * bins + threadIdx.x] = at;
+            at += c;
+        }
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < ITEMS; ++k)
@@ -263,8 +274,7 @@ __global__ __launch_bounds__(256) void sort_small_kernel(const SortArgs A) {
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k)
         if (k * 64 + lane < have) {
-            A.key_out[base + k * 64 + lane] = key[k];
-            A.pos_out[base + k * 64 + lane] = pos[k];
+            A.out[base + k * 64 + lane] = make_uint2(key[k], pos[k]);
         }
 }
 
@@ -276,11 +286,10 @@ __global__ __launch_bounds__(256) void sort_small_kernel(const SortArgs A) {
 constexpr uint32_t kNoKey = 0xffffffffu;
 
 struct SegArgs {
-    const uint32_t *key, *pos;    // level 0: sorted keys and positions
-    const uint32_t *flag;         // level > 0: 1 where the entry carries a row
+    const uint2 *entry;           // (key, position) at level 0; above (key, 1 where the entry carries a row)
     const void *src;              // level 0: dy; level > 0: f32 partial rows
     void *out;                    // dtable
-    uint32_t *nkey, *nflag;       // next level's entries, two a chunk
+    uint2 *nentry;                // next level's entries, two a chunk
     float *nsrc;
     long long n;
     uint32_t vocab;
@@ -300,8 +309,8 @@ __global__ __launch_bounds__(256) void seg_sum_kernel(const SegArgs A) {
     const int j = !on ? 0 : (j0 + V <= A.dim ? j0 : A.dim - V);
     const S *src = static_cast<const S *>(A.src) + j;
     T *out = static_cast<T *>(A.out) + j;
-    const uint32_t before = e0 > 0 ? A.key[e0 - 1] : kNoKey, after = e1 < A.n ? A.key[e1] : kNoKey;
-    const uint32_t head = A.key[e0], tail = A.key[e1 - 1];
+    const uint32_t before = e0 > 0 ? A.entry[e0 - 1].x : kNoKey, after = e1 < A.n ? A.entry[e1].x : kNoKey;
+    const uint32_t head = A.entry[e0].x, tail = A.entry[e1 - 1].x;
     const bool open_head = head < A.vocab && head == before;
     const bool open_tail = tail < A.vocab && tail == after;
     uint32_t k0 = kNoKey, k1 = kNoKey, f0 = 0, f1 = 0;
@@ -318,8 +327,9 @@ __global__ __launch_bounds__(256) void seg_sum_kernel(const SegArgs A) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const long long i = e + u < e1 ? e + u : e1 - 1;
-            k_[u] = A.key[i];
-            p_[u] = LEAF ? A.pos[i] : A.flag[i];
+            const uint2 en = A.entry[i];
+            k_[u] = en.x;
+            p_[u] = en.y;
         }
     };
     entries(e0, kn, pn);
@@ -374,11 +384,9 @@ __global__ __launch_bounds__(256) void seg_sum_kernel(const SegArgs A) {
             stv<T, V>(out + (long long)cur * A.dim, acc);
         }
     }
-    if (lane == 0 && blockIdx.y == 0 && A.nkey) {
-        A.nkey[2 * c] = k0;
-        A.nkey[2 * c + 1] = k1;
-        A.nflag[2 * c] = f0;
-        A.nflag[2 * c + 1] = f1;
+    if (lane == 0 && blockIdx.y == 0 && A.nentry) {
+        A.nentry[2 * c] = make_uint2(k0, f0);
+        A.nentry[2 * c + 1] = make_uint2(k1, f1);
     }
 }
 
@@ -454,24 +462,20 @@ extern "C" int gatmi_embedding_fwd(int32_t dtype, int64_t n, int64_t vocab, int6
 }
 
 struct EmbWs {
-    uint32_t *key[2], *pos[2], *hist, *total;
-    uint32_t *lkey[2], *lflag[2];
+    uint2 *pair[2], *lentry[2];
+    uint32_t *hist, *total;
     float *lsrc[2];
     size_t bytes;
 };
 static EmbWs emb_carve(const EmbGeom &G, long long dim, void *ws) {
     Carver cv(ws);
     EmbWs w;
-    for (int i = 0; i < 2; ++i) {
-        w.key[i] = cv.take<uint32_t>(G.n);
-        w.pos[i] = cv.take<uint32_t>(G.n);
-    }
+    for (int i = 0; i < 2; ++i) w.pair[i] = cv.take<uint2>(G.n);
     w.hist = cv.take<uint32_t>((1ll << G.bits) * G.blocks);
     w.total = cv.take<uint32_t>(1ll << G.bits);
     for (int i = 0; i < 2; ++i) {        // levels 1, 3, .. and 2, 4, ..
         const long long m = G.levels > 1 + i ? G.entries[1 + i] : 0;
-        w.lkey[i] = cv.take<uint32_t>(m);
-        w.lflag[i] = cv.take<uint32_t>(m);
+        w.lentry[i] = cv.take<uint2>(m);
         w.lsrc[i] = cv.take<float>(m * dim);
     }
     w.bytes = cv.off + 256;
@@ -526,23 +530,20 @@ extern "C" int gatmi_embedding_bwd(int32_t dtype, int64_t n, int64_t vocab, int6
         S.passes = G.passes;
         if (n <= kSmallSort) {
             S.ids = ids;
-            S.key_out = w.key[(G.passes - 1) & 1];
-            S.pos_out = w.pos[(G.passes - 1) & 1];
+            S.out = w.pair[(G.passes - 1) & 1];
             hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(256), 0, st, S);
         }
         for (int p = 0; n > kSmallSort && p < G.passes; ++p) {
             const size_t bins = (size_t)1 << G.bits;
             S.ids = p == 0 ? ids : nullptr;
-            S.key_in = w.key[(p + 1) & 1];
-            S.pos_in = w.pos[(p + 1) & 1];
-            S.key_out = w.key[p & 1];
-            S.pos_out = w.pos[p & 1];
+            S.in = w.pair[(p + 1) & 1];
+            S.out = w.pair[p & 1];
             S.shift = G.bits * p;
             auto count = G.items == 16 ? sort_count_kernel<16> : sort_count_kernel<4>;
             auto scatter = G.items == 16 ? sort_scatter_kernel<16> : sort_scatter_kernel<4>;
             hipLaunchKernelGGL(count, dim3(G.blocks), dim3(256), bins * 4, st, S);
             hipLaunchKernelGGL(sort_scan_kernel, dim3((unsigned)bins), dim3(256), 0, st, S);
-            hipLaunchKernelGGL(scatter, dim3(G.blocks), dim3(256), bins * 16, st, S);
+            hipLaunchKernelGGL(scatter, dim3(G.blocks), dim3(256), bins * 20 + 2048ll * G.items, st, S);
         }
         GATMI_HIP(hipGetLastError());
     }
@@ -557,13 +558,10 @@ extern "C" int gatmi_embedding_bwd(int32_t dtype, int64_t n, int64_t vocab, int6
     for (int l = 0; l < G.levels; ++l) {
         A.n = G.entries[l];
         A.chunk = l == 0 ? G.chunk0 : G.chunk;
-        A.key = l == 0 ? w.key[last] : w.lkey[(l - 1) & 1];
-        A.pos = w.pos[last];
-        A.flag = l == 0 ? nullptr : w.lflag[(l - 1) & 1];
+        A.entry = l == 0 ? w.pair[last] : w.lentry[(l - 1) & 1];
         A.src = l == 0 ? grad_y : w.lsrc[(l - 1) & 1];
         const bool more = l + 1 < G.levels;
-        A.nkey = more ? w.lkey[l & 1] : nullptr;
-        A.nflag = w.lflag[l & 1];
+        A.nentry = more ? w.lentry[l & 1] : nullptr;
         A.nsrc = w.lsrc[l & 1];
         // f32 partial rows take vectors of their own width
         const int v = l == 0 ? vec_of(dtype, dim) : vec_of(GATMI_F32, dim);

@@ -286,27 +286,26 @@ __device__ __forceinline__ GnWalk gn_walk(int width) {
 __global__ __launch_bounds__(256) void gn_finalize_kernel(const GnArgs A) {
     __shared__ double red[256];
     const int g = blockIdx.x;
-    const long long per = (A.length + A.chunks - 1) / A.chunks;
+    const int per = (int)((A.length + A.chunks - 1) / A.chunks);
+    const int full = (int)(A.length / per), rest = (int)(A.length - (long long)full * per);
     const float *p = A.part + (long long)blockIdx.y * A.chunks * 2 * A.C + g * A.width;
-    auto rows = [&](int c) -> double {
-        const long long r0 = c * per, r1 = r0 + per < A.length ? r0 + per : A.length;
-        return r1 > r0 ? (double)(r1 - r0) : 0.0;
-    };
     const GnWalk w = gn_walk(A.width);
-    double s = 0.0;
-    for (int j = w.j; j < A.width; j += w.jstep)
-#pragma unroll 8
-        for (int c = w.c; c < A.chunks; c += w.step) s += rows(c) * p[(long long)c * 2 * A.C + j];
-    const double count = (double)A.length * A.width;
-    const double mean = block_sum(s, red) / count;
-    s = 0.0;
+    // deviations from one of the chunk means: what a difference of squares loses is then of the spread's size
+    const float ref = p[0];
+    double s = 0.0, q = 0.0;
     for (int j = w.j; j < A.width; j += w.jstep)
 #pragma unroll 8
         for (int c = w.c; c < A.chunks; c += w.step) {
-            const double d = p[(long long)c * 2 * A.C + j] - mean;
-            s += p[(long long)c * 2 * A.C + A.C + j] + rows(c) * d * d;
+            const double rows = c < full ? per : (c == full ? rest : 0);
+            const double d = (double)p[(long long)c * 2 * A.C + j] - ref;
+            const double nd = rows > 0.0 ? rows * d : 0.0;
+            s += nd;
+            q += p[(long long)c * 2 * A.C + A.C + j] + nd * d;
         }
-    const double var = block_sum(s, red) / count;
+    const double count = (double)A.length * A.width;
+    const double off = block_sum(s, red) / count, mean = ref + off;
+    double var = block_sum(q, red) / count - off * off;
+    var = var < 0.0 ? 0.0 : var;
     if (threadIdx.x == 0) {
         A.mean[(long long)blockIdx.y * A.groups + g] = (float)mean;
         A.rstd[(long long)blockIdx.y * A.groups + g] = (float)(1.0 / sqrt(var + (double)A.eps));
@@ -359,7 +358,7 @@ template <class T, int V, int ACT> __global__ __launch_bounds__(256) void gn_red
     if (L.on) {
         GnCols<T, V> P;
         P.load(A, L.off, blockIdx.y);
-#pragma unroll 2
+#pragma unroll 4
         for (long long r = L.r0 + L.rsub; r < L.r1; r += L.rpp) {
             const VecF<V> v = ldv<T, V>(x + r * A.C), g = ldv<T, V>(dy + r * A.C);
 #pragma unroll

@@ -536,7 +536,6 @@ template <class T, int C> struct TileT {
         const char *at = lds + p * PLANE + row * STRIDE + col * 2;
         const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at));
         const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 4 * STRIDE));
-        typedef short v8s __attribute__((ext_vector_type(8)));
         return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 };
@@ -852,7 +851,6 @@ template <class T, bool FWD, bool CUT> static void lin_launch_nt(LinArgs A, hipS
     else if (A.N < 8) lin_go<T, 128, 32, 4, 1, FWD, CUT, false, true>(A, st);
     else if (A.N <= 32) lin_go<T, 128, 32, 4, 1, FWD, CUT>(A, st);
     else if (big < device_cus()) lin_go<T, 64, 64, 2, 2, FWD, CUT>(A, st);
-    else if (A.N <= 64) lin_go<T, 128, 64, 4, 1, FWD, CUT>(A, st);
     else if (A.N <= 64) lin_go<T, 128, 64, 4, 1, FWD, CUT>(A, st);
     else lin_go<T, 128, 128, 2, 2, FWD, CUT>(A, st);
 }
