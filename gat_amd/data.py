@@ -13,10 +13,11 @@ import torch
 
 class Data:
     """x float32 [N, F], edge_index int64 [2, E] (row 0 = source, row 1 = destination),
-    y int64 [N]; num_features == x.size(1) as torch_geometric.data.Data reports it."""
+    y int64 [N]; num_features == x.size(1) as torch_geometric.data.Data reports it.  ids (not in the
+    reference): int64 [N] or [N, K], categorical codes of the nodes for GAT(embedding=...), -1 for none."""
 
-    def __init__(self, x, edge_index, y=None):
-        self.x, self.edge_index, self.y = x, edge_index, y
+    def __init__(self, x, edge_index, y=None, ids=None):
+        self.x, self.edge_index, self.y, self.ids = x, edge_index, y, ids
 
     @property
     def num_features(self) -> int:
@@ -28,7 +29,7 @@ class Data:
 
     def to(self, device):
         mv = lambda t: None if t is None else t.to(device)
-        return Data(mv(self.x), mv(self.edge_index), mv(self.y))
+        return Data(mv(self.x), mv(self.edge_index), mv(self.y), mv(self.ids))
 
 
 def _values(X) -> np.ndarray:

@@ -54,32 +54,15 @@ _raw_stream = torch._C._cuda_getCurrentRawStream      # the current stream's han
 _current = torch._C._cuda_getDevice
 
 
-class _on:
-    """The tensor's device made current when it is not, and its stream (torch's own context manager and
-    Stream object cost more than a small kernel)."""
-    __slots__ = ("index", "prev")
-
-    def __init__(self, dev: torch.device):
-        self.index = dev.index
-
-    def __enter__(self):
-        prev = _current()
-        self.prev = prev if prev != self.index else None
-        if self.prev is not None:
-            torch.cuda.set_device(self.index)
-        return _raw_stream(self.index)
-
-    def __exit__(self, *exc):
-        if self.prev is not None:
-            torch.cuda.set_device(self.prev)
-
-
 def _once(backward):
     """A backward that cannot itself be differentiated.  Without create_graph nothing could, and the guard
     (which costs as much as the call) is left out."""
     guarded = once_differentiable(backward)
 
     def run(ctx, grad_y):
+        if _current() != grad_y.device.index:
+            with torch.cuda.device(grad_y.device):
+                return run(ctx, grad_y)
         return guarded(ctx, grad_y) if torch.is_grad_enabled() else backward(ctx, grad_y)
     return staticmethod(run)
 
@@ -91,7 +74,11 @@ class _NoCtx:
         pass
 
 
-def _apply(fn, needs_grad: bool, *args):
+def _apply(fn, x: Tensor, needs_grad: bool, *args):
+    """fn on x's device, without autograd's machinery where nothing needs a gradient"""
+    if _current() != x.device.index:
+        with torch.cuda.device(x.device):
+            return _apply(fn, x, needs_grad, *args)
     return fn.apply(*args) if needs_grad else fn.forward(_NoCtx(), *args)
 
 
@@ -109,16 +96,16 @@ class _LinearFn(torch.autograd.Function):
         residual = None if residual is None else residual.contiguous()
         k, n = x.size(-1), weight.size(0)
         desc = _lib.Linear(x.numel() // k, k, n, dtype, act)
-        with _on(dev) as st:
-            y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=dev)
-            slope = None
-            if keep and act:
-                slope = torch.empty(y.shape, dtype=torch.float32 if dtype == 0 else torch.int16, device=dev)
-            need = lib.gatmi_linear_fwd_workspace_bytes(C.byref(desc))
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            _lib.check(lib.gatmi_linear_fwd(C.byref(desc), x.data_ptr(), weight.data_ptr(), _ptr(bias),
-                                            _ptr(residual), y.data_ptr(), _ptr(slope), _ptr(ws), need, st),
-                       "gatmi_linear_fwd")
+        st = _raw_stream(dev.index)
+        y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=dev)
+        slope = None
+        if keep and act:
+            slope = torch.empty(y.shape, dtype=torch.float32 if dtype == 0 else torch.int16, device=dev)
+        need = lib.gatmi_linear_fwd_workspace_bytes(C.byref(desc))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _lib.check(lib.gatmi_linear_fwd(C.byref(desc), x.data_ptr(), weight.data_ptr(), _ptr(bias),
+                                        _ptr(residual), y.data_ptr(), _ptr(slope), _ptr(ws), need, st),
+                   "gatmi_linear_fwd")
         ctx.save_for_backward(x, weight, slope)
         ctx.desc = desc
         return y
@@ -132,14 +119,14 @@ class _LinearFn(torch.autograd.Function):
         gx = gw = gb = None
         if need_x or need_w or need_b:
             gy = grad_y.contiguous()
-            with _on(dev) as st:
-                gx = torch.empty_like(x) if need_x else None
-                gw = torch.empty_like(weight) if need_w else None
-                gb = torch.empty(weight.size(0), dtype=x.dtype, device=dev) if need_b else None
-                ws = torch.empty(lib.gatmi_linear_bwd_workspace_bytes(C.byref(desc)), dtype=torch.uint8, device=dev)
-                _lib.check(lib.gatmi_linear_bwd(C.byref(desc), x.data_ptr(), weight.data_ptr(), _ptr(slope),
-                                                gy.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), ws.data_ptr(),
-                                                ws.numel(), st), "gatmi_linear_bwd")
+            st = _raw_stream(dev.index)
+            gx = torch.empty_like(x) if need_x else None
+            gw = torch.empty_like(weight) if need_w else None
+            gb = torch.empty(weight.size(0), dtype=x.dtype, device=dev) if need_b else None
+            ws = torch.empty(lib.gatmi_linear_bwd_workspace_bytes(C.byref(desc)), dtype=torch.uint8, device=dev)
+            _lib.check(lib.gatmi_linear_bwd(C.byref(desc), x.data_ptr(), weight.data_ptr(), _ptr(slope),
+                                            gy.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), ws.data_ptr(),
+                                            ws.numel(), st), "gatmi_linear_bwd")
         return gx, gw, gb, grad_res, None, None, None
 
 
@@ -161,7 +148,7 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: st
     grad = torch.is_grad_enabled()
     keep = grad and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad))
     needs = keep or (grad and residual is not None and residual.requires_grad)
-    return _apply(_LinearFn, needs, x, weight, bias, residual, dtype, code, keep)
+    return _apply(_LinearFn, x, needs, x, weight, bias, residual, dtype, code, keep)
 
 
 # ---- group norm ------------------------------------------------------------------------------
@@ -179,17 +166,17 @@ class _GroupNormFn(torch.autograd.Function):
         lib, dev = _lib.lib(), x.device
         x, weight, bias = x.contiguous(), weight.contiguous(), bias.contiguous()
         desc = _gn_desc(x.shape, groups, dtype, act, eps, weight, bias)
-        with _on(dev) as st:
-            y = torch.empty_like(x)
-            stats = ws = None
-            if keep or desc.length > 1 or desc.width > 2048:
-                stats = torch.empty(2, x.size(0), groups, dtype=torch.float32, device=dev)
-                ws = torch.empty(lib.gatmi_group_norm_workspace_bytes(C.byref(desc)), dtype=torch.uint8, device=dev)
-            mean = _ptr(stats)
-            _lib.check(lib.gatmi_group_norm_fwd(
-                C.byref(desc), x.data_ptr(), y.data_ptr(), mean,
-                None if stats is None else mean + 4 * x.size(0) * groups, _ptr(ws),
-                0 if ws is None else ws.numel(), st), "gatmi_group_norm_fwd")
+        st = _raw_stream(dev.index)
+        y = torch.empty_like(x)
+        stats = ws = None
+        if keep or desc.length > 1 or desc.width > 2048:
+            stats = torch.empty(2, x.size(0), groups, dtype=torch.float32, device=dev)
+            ws = torch.empty(lib.gatmi_group_norm_workspace_bytes(C.byref(desc)), dtype=torch.uint8, device=dev)
+        mean = _ptr(stats)
+        _lib.check(lib.gatmi_group_norm_fwd(
+            C.byref(desc), x.data_ptr(), y.data_ptr(), mean,
+            None if stats is None else mean + 4 * x.size(0) * groups, _ptr(ws),
+            0 if ws is None else ws.numel(), st), "gatmi_group_norm_fwd")
         ctx.save_for_backward(x, weight, bias, stats)
         ctx.cfg = (groups, dtype, act, eps)
         return y
@@ -200,13 +187,13 @@ class _GroupNormFn(torch.autograd.Function):
         lib, dev = _lib.lib(), x.device
         desc = _gn_desc(x.shape, *ctx.cfg, weight, bias)
         gy = grad_y.contiguous()
-        with _on(dev) as st:
-            gx, gw, gb = torch.empty_like(x), torch.empty_like(weight), torch.empty_like(bias)
-            ws = torch.empty(lib.gatmi_group_norm_workspace_bytes(C.byref(desc)), dtype=torch.uint8, device=dev)
-            mean = stats.data_ptr()
-            _lib.check(lib.gatmi_group_norm_bwd(
-                C.byref(desc), x.data_ptr(), gy.data_ptr(), mean, mean + 4 * x.size(0) * ctx.cfg[0],
-                gx.data_ptr(), gw.data_ptr(), gb.data_ptr(), ws.data_ptr(), ws.numel(), st), "gatmi_group_norm_bwd")
+        st = _raw_stream(dev.index)
+        gx, gw, gb = torch.empty_like(x), torch.empty_like(weight), torch.empty_like(bias)
+        ws = torch.empty(lib.gatmi_group_norm_workspace_bytes(C.byref(desc)), dtype=torch.uint8, device=dev)
+        mean = stats.data_ptr()
+        _lib.check(lib.gatmi_group_norm_bwd(
+            C.byref(desc), x.data_ptr(), gy.data_ptr(), mean, mean + 4 * x.size(0) * ctx.cfg[0],
+            gx.data_ptr(), gw.data_ptr(), gb.data_ptr(), ws.data_ptr(), ws.numel(), st), "gatmi_group_norm_bwd")
         return gx, gw, gb, None, None, None, None, None
 
 
@@ -231,7 +218,7 @@ def group_norm_act(x: Tensor, groups: int, weight: Tensor, bias: Tensor, eps: fl
     if not eps >= 0.0:
         raise ValueError(f"group_norm_act: eps must not be negative, got {eps}")
     keep = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or bias.requires_grad)
-    return _apply(_GroupNormFn, keep, x, weight, bias, groups, dtype, code, float(eps), keep)
+    return _apply(_GroupNormFn, x, keep, x, weight, bias, groups, dtype, code, float(eps), keep)
 
 
 # ---- embedding -------------------------------------------------------------------------------
@@ -241,10 +228,10 @@ class _EmbeddingFn(torch.autograd.Function):
         lib, dev = _lib.lib(), table.device
         ids, table = ids.contiguous(), table.contiguous()
         vocab, dim = table.shape
-        with _on(dev) as st:
-            y = torch.empty(ids.shape + (dim,), dtype=table.dtype, device=dev)
-            _lib.check(lib.gatmi_embedding_fwd(dtype, ids.numel(), vocab, dim, scale, ids.data_ptr(),
-                                               table.data_ptr(), y.data_ptr(), st), "gatmi_embedding_fwd")
+        st = _raw_stream(dev.index)
+        y = torch.empty(ids.shape + (dim,), dtype=table.dtype, device=dev)
+        _lib.check(lib.gatmi_embedding_fwd(dtype, ids.numel(), vocab, dim, scale, ids.data_ptr(),
+                                           table.data_ptr(), y.data_ptr(), st), "gatmi_embedding_fwd")
         ctx.save_for_backward(ids)
         ctx.cfg = (dtype, vocab, dim, scale)
         return y
@@ -255,11 +242,11 @@ class _EmbeddingFn(torch.autograd.Function):
         dtype, vocab, dim, scale = ctx.cfg
         lib, dev = _lib.lib(), ids.device
         gy = grad_y.contiguous()
-        with _on(dev) as st:
-            grad = torch.empty(vocab, dim, dtype=gy.dtype, device=dev)
-            ws = torch.empty(lib.gatmi_embedding_bwd_workspace_bytes(ids.numel(), vocab, dim), dtype=torch.uint8, device=dev)
-            _lib.check(lib.gatmi_embedding_bwd(dtype, ids.numel(), vocab, dim, scale, ids.data_ptr(), gy.data_ptr(),
-                                               grad.data_ptr(), ws.data_ptr(), ws.numel(), st), "gatmi_embedding_bwd")
+        st = _raw_stream(dev.index)
+        grad = torch.empty(vocab, dim, dtype=gy.dtype, device=dev)
+        ws = torch.empty(lib.gatmi_embedding_bwd_workspace_bytes(ids.numel(), vocab, dim), dtype=torch.uint8, device=dev)
+        _lib.check(lib.gatmi_embedding_bwd(dtype, ids.numel(), vocab, dim, scale, ids.data_ptr(), gy.data_ptr(),
+                                           grad.data_ptr(), ws.data_ptr(), ws.numel(), st), "gatmi_embedding_bwd")
         return None, grad, None, None
 
 
@@ -274,7 +261,7 @@ def embedding(ids: Tensor, table: Tensor, scale: float = 1.0) -> Tensor:
         raise TypeError(f"embedding: ids must be int64, got {ids.dtype}")
     if table.dim() != 2 or table.size(1) < 1:
         raise ValueError(f"embedding: table must be [entries, dim], got {tuple(table.shape)}")
-    return _apply(_EmbeddingFn, torch.is_grad_enabled() and table.requires_grad, ids, table, float(scale), dtype)
+    return _apply(_EmbeddingFn, table, torch.is_grad_enabled() and table.requires_grad, ids, table, float(scale), dtype)
 
 
 # ---- dropout ---------------------------------------------------------------------------------
@@ -286,14 +273,14 @@ class _DropoutFn(torch.autograd.Function):
         residual = None if residual is None else residual.contiguous()
         cols = x.size(-1)
         rows = x.numel() // cols if cols else 0
-        with _on(dev) as st:
-            y = torch.empty_like(x)
-            used = None
-            if isinstance(seed, Tensor):
-                used = torch.empty(1, dtype=torch.int64, device=dev)
-            _lib.check(lib.gatmi_dropout(dtype, rows, max(cols, 1), p, 0 if used is not None else seed,
-                                         seed.data_ptr() if used is not None else None, _ptr(used), x.data_ptr(),
-                                         _ptr(residual), y.data_ptr(), st), "gatmi_dropout")
+        st = _raw_stream(dev.index)
+        y = torch.empty_like(x)
+        used = None
+        if isinstance(seed, Tensor):
+            used = torch.empty(1, dtype=torch.int64, device=dev)
+        _lib.check(lib.gatmi_dropout(dtype, rows, max(cols, 1), p, 0 if used is not None else seed,
+                                     seed.data_ptr() if used is not None else None, _ptr(used), x.data_ptr(),
+                                     _ptr(residual), y.data_ptr(), st), "gatmi_dropout")
         ctx.save_for_backward(used)
         ctx.cfg = (p, seed if used is None else 0, dtype, residual is not None)
         return y
@@ -307,10 +294,10 @@ class _DropoutFn(torch.autograd.Function):
             lib, dev = _lib.lib(), grad_y.device
             gy = grad_y.contiguous()
             cols = gy.size(-1)
-            with _on(dev) as st:
-                gx = torch.empty_like(gy)
-                _lib.check(lib.gatmi_dropout(dtype, gy.numel() // cols if cols else 0, max(cols, 1), p, seed, _ptr(used),
-                                             None, gy.data_ptr(), None, gx.data_ptr(), st), "gatmi_dropout")
+            st = _raw_stream(dev.index)
+            gx = torch.empty_like(gy)
+            _lib.check(lib.gatmi_dropout(dtype, gy.numel() // cols if cols else 0, max(cols, 1), p, seed, _ptr(used),
+                                         None, gy.data_ptr(), None, gx.data_ptr(), st), "gatmi_dropout")
         return gx, grad_y if ctx.needs_input_grad[1] else None, None, None, None
 
 
@@ -339,4 +326,4 @@ def dropout(x: Tensor, p: float, training: bool = True, seed=None, residual: Opt
     else:
         seed = int(seed) & 0xFFFFFFFFFFFFFFFF
     needs = torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad))
-    return _apply(_DropoutFn, needs, x, residual, float(p), seed, dtype)
+    return _apply(_DropoutFn, x, needs, x, residual, float(p), seed, dtype)

@@ -1018,17 +1018,24 @@ class PartitionedGAT(nn.Module):
     (Chan's combination of every rank's rows / mean / M2) and the backward's two column sums
     exchanged between the passes -- and log_softmax + nll_loss on tail.hip (`forward_loss`).
     fused=False keeps the stock torch ops (what the CPU stand-in backend of the tests runs).
-    feature_dtype=torch.bfloat16: bf16 feature tables in the layers (see PartitionedGATConv)."""
+    feature_dtype=torch.bfloat16: bf16 feature tables in the layers (see PartitionedGATConv).
+    norm="group" (default "batch"): group norm -> ELU -> dropout between the layers, one group per head, as
+    GAT(norm="group"): a row is normalised by itself, so the blocks between the layers exchange nothing."""
 
     def __init__(self, num_features, num_classes, hidden_dim=16, dropout=0.7, backend=None, group=None,
-                 balance="edges", feature_dtype=None, chunks=None, padding="auto", fused=None):
+                 balance="edges", feature_dtype=None, chunks=None, padding="auto", fused=None, norm="batch"):
         super().__init__()
+        if norm not in ("batch", "group"):
+            raise ValueError(f"norm must be 'batch' or 'group', got {norm!r}")
+        self.norm = norm
+        make_norm = (lambda: nn.BatchNorm1d(hidden_dim * 8)) if norm == "batch" else \
+            (lambda: nn.GroupNorm(8, hidden_dim * 8))
         kw = dict(dropout=dropout, backend=backend, group=group, balance=balance,
                   feature_dtype=feature_dtype, chunks=chunks, padding=padding)
         self.conv1 = PartitionedGATConv(num_features, hidden_dim, heads=8, **kw)
-        self.bn1 = nn.BatchNorm1d(hidden_dim * 8)
+        self.bn1 = make_norm()
         self.conv2 = PartitionedGATConv(hidden_dim * 8, hidden_dim, heads=8, **kw)
-        self.bn2 = nn.BatchNorm1d(hidden_dim * 8)
+        self.bn2 = make_norm()
         self.conv3 = PartitionedGATConv(hidden_dim * 8, num_classes, heads=1, **kw)
         self.p, self.group = dropout, group
         self.fused = isinstance(self.conv1.backend, HipBackend) if fused is None else bool(fused)
@@ -1056,14 +1063,24 @@ class PartitionedGAT(nn.Module):
         keep = torch.rand(t.shape, generator=self._generator(t.device), device=t.device) >= self.p
         return t * keep.to(t.dtype) / (1.0 - self.p)
 
-    def _glue(self, x: Tensor, bn: nn.BatchNorm1d, num_nodes: int) -> Tensor:
-        """dropout(bn(elu(x))) with the batch statistics of all N rows (model.py:40-42, 43-45)"""
+    def _mask_seed(self) -> int:
+        """the next of a mask stream of this rank's own"""
+        return int(torch.empty((), dtype=torch.int64).random_(generator=self._generator(torch.device("cpu"))).item())
+
+    def _glue(self, x: Tensor, bn: nn.Module, num_nodes: int) -> Tensor:
+        """dropout(bn(elu(x))) with the batch statistics of all N rows (model.py:40-42, 43-45); with
+        norm="group" dropout(elu(group_norm(x))), row by row"""
+        if self.norm == "group":
+            if not self.fused:
+                return self._drop(torch.nn.functional.elu(bn(x)))
+            from .dense import dropout, group_norm_act
+            x = group_norm_act(x, bn.num_groups, bn.weight, bn.bias, bn.eps, "elu")
+            if not self.training or self.p <= 0.0:
+                return x
+            return dropout(x, self.p, seed=self._mask_seed())
         if self.fused:
             from .glue import elu_bn_dropout_rows
-            seed = None
-            if self.training and self.p > 0.0:      # a mask stream of this rank's own
-                seed = int(torch.empty((), dtype=torch.int64).random_(
-                    generator=self._generator(torch.device("cpu"))).item())
+            seed = self._mask_seed() if self.training and self.p > 0.0 else None
             return elu_bn_dropout_rows(x, bn, self.p, self.training, num_nodes, self._exchange, seed)
         return self._drop(sync_elu_bn_dropout(x, bn, 0.0, self.training, num_nodes, self.group))
 

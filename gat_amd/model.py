@@ -19,6 +19,14 @@ Differences a caller can see, all forced by the move to a GPU or to torch 2.10:
     small graphs (the reference's own data, Cora-shaped) an epoch is some sixty kernel launches
     whose host cost exceeds their run time.  The dropout seeds then live on the device
     (GATMI_MASK_HASH_DEV), advanced inside the graph, so every replay draws new masks.
+
+Options the reference does not have, all off by default (the default network and its state_dict are the
+reference's), on the dense operators of gat_amd/dense.py:
+  * `norm="group"`: conv -> group norm (one group per head) -> ELU -> dropout between the layers instead of
+    ELU -> BatchNorm -> dropout: a node is normalised by itself, in training and evaluation alike;
+  * `skip=True`: a linear skip connection beside conv1 and conv2, added in that product's epilogue;
+  * `embedding=(entries, dim)` or `(entries, dim, columns)`: learned features for the categorical codes in
+    `data.ids` (one table for all columns), looked up and put behind `data.x`.
 """
 from __future__ import annotations
 
@@ -30,6 +38,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .data import Data, Metrics
+from .dense import dropout, embedding as embed, group_norm_act, linear_act
 from .glue import elu_bn_dropout, log_softmax_nll
 from .layer import GATConv
 
@@ -77,8 +86,11 @@ def print_epoch_stats(epoch, seconds, tr, va, cm):
 class GAT(nn.Module):
     def __init__(self, optimizer, num_features, num_classes, weight_decay=1e-3, dropout=0.7,
                  hidden_dim=16, epochs=30, lr=0.005, patience=3, device=None, verbose=True,
-                 feature_dtype=None, hipgraph=False):
+                 feature_dtype=None, hipgraph=False, norm="batch", skip=False, embedding=None):
         super().__init__()
+        if norm not in ("batch", "group"):
+            raise ValueError(f"norm must be 'batch' or 'group', got {norm!r}")
+        self.norm, self.skip = norm, bool(skip)
         self.epochs, self.patience, self.num_classes = epochs, patience, num_classes
         self.verbose = verbose
         self.checkpoint_path = "best_model.pth"
@@ -90,10 +102,20 @@ class GAT(nn.Module):
         # rows in bf16 (gat_amd/layer.py); with the reference's widths that is conv2 when
         # hidden_dim is a multiple of 8.  The parity claims of this package are for the default.
         kw = dict(dropout=dropout, feature_dtype=feature_dtype)
+        self.table = None
+        if embedding is not None:
+            entries, dim, columns = (tuple(embedding) + (1,))[:3]
+            self.table = nn.Embedding(entries, dim)
+            num_features += dim * columns
+        make_norm = (lambda: nn.BatchNorm1d(hidden_dim * 8)) if norm == "batch" else \
+            (lambda: nn.GroupNorm(8, hidden_dim * 8))
         self.conv1 = GATConv(num_features, hidden_dim, heads=8, **kw)
-        self.bn1 = nn.BatchNorm1d(hidden_dim * 8)
+        self.bn1 = make_norm()
         self.conv2 = GATConv(hidden_dim * 8, hidden_dim, heads=8, **kw)
-        self.bn2 = nn.BatchNorm1d(hidden_dim * 8)
+        self.bn2 = make_norm()
+        if self.skip:
+            self.skip1 = nn.Linear(num_features, hidden_dim * 8)
+            self.skip2 = nn.Linear(hidden_dim * 8, hidden_dim * 8)
         self.conv3 = GATConv(hidden_dim * 8, num_classes, heads=1, concat=True, **kw)
         self.dropout = nn.Dropout(p=dropout)
         self.device = torch.device(device) if device is not None else default_device()
@@ -104,13 +126,13 @@ class GAT(nn.Module):
         self._resident = {}
         self.hipgraph = bool(hipgraph)
         self._graphs, self._eager_done = {}, set()
-        self._glue_seeds = [None, None]
+        self._glue_seeds = [None, None, None]      # the two blocks' dropouts, the input's
         if self.hipgraph:
             base = int(torch.empty((), dtype=torch.int64).random_().item())
             mk = lambda i: torch.tensor([(base + 0x632BE59BD9B4E019 * i) % (1 << 63)], dtype=torch.int64,
                                         device=self.device)
             self.conv1.device_seed, self.conv2.device_seed, self.conv3.device_seed = mk(0), mk(1), mk(2)
-            self._glue_seeds = [mk(3), mk(4)]
+            self._glue_seeds = [mk(3), mk(4), mk(5)]
 
     # -- data residency: move each Data object to the GPU once
     def _on_device(self, data) -> Data:
@@ -118,22 +140,54 @@ class GAT(nn.Module):
             return data
         hit = self._resident.get(id(data))
         if hit is None or hit[0] is not data:
-            hit = (data, Data(data.x, data.edge_index, data.y).to(self.device))
+            hit = (data, Data(data.x, data.edge_index, data.y, getattr(data, "ids", None)).to(self.device))
             self._resident[id(data)] = hit
         return hit[1]
 
-    def _logits(self, data):
-        x, edge_index = data.x, data.edge_index
-        x = self.dropout(x)
+    def _features(self, data):
+        """data.x with the embedded categorical codes behind it, after the input dropout"""
+        x, p = data.x, self.dropout.p
+        if self.table is not None:
+            if getattr(data, "ids", None) is None:
+                raise ValueError("GAT(embedding=...) needs data.ids")
+            rows = embed(data.ids, self.table.weight) if self.fused_glue else self.table(data.ids)
+            x = torch.cat([x, rows.flatten(1)], dim=1)
+        if self.norm == "batch" or not self.fused_glue:
+            return self.dropout(x)
+        return dropout(x, p, self.training, self._glue_seeds[2])
+
+    def _conv(self, conv, skip, x, edge_index):
+        """conv(x), plus skip(x) when there is one (in the epilogue of its product)"""
+        h = conv(x, edge_index)
+        if not self.skip:
+            return h
         if self.fused_glue:
-            p = self.dropout.p
-            x = elu_bn_dropout(self.conv1(x, edge_index), self.bn1, p, self.training, self._glue_seeds[0])
-            x = elu_bn_dropout(self.conv2(x, edge_index), self.bn2, p, self.training, self._glue_seeds[1])
-        else:
-            x = self.bn1(F.elu(self.conv1(x, edge_index)))
-            x = self.dropout(x)
-            x = self.bn2(F.elu(self.conv2(x, edge_index)))
-            x = self.dropout(x)
+            return linear_act(x, skip.weight, skip.bias, residual=h)
+        return h + skip(x)
+
+    def _between(self, x, norm, seed):
+        """normalisation, ELU and dropout between two layers"""
+        p = self.dropout.p
+        if self.norm == "batch":
+            if self.fused_glue:
+                return elu_bn_dropout(x, norm, p, self.training, seed)
+            return self.dropout(norm(F.elu(x)))
+        if self.fused_glue:
+            x = group_norm_act(x, norm.num_groups, norm.weight, norm.bias, norm.eps, "elu")
+            return dropout(x, p, self.training, seed)
+        # not F.group_norm: its weight and bias gradients are wrong on this platform for rows without further
+        # axes (more than 128 of them)
+        v = x.view(x.size(0), norm.num_groups, -1)
+        var, mean = torch.var_mean(v, dim=2, unbiased=False, keepdim=True)
+        v = ((v - mean) * torch.rsqrt(var + norm.eps)).view_as(x)
+        return self.dropout(F.elu(v * norm.weight + norm.bias))
+
+    def _logits(self, data):
+        x, edge_index = self._features(data), data.edge_index
+        x = self._between(self._conv(self.conv1, getattr(self, "skip1", None), x, edge_index), self.bn1,
+                          self._glue_seeds[0])
+        x = self._between(self._conv(self.conv2, getattr(self, "skip2", None), x, edge_index), self.bn2,
+                          self._glue_seeds[1])
         return self.conv3(x, edge_index)
 
     def forward(self, data):
