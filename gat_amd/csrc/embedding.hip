@@ -415,7 +415,7 @@ static EmbGeom emb_geom(long long n, long long vocab) {
     G.items = n >= (1 << 20) ? 16 : 4;
     G.blocks = (int)((n + 256ll * G.items - 1) / (256ll * G.items));
     // long chunks leave fewer ends to sum again, short ones keep the chip busy when there are few rows
-    G.chunk0 = n >= (1 << 20) ? 64 : (n >= (1 << 17) ? 32 : 16);
+    G.chunk0 = n >= (1 << 20) || n <= 64 ? 64 : (n >= (1 << 17) ? 32 : 16);
     G.chunk = 32;
     G.entries[0] = n;
     G.levels = 1;

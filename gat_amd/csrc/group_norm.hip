@@ -467,14 +467,17 @@ __global__ __launch_bounds__(256) void colsum_slab_kernel(const float *in, long 
         slab[((long long)blockIdx.y * gridDim.z + blockIdx.z) * cols + c] = s;
     }
 }
+// (few rows: the rows themselves as slabs)
 template <class T>
-__global__ __launch_bounds__(256) void colsum_final_kernel(const float *slab, int nslab, int cols, T *out0, T *out1) {
+__global__ __launch_bounds__(256) void colsum_final_kernel(const float *slab, int nslab, long long ld, long long set,
+                                                           int cols, T *out0, T *out1) {
     __shared__ double red[256];
     const int i = blockIdx.x * 32 + (threadIdx.x & 31), rg = threadIdx.x >> 5;     // i over [2][cols]
+    const float *at = i < cols ? slab + i : slab + set + (i - cols);
     double s = 0.0;
     if (i < 2 * cols)
 #pragma unroll 8
-        for (int q = rg; q < nslab; q += 8) s += slab[(long long)q * 2 * cols + i];
+        for (int q = rg; q < nslab; q += 8) s += at[q * ld];
     red[threadIdx.x] = s;
     __syncthreads();
     if (rg == 0 && i < 2 * cols) {
@@ -703,12 +706,19 @@ extern "C" int gatmi_group_norm_bwd(const gatmi_group_norm *g, const void *x, co
         out1 = grad_weight;
     }
     ProfScope ps("group_norm_param_sums", st);
-    const int slabs = rows < G.slabs ? (int)(rows < 1 ? 0 : rows) : G.slabs;
-    if (slabs > 0)
-        hipLaunchKernelGGL(colsum_slab_kernel, dim3((C + 31) / 32, slabs, 2), dim3(256), 0, st, A.part, rows, ld, set,
+    const float *sums = A.part;
+    int nsum = (int)rows;
+    if (rows > 4 * G.slabs) {
+        hipLaunchKernelGGL(colsum_slab_kernel, dim3((C + 31) / 32, G.slabs, 2), dim3(256), 0, st, A.part, rows, ld, set,
                            C, slab);
+        sums = slab;
+        nsum = G.slabs;
+        ld = 2ll * C;
+        set = C;
+    }
     GATMI_WITH_TYPE(g->dtype, hipLaunchKernelGGL((colsum_final_kernel<T>), dim3((2 * C + 31) / 32), dim3(256), 0, st,
-                                                 slab, slabs, C, static_cast<T *>(out0), static_cast<T *>(out1)));
+                                                 sums, nsum, ld, set, C, static_cast<T *>(out0),
+                                                 static_cast<T *>(out1)));
     GATMI_HIP(hipGetLastError());
     return GATMI_OK;
 }

@@ -154,6 +154,7 @@ struct LinArgs {
     void *C;                  // [M, N]
     void *slope;              // forward: act'(z) out
     float *part, *dbpart;     // dW: [splits][N][K] slabs, [splits][N] column sums
+    void *dw, *db;            // one split: the gradients themselves instead
     long long M;
     int N, K, ldb, act;
     long long tiles_n, tiles;
@@ -558,7 +559,7 @@ template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = (wave / WN) * 64, wn = (wave % WN) * 64;
     typedef typename SlopeOf<T>::type ST;
-    const bool sloped = A.aslope, sums = A.dbpart && k0 == 0;
+    const bool sloped = A.aslope, sums = (A.dbpart || A.db) && k0 == 0;
     Gran<T> ga[NA], gb[NB];
     SlopeGran<T> gs[NA];
     VecF<8> db;
@@ -662,7 +663,8 @@ template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void
         if (threadIdx.x < kBM && n0 + (int)threadIdx.x < A.N) {
             float s = 0.f;
             for (int q = 0; q < RA; ++q) s += red[q * kBM + threadIdx.x];
-            A.dbpart[split * A.N + n0 + threadIdx.x] = s;
+            if (A.db) static_cast<T *>(A.db)[n0 + threadIdx.x] = (T)s;
+            else A.dbpart[split * A.N + n0 + threadIdx.x] = s;
         }
     }
     float *part = A.part + split * (long long)A.N * A.K;
@@ -683,7 +685,8 @@ template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void
                         v = fmaf(d, (float)pb[m * A.K + k], v);
                     }
                 }
-                part[(long long)n * A.K + k] = v;
+                if (A.dw) static_cast<T *>(A.dw)[(long long)n * A.K + k] = (T)v;
+                else part[(long long)n * A.K + k] = v;
             }
 }
 
@@ -956,7 +959,10 @@ extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void
         A.N = N;
         A.K = K;
         A.part = slabs;
-        A.dbpart = grad_bias ? dbpart : nullptr;
+        const bool one = G.splits == 1 && grad_weight;
+        A.dbpart = grad_bias && !one ? dbpart : nullptr;
+        A.dw = one ? grad_weight : nullptr;
+        A.db = one ? grad_bias : nullptr;
         A.per_split = G.per_split;
         GATMI_WITH_TYPE(l->dtype, {
             const bool wide = K > 128;      // dz is made once for twice the columns of x
@@ -966,10 +972,10 @@ extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void
                                      : (wide ? lin_tn_kernel<T, 256, false> : lin_tn_kernel<T, 128, false>);
             hipLaunchKernelGGL(tn, dim3((unsigned)(A.tiles * G.splits)), dim3(wide ? 512 : 256), 0, st, A);
             const long long size = (long long)N * K;
-            if (grad_weight)
+            if (grad_weight && !one)
                 hipLaunchKernelGGL((lin_slabs_kernel<T>), dim3((unsigned)((size + 63) / 64)), dim3(256), 0, st, slabs,
                                    G.splits, size, static_cast<T *>(grad_weight));
-            if (grad_bias)
+            if (grad_bias && !one)
                 hipLaunchKernelGGL((lin_db_kernel<T>), dim3((N + 7) / 8), dim3(256), 0, st, dbpart, G.splits, N,
                                    static_cast<T *>(grad_bias));
         });
