@@ -12,6 +12,7 @@ refused.
 from __future__ import annotations
 
 import ctypes as C
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -82,6 +83,26 @@ def _apply(fn, x: Tensor, needs_grad: bool, *args):
     return fn.apply(*args) if needs_grad else fn.forward(_NoCtx(), *args)
 
 
+# Workspace sizes by shape (a query through the C ABI costs as much as a small kernel)
+@lru_cache(maxsize=4096)
+def _linear_ws(device, rows, k, n, dtype, act):
+    desc = _lib.Linear(rows, k, n, dtype, act)
+    lib = _lib.lib()
+    return (int(lib.gatmi_linear_fwd_workspace_bytes(C.byref(desc))),
+            int(lib.gatmi_linear_bwd_workspace_bytes(C.byref(desc))))
+
+
+@lru_cache(maxsize=4096)
+def _embedding_ws(n, vocab, dim):
+    return int(_lib.lib().gatmi_embedding_bwd_workspace_bytes(n, vocab, dim))
+
+
+@lru_cache(maxsize=4096)
+def _group_norm_ws(batch, length, groups, width, dtype):
+    desc = _lib.GroupNorm(batch, length, groups, width, dtype, 0, 0.0, 0, None, None)
+    return int(_lib.lib().gatmi_group_norm_workspace_bytes(C.byref(desc)))
+
+
 def _ptr(t: Optional[Tensor]):
     return None if t is None else t.data_ptr()
 
@@ -101,7 +122,7 @@ class _LinearFn(torch.autograd.Function):
         slope = None
         if keep and act:
             slope = torch.empty(y.shape, dtype=torch.float32 if dtype == 0 else torch.int16, device=dev)
-        need = lib.gatmi_linear_fwd_workspace_bytes(C.byref(desc))
+        need = _linear_ws(dev.index, desc.rows, k, n, dtype, act)[0]
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _lib.check(lib.gatmi_linear_fwd(C.byref(desc), x.data_ptr(), weight.data_ptr(), _ptr(bias),
                                         _ptr(residual), y.data_ptr(), _ptr(slope), _ptr(ws), need, st),
@@ -123,10 +144,11 @@ class _LinearFn(torch.autograd.Function):
             gx = torch.empty_like(x) if need_x else None
             gw = torch.empty_like(weight) if need_w else None
             gb = torch.empty(weight.size(0), dtype=x.dtype, device=dev) if need_b else None
-            ws = torch.empty(lib.gatmi_linear_bwd_workspace_bytes(C.byref(desc)), dtype=torch.uint8, device=dev)
+            need = _linear_ws(dev.index, desc.rows, desc.in_features, desc.out_features, desc.dtype, desc.act)[1]
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
             _lib.check(lib.gatmi_linear_bwd(C.byref(desc), x.data_ptr(), weight.data_ptr(), _ptr(slope),
                                             gy.data_ptr(), _ptr(gx), _ptr(gw), _ptr(gb), ws.data_ptr(),
-                                            ws.numel(), st), "gatmi_linear_bwd")
+                                            need, st), "gatmi_linear_bwd")
         return gx, gw, gb, grad_res, None, None, None
 
 
@@ -171,7 +193,7 @@ class _GroupNormFn(torch.autograd.Function):
         stats = ws = None
         if keep or desc.length > 1 or desc.width > 2048:
             stats = torch.empty(2, x.size(0), groups, dtype=torch.float32, device=dev)
-            ws = torch.empty(lib.gatmi_group_norm_workspace_bytes(C.byref(desc)), dtype=torch.uint8, device=dev)
+            ws = torch.empty(_group_norm_ws(desc.batch, desc.length, groups, desc.width, dtype), dtype=torch.uint8, device=dev)
         mean = _ptr(stats)
         _lib.check(lib.gatmi_group_norm_fwd(
             C.byref(desc), x.data_ptr(), y.data_ptr(), mean,
@@ -189,11 +211,12 @@ class _GroupNormFn(torch.autograd.Function):
         gy = grad_y.contiguous()
         st = _raw_stream(dev.index)
         gx, gw, gb = torch.empty_like(x), torch.empty_like(weight), torch.empty_like(bias)
-        ws = torch.empty(lib.gatmi_group_norm_workspace_bytes(C.byref(desc)), dtype=torch.uint8, device=dev)
+        need = _group_norm_ws(desc.batch, desc.length, desc.groups, desc.width, desc.dtype)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
         mean = stats.data_ptr()
         _lib.check(lib.gatmi_group_norm_bwd(
             C.byref(desc), x.data_ptr(), gy.data_ptr(), mean, mean + 4 * x.size(0) * ctx.cfg[0],
-            gx.data_ptr(), gw.data_ptr(), gb.data_ptr(), ws.data_ptr(), ws.numel(), st), "gatmi_group_norm_bwd")
+            gx.data_ptr(), gw.data_ptr(), gb.data_ptr(), ws.data_ptr(), need, st), "gatmi_group_norm_bwd")
         return gx, gw, gb, None, None, None, None, None
 
 
@@ -244,9 +267,11 @@ class _EmbeddingFn(torch.autograd.Function):
         gy = grad_y.contiguous()
         st = _raw_stream(dev.index)
         grad = torch.empty(vocab, dim, dtype=gy.dtype, device=dev)
-        ws = torch.empty(lib.gatmi_embedding_bwd_workspace_bytes(ids.numel(), vocab, dim), dtype=torch.uint8, device=dev)
-        _lib.check(lib.gatmi_embedding_bwd(dtype, ids.numel(), vocab, dim, scale, ids.data_ptr(), gy.data_ptr(),
-                                           grad.data_ptr(), ws.data_ptr(), ws.numel(), st), "gatmi_embedding_bwd")
+        n = ids.numel()
+        need = _embedding_ws(n, vocab, dim)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        _lib.check(lib.gatmi_embedding_bwd(dtype, n, vocab, dim, scale, ids.data_ptr(), gy.data_ptr(),
+                                           grad.data_ptr(), ws.data_ptr(), need, st), "gatmi_embedding_bwd")
         return None, grad, None, None
 
 
