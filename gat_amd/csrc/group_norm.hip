@@ -19,7 +19,10 @@ namespace gatmi {
 
 constexpr int kGnMaxT = 8;         // vectors per lane of the segment kernels
 constexpr int kGnFwdBlocks = 4096, kGnBwdBlocks = 1024;
-constexpr int kGnChunks = 1536;    // blocks of the length > 1 form, over all samples
+// Blocks of the length > 1 form, over all samples: of the passes that leave sums (each block's are read again)
+// and of those that only apply.  Twelve blocks a CU for the sums: 158 -> 137 us for the backward's at
+// [3, 169343, 256] bf16 against six; the forward's does not care.
+constexpr int kGnChunks = 3072, kGnApply = 6144, kGnJoin = 1024;   // (kGnJoin: threads of a joining block)
 constexpr int kGnSlabs = 64;       // row slabs of the column sums
 
 struct GnArgs {
@@ -254,15 +257,14 @@ template <class T, int V> __global__ __launch_bounds__(256) void gn_stats_kernel
     }
 }
 
+// sum over the kGnJoin threads of a block: waves first, then their sums in order
 __device__ __forceinline__ double block_sum(double v, double *red) {
-    red[threadIdx.x] = v;
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     __syncthreads();
-    for (int o = 128; o > 0; o >>= 1) {
-        if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
-        __syncthreads();
-    }
-    const double r = red[0];
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
+    double r = 0.0;
+    for (int w = 0; w < kGnJoin / 64; ++w) r += red[w];
     return r;
 }
 
@@ -273,8 +275,8 @@ struct GnWalk {
 };
 __device__ __forceinline__ GnWalk gn_walk(int width) {
     GnWalk w;
-    const int lanes = width < 256 ? width : 256;
-    w.step = 256 / lanes;
+    const int lanes = width < kGnJoin ? width : kGnJoin;
+    w.step = kGnJoin / lanes;
     w.j = threadIdx.x % lanes;
     w.c = threadIdx.x / lanes;
     w.jstep = lanes;
@@ -283,8 +285,8 @@ __device__ __forceinline__ GnWalk gn_walk(int width) {
 }
 
 // one block per (group, sample): Chan over the group's channels and chunks, in double
-__global__ __launch_bounds__(256) void gn_finalize_kernel(const GnArgs A) {
-    __shared__ double red[256];
+__global__ __launch_bounds__(kGnJoin) void gn_finalize_kernel(const GnArgs A) {
+    __shared__ double red[kGnJoin / 64];
     const int g = blockIdx.x;
     const int per = (int)((A.length + A.chunks - 1) / A.chunks);
     const int full = (int)(A.length / per), rest = (int)(A.length - (long long)full * per);
@@ -358,7 +360,7 @@ template <class T, int V, int ACT> __global__ __launch_bounds__(256) void gn_red
     if (L.on) {
         GnCols<T, V> P;
         P.load(A, L.off, blockIdx.y);
-#pragma unroll 4
+#pragma unroll 2
         for (long long r = L.r0 + L.rsub; r < L.r1; r += L.rpp) {
             const VecF<V> v = ldv<T, V>(x + r * A.C), g = ldv<T, V>(dy + r * A.C);
 #pragma unroll
@@ -393,8 +395,8 @@ template <class T, int V, int ACT> __global__ __launch_bounds__(256) void gn_red
 }
 
 // one block per (group, sample): mean(g) and mean(g xh) of the group
-template <class T> __global__ __launch_bounds__(256) void gn_coef_kernel(const GnArgs A) {
-    __shared__ double red[256];
+template <class T> __global__ __launch_bounds__(kGnJoin) void gn_coef_kernel(const GnArgs A) {
+    __shared__ double red[kGnJoin / 64];
     const int g = blockIdx.x;
     const float *p = A.part + (long long)blockIdx.y * A.chunks * 2 * A.C + g * A.width;
     const T *w = static_cast<const T *>(A.w) + g * A.width;
@@ -432,7 +434,7 @@ template <class T, int V, int ACT> __global__ __launch_bounds__(256) void gn_app
         m1.e[k] = o[0];
         m2.e[k] = o[1];
     }
-#pragma unroll 2
+#pragma unroll 4
     for (long long r = L.r0 + L.rsub; r < L.r1; r += L.rpp) {
         const VecF<V> v = ldv<T, V>(x + r * A.C);
         VecF<V> g = ldv<T, V>(dy + r * A.C);
@@ -513,7 +515,7 @@ struct GnGeom {
     int V, TT, W, w_log;
     int blocks_fwd, blocks_bwd;
     long long slots;      // lane groups of the backward's grid
-    int chunks, zblocks;
+    int chunks, apply, zblocks;      // row ranges a sample is cut into
     int slabs;
     size_t part_floats, slab_floats, coef_floats;
 };
@@ -551,9 +553,13 @@ static GnGeom gn_geom(const gatmi_group_norm *g) {
         const int rpp = nslot < 256 ? 256 / nslot : 1;
         // at least eight rows a lane; at most kGnChunks blocks over all samples
         const long long want = (g->length + 8ll * rpp - 1) / (8ll * rpp);
-        long long most = kGnChunks / ((long long)G.zblocks * (g->batch > 0 ? g->batch : 1));
-        if (most < 1) most = 1;
-        G.chunks = (int)(want < most ? want : most);
+        const long long lots = (long long)G.zblocks * (g->batch > 0 ? g->batch : 1);
+        auto cut = [&](long long blocks) {
+            const long long most = blocks / lots < 1 ? 1 : blocks / lots;
+            return (int)(want < most ? want : most);
+        };
+        G.chunks = cut(kGnChunks);
+        G.apply = cut(kGnApply);
         G.part_floats = (size_t)g->batch * G.chunks * 2 * C;
         G.coef_floats = (size_t)g->batch * g->groups * 2;
     }
@@ -636,12 +642,14 @@ extern "C" int gatmi_group_norm_fwd(const gatmi_group_norm *g, const void *x, vo
         GATMI_WITH_TYPE(g->dtype, with_vec<T>(G.V, [&](auto V) {
             hipLaunchKernelGGL((gn_stats_kernel<T, decltype(V)::value>), grid, dim3(256), 0, st, A);
         }));
-        hipLaunchKernelGGL(gn_finalize_kernel, dim3(g->groups, (unsigned)g->batch), dim3(256), 0, st, A);
+        hipLaunchKernelGGL(gn_finalize_kernel, dim3(g->groups, (unsigned)g->batch), dim3(kGnJoin), 0, st, A);
         GATMI_HIP(hipGetLastError());
     }
     ProfScope ps("group_norm_apply_fwd", st);
+    A.chunks = G.apply;
+    const dim3 apply(G.apply, (unsigned)g->batch, G.zblocks);
     GATMI_WITH_TYPE(g->dtype, GATMI_WITH_ACT(g->act, with_vec<T>(G.V, [&](auto V) {
-            hipLaunchKernelGGL((gn_apply_fwd_kernel<T, decltype(V)::value, ACT>), grid, dim3(256), 0, st, A);
+            hipLaunchKernelGGL((gn_apply_fwd_kernel<T, decltype(V)::value, ACT>), apply, dim3(256), 0, st, A);
         })));
     GATMI_HIP(hipGetLastError());
     return GATMI_OK;
@@ -691,12 +699,14 @@ extern "C" int gatmi_group_norm_bwd(const gatmi_group_norm *g, const void *x, co
             hipLaunchKernelGGL((gn_reduce_bwd_kernel<T, decltype(V)::value, ACT>), grid, dim3(256), 0, st, A);
         })));
             GATMI_WITH_TYPE(g->dtype, hipLaunchKernelGGL((gn_coef_kernel<T>), dim3(g->groups, (unsigned)g->batch),
-                                                         dim3(256), 0, st, A));
+                                                         dim3(kGnJoin), 0, st, A));
             GATMI_HIP(hipGetLastError());
         }
         ProfScope ps("group_norm_apply_bwd", st);
+        A.chunks = G.apply;
+        const dim3 apply(G.apply, (unsigned)g->batch, G.zblocks);
         GATMI_WITH_TYPE(g->dtype, GATMI_WITH_ACT(g->act, with_vec<T>(G.V, [&](auto V) {
-            hipLaunchKernelGGL((gn_apply_bwd_kernel<T, decltype(V)::value, ACT>), grid, dim3(256), 0, st, A);
+            hipLaunchKernelGGL((gn_apply_bwd_kernel<T, decltype(V)::value, ACT>), apply, dim3(256), 0, st, A);
         })));
         GATMI_HIP(hipGetLastError());
         rows = g->batch * G.chunks;
