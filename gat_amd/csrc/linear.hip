@@ -118,12 +118,13 @@ __device__ __forceinline__ void cut3(float a, float b, uint32_t &p0, uint32_t &p
 }
 
 // A tile of R rows x BK contraction elements in LDS, PIECES planes of 16-bit elements.  16-byte granules
-// are XOR-swizzled so that eight lanes reading one granule column of eight rows hit all banks.
+// are XOR-swizzled so that sixteen lanes reading one granule column of sixteen rows hit all 64 banks: rows of
+// 128 bytes lie in halves of the banks by their parity, rows of 64 bytes in quarters.
 template <class T, int R> struct Tile {
     static constexpr int BK = Mul<T>::BK, G = BK / 8, P = Mul<T>::PIECES;
     static constexpr int PLANE = R * BK * 2, BYTES = PLANE * P;
     static __device__ __forceinline__ int at(int row, int g) {
-        const int s = G == 8 ? (row & 7) : ((row >> 1) & 3);
+        const int s = G == 8 ? ((row >> 1) & 7) : ((row >> 2) & 3);
         return row * (BK * 2) + ((g ^ s) << 4);
     }
     static __device__ __forceinline__ void put(char *lds, int row, int g, const Gran<T> &v) {
