@@ -150,7 +150,11 @@ class GAT(nn.Module):
         if self.table is not None:
             if getattr(data, "ids", None) is None:
                 raise ValueError("GAT(embedding=...) needs data.ids")
-            rows = embed(data.ids, self.table.weight) if self.fused_glue else self.table(data.ids)
+            if self.fused_glue:
+                rows = embed(data.ids, self.table.weight)
+            else:       # nn.Embedding knows no "none": row 0, cleared
+                known = (data.ids >= 0) & (data.ids < self.table.num_embeddings)
+                rows = self.table(data.ids * known) * known.unsqueeze(-1)
             x = torch.cat([x, rows.flatten(1)], dim=1)
         if self.norm == "batch" or not self.fused_glue:
             return self.dropout(x)

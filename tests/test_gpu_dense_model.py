@@ -106,3 +106,21 @@ def test_refusals(cuda):
         d = graph_data()
         d.ids = None
         make(cuda, embedding=(40, 6, 2))(d)
+
+
+def test_codes_of_none_on_stock_modules(cuda):
+    """-1 and codes past the table are zero features, without a gradient, on the stock modules too"""
+    data = graph_data()
+    data.ids[5, 0] = 40
+    a = make(cuda, embedding=(40, 6, 2))
+    b = copy.deepcopy(a)
+    b.fused_glue = False
+    dev = a._on_device(data)
+    x = [m._features(dev) for m in (a, b)]
+    assert torch.equal(x[0], x[1])
+    none = (data.ids < 0) | (data.ids >= 40)
+    assert not x[1][:, 25:].detach().cpu().view(-1, 2, 6)[none].any()
+    up = torch.randn(x[0].shape, generator=torch.Generator().manual_seed(1)).to(cuda)
+    grads = [torch.autograd.grad(v, m.table.weight, up)[0] for v, m in zip(x, (a, b))]
+    # sums of at most 800 f32 terms in another order: 800 U = 5e-5 of the terms' sizes
+    torch.testing.assert_close(grads[0], grads[1], rtol=0, atol=5e-5 * float(up.abs().max()) * 40)
