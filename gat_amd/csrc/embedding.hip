@@ -453,10 +453,18 @@ extern "C" int gatmi_embedding_fwd(int32_t dtype, int64_t n, int64_t vocab, int6
     A.w_log = ilog2(A.W);
     const long long per = (256 >> A.w_log) * kEmbUnroll;
     ProfScope ps("embedding_fwd", st);
-    GATMI_WITH_TYPE(dtype, with_vec<T>(v, [&](auto V) {
-        hipLaunchKernelGGL((emb_fwd_kernel<T, decltype(V)::value>), dim3((unsigned)((n + per - 1) / per)), dim3(256), 0,
-                           st, A);
-    }));
+    // a launch counts its threads in 32 bits: 2^23 blocks of 256 at most
+    for (long long i = 0; i < n; i += per << 23) {
+        A.ids = ids + i;
+        A.n = n - i < per << 23 ? n - i : per << 23;
+        GATMI_WITH_TYPE(dtype, {
+            A.y = static_cast<T *>(y) + i * dim;
+            with_vec<T>(v, [&](auto V) {
+                hipLaunchKernelGGL((emb_fwd_kernel<T, decltype(V)::value>), dim3((unsigned)((A.n + per - 1) / per)),
+                                   dim3(256), 0, st, A);
+            });
+        });
+    }
     GATMI_HIP(hipGetLastError());
     return GATMI_OK;
 }

@@ -22,7 +22,9 @@ constexpr int kGnFwdBlocks = 4096, kGnBwdBlocks = 1024;
 // Blocks of the length > 1 form, over all samples: of the passes that leave sums (each block's are read again)
 // and of those that only apply.  Twelve blocks a CU for the sums: 158 -> 137 us for the backward's at
 // [3, 169343, 256] bf16 against six; the forward's does not care.
-constexpr int kGnChunks = 3072, kGnApply = 6144, kGnJoin = 1024;   // (kGnJoin: threads of a joining block)
+constexpr int kGnChunks = 3072, kGnApply = 6144;
+constexpr int kGnJoin = 1024;      // most threads of a block that joins a group's chunks
+constexpr int kGnSamples = 65535;  // samples of one launch
 constexpr int kGnSlabs = 64;       // row slabs of the column sums
 
 struct GnArgs {
@@ -257,14 +259,14 @@ template <class T, int V> __global__ __launch_bounds__(256) void gn_stats_kernel
     }
 }
 
-// sum over the kGnJoin threads of a block: waves first, then their sums in order
+// sum over a block's threads: waves first, then their sums in order
 __device__ __forceinline__ double block_sum(double v, double *red) {
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     double r = 0.0;
-    for (int w = 0; w < kGnJoin / 64; ++w) r += red[w];
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) r += red[w];
     return r;
 }
 
@@ -275,8 +277,8 @@ struct GnWalk {
 };
 __device__ __forceinline__ GnWalk gn_walk(int width) {
     GnWalk w;
-    const int lanes = width < kGnJoin ? width : kGnJoin;
-    w.step = kGnJoin / lanes;
+    const int lanes = width < (int)blockDim.x ? width : (int)blockDim.x;
+    w.step = blockDim.x / lanes;
     w.j = threadIdx.x % lanes;
     w.c = threadIdx.x / lanes;
     w.jstep = lanes;
@@ -503,9 +505,6 @@ static int gn_check(const gatmi_group_norm *g) {
                   GATMI_GROUP_NORM_MAX_CHANNELS);
     GATMI_REQUIRE(g->batch >= 0 && g->length >= 1 && g->batch < (1ll << 31) && g->length < (1ll << 31),
                   "group_norm: batch %lld / length %lld out of range", (long long)g->batch, (long long)g->length);
-    GATMI_REQUIRE(gn_in_registers(g) || g->batch <= 65535,
-                  "group_norm: at most 65535 samples when a group does not fit a wave's registers (length > 1, or %d "
-                  "channels a group)", g->width);
     GATMI_REQUIRE(g->eps >= 0.f, "group_norm: negative eps");
     return GATMI_OK;
 }
@@ -516,6 +515,7 @@ struct GnGeom {
     int blocks_fwd, blocks_bwd;
     long long slots;      // lane groups of the backward's grid
     int chunks, apply, zblocks;      // row ranges a sample is cut into
+    int join;             // threads of a joining block
     int slabs;
     size_t part_floats, slab_floats, coef_floats;
 };
@@ -560,6 +560,9 @@ static GnGeom gn_geom(const gatmi_group_norm *g) {
         };
         G.chunks = cut(kGnChunks);
         G.apply = cut(kGnApply);
+        // about four values a thread: many samples of a few chunks each take a wave per group, not sixteen
+        G.join = next_pow2(G.chunks * g->width / 4 + 1);
+        G.join = G.join < 64 ? 64 : (G.join > kGnJoin ? kGnJoin : G.join);
         G.part_floats = (size_t)g->batch * G.chunks * 2 * C;
         G.coef_floats = (size_t)g->batch * g->groups * 2;
     }
@@ -582,6 +585,26 @@ static void gn_fill(GnArgs &A, const gatmi_group_norm *g, const GnGeom &G) {
     A.w_log = G.w_log;
     A.eps = g->eps;
     A.inv_n = 1.0f / (float)g->width;
+}
+
+// f(samples, their arguments) of the chunk form: a launch takes at most kGnSamples samples (grid.y)
+template <class F> static void gn_slices(const gatmi_group_norm *g, const GnArgs &all, F f) {
+    const long long el = g->dtype == GATMI_F32 ? 4 : 2, sample = g->length * all.C * el;
+    auto move = [](auto *&p, long long bytes) {
+        if (p) p = reinterpret_cast<std::remove_reference_t<decltype(p)>>((uintptr_t)p + bytes);
+    };
+    for (long long s = 0; s < g->batch; s += kGnSamples) {
+        GnArgs A = all;
+        move(A.x, s * sample);
+        move(A.dy, s * sample);
+        move(A.y, s * sample);
+        move(A.dx, s * sample);
+        A.mean += s * A.groups;
+        A.rstd += s * A.groups;
+        A.part += s * A.chunks * 2 * A.C;
+        if (A.coef) A.coef += s * A.groups * 2;
+        f((unsigned)(g->batch - s < kGnSamples ? g->batch - s : kGnSamples), A);
+    }
 }
 
 // f(V, TT) of the segment form: several vectors a lane only when they are full ones
@@ -636,21 +659,18 @@ extern "C" int gatmi_group_norm_fwd(const gatmi_group_norm *g, const void *x, vo
         return GATMI_ERR_WS;
     }
     A.part = static_cast<float *>(ws);
-    const dim3 grid(G.chunks, (unsigned)g->batch, G.zblocks);
-    {
-        ProfScope ps("group_norm_stats", st);
+    ProfScope ps("group_norm_fwd", st);
+    gn_slices(g, A, [&](unsigned samples, GnArgs S) {
+        const dim3 grid(G.chunks, samples, G.zblocks), apply(G.apply, samples, G.zblocks);
         GATMI_WITH_TYPE(g->dtype, with_vec<T>(G.V, [&](auto V) {
-            hipLaunchKernelGGL((gn_stats_kernel<T, decltype(V)::value>), grid, dim3(256), 0, st, A);
+            hipLaunchKernelGGL((gn_stats_kernel<T, decltype(V)::value>), grid, dim3(256), 0, st, S);
         }));
-        hipLaunchKernelGGL(gn_finalize_kernel, dim3(g->groups, (unsigned)g->batch), dim3(kGnJoin), 0, st, A);
-        GATMI_HIP(hipGetLastError());
-    }
-    ProfScope ps("group_norm_apply_fwd", st);
-    A.chunks = G.apply;
-    const dim3 apply(G.apply, (unsigned)g->batch, G.zblocks);
-    GATMI_WITH_TYPE(g->dtype, GATMI_WITH_ACT(g->act, with_vec<T>(G.V, [&](auto V) {
-            hipLaunchKernelGGL((gn_apply_fwd_kernel<T, decltype(V)::value, ACT>), apply, dim3(256), 0, st, A);
+        hipLaunchKernelGGL(gn_finalize_kernel, dim3(g->groups, samples), dim3(G.join), 0, st, S);
+        S.chunks = G.apply;
+        GATMI_WITH_TYPE(g->dtype, GATMI_WITH_ACT(g->act, with_vec<T>(G.V, [&](auto V) {
+            hipLaunchKernelGGL((gn_apply_fwd_kernel<T, decltype(V)::value, ACT>), apply, dim3(256), 0, st, S);
         })));
+    });
     GATMI_HIP(hipGetLastError());
     return GATMI_OK;
 }
@@ -692,22 +712,19 @@ extern "C" int gatmi_group_norm_bwd(const gatmi_group_norm *g, const void *x, co
         ld = C;
         set = G.slots * (long long)g->width;
     } else if (g->batch > 0) {
-        const dim3 grid(G.chunks, (unsigned)g->batch, G.zblocks);
-        {
-            ProfScope ps("group_norm_reduce_bwd", st);
+        ProfScope ps("group_norm_bwd", st);
+        gn_slices(g, A, [&](unsigned samples, GnArgs S) {
+            const dim3 grid(G.chunks, samples, G.zblocks), apply(G.apply, samples, G.zblocks);
             GATMI_WITH_TYPE(g->dtype, GATMI_WITH_ACT(g->act, with_vec<T>(G.V, [&](auto V) {
-            hipLaunchKernelGGL((gn_reduce_bwd_kernel<T, decltype(V)::value, ACT>), grid, dim3(256), 0, st, A);
-        })));
-            GATMI_WITH_TYPE(g->dtype, hipLaunchKernelGGL((gn_coef_kernel<T>), dim3(g->groups, (unsigned)g->batch),
-                                                         dim3(kGnJoin), 0, st, A));
-            GATMI_HIP(hipGetLastError());
-        }
-        ProfScope ps("group_norm_apply_bwd", st);
-        A.chunks = G.apply;
-        const dim3 apply(G.apply, (unsigned)g->batch, G.zblocks);
-        GATMI_WITH_TYPE(g->dtype, GATMI_WITH_ACT(g->act, with_vec<T>(G.V, [&](auto V) {
-            hipLaunchKernelGGL((gn_apply_bwd_kernel<T, decltype(V)::value, ACT>), apply, dim3(256), 0, st, A);
-        })));
+                hipLaunchKernelGGL((gn_reduce_bwd_kernel<T, decltype(V)::value, ACT>), grid, dim3(256), 0, st, S);
+            })));
+            GATMI_WITH_TYPE(g->dtype, hipLaunchKernelGGL((gn_coef_kernel<T>), dim3(g->groups, samples), dim3(G.join), 0,
+                                                         st, S));
+            S.chunks = G.apply;
+            GATMI_WITH_TYPE(g->dtype, GATMI_WITH_ACT(g->act, with_vec<T>(G.V, [&](auto V) {
+                hipLaunchKernelGGL((gn_apply_bwd_kernel<T, decltype(V)::value, ACT>), apply, dim3(256), 0, st, S);
+            })));
+        });
         GATMI_HIP(hipGetLastError());
         rows = g->batch * G.chunks;
         ld = 2ll * C;

@@ -843,10 +843,24 @@ static LinGeom lin_geom(const gatmi_linear *l) {
 
 template <class T, int BM, int BN, int WM, int WN, bool FWD, bool CUT, bool SHORT = false, bool SHORT_N = false>
 static void lin_go(LinArgs &A, hipStream_t st) {
+    typedef typename SlopeOf<T>::type ST;
     A.tiles_n = (A.N + BN - 1) / BN;
-    A.tiles = (A.M + BM - 1) / BM * A.tiles_n;
-    const unsigned grid = (unsigned)((A.tiles + 7) / 8 * 8);
-    hipLaunchKernelGGL((lin_nt_kernel<T, BM, BN, WM, WN, FWD, CUT, SHORT, SHORT_N>), dim3(grid), dim3(WM * WN * 64), 0, st, A);
+    // a launch counts its threads in 32 bits: 2^23 blocks of 256 at most
+    const long long rows = A.M, most = (1ll << 23) / A.tiles_n * BM;
+    auto move = [](auto *p, long long bytes) { return p ? reinterpret_cast<decltype(p)>((uintptr_t)p + bytes) : p; };
+    for (long long m = 0; m < rows; m += most) {
+        LinArgs S = A;
+        S.M = rows - m < most ? rows - m : most;
+        S.A = move(A.A, m * A.K * sizeof(T));
+        S.aslope = move(A.aslope, m * A.K * sizeof(ST));
+        S.res = move(A.res, m * A.N * sizeof(T));
+        S.C = move(A.C, m * A.N * sizeof(T));
+        S.slope = move(A.slope, m * A.N * sizeof(ST));
+        S.tiles = (S.M + BM - 1) / BM * S.tiles_n;
+        const unsigned grid = (unsigned)((S.tiles + 7) / 8 * 8);
+        hipLaunchKernelGGL((lin_nt_kernel<T, BM, BN, WM, WN, FWD, CUT, SHORT, SHORT_N>), dim3(grid), dim3(WM * WN * 64), 0,
+                           st, S);
+    }
 }
 // The tile: narrow ones for narrow results; 64 x 64 while larger ones would leave compute units idle
 template <class T, bool FWD, bool CUT> static void lin_launch_nt(LinArgs A, hipStream_t st) {

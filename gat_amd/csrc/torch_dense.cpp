@@ -164,6 +164,7 @@ Tensor linear_act(const Tensor &x, const Tensor &w, const MaybeTensor &b, int64_
     check_act(me, act);
     TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && w.numel() > 0, me,
                       ": x must be [..., in] and weight [out, in], got ", x.sizes(), " and ", w.sizes());
+    TORCH_CHECK_VALUE(w.size(0) <= 65536 && w.size(1) <= 65536, me, " covers up to 65536 features, got weight ", w.sizes());
     TORCH_CHECK_VALUE(!b || (b->dim() == 1 && b->size(0) == w.size(0)), me, ": bias must be [", w.size(0), "], got ",
                       b ? b->sizes() : at::IntArrayRef());
     if (r) {
@@ -366,7 +367,7 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
     }
 };
 
-Tensor dropout(const Tensor &x, double p, bool training, uint64_t seed, const MaybeTensor &seed_dev, int64_t step,
+Tensor dropout(const Tensor &x, double p, bool training, uint64_t seed, MaybeTensor seed_dev, int64_t step,
                const MaybeTensor &r) {
     const char *me = "dropout";
     const int dtype = dtype_code(me, x);
@@ -378,9 +379,10 @@ Tensor dropout(const Tensor &x, double p, bool training, uint64_t seed, const Ma
     TORCH_CHECK_VALUE(!seed_dev || (seed_dev->scalar_type() == at::kLong && seed_dev->numel() == 1 &&
                                     seed_dev->device() == x.device()),
                       me, ": a seed tensor is one int64 on ", x.device());
-    if (!training || p == 0.0) return r ? x + *r : x;
+    if (!training) p = 0.0;
+    if (p == 0.0 && !r) return x;
     c10::DeviceGuard guard(x.device());
-    if (seed_dev) {
+    if (seed_dev && p > 0.0) {
         at::AutoDispatchBelowADInplaceOrView below;
         const_cast<Tensor &>(*seed_dev).add_(step);
     }

@@ -495,7 +495,7 @@ int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void *weight, c
  * sample, e.g. a node's channels normalised head by head. */
 #define GATMI_GROUP_NORM_MAX_CHANNELS 8192
 typedef struct gatmi_group_norm {
-    int64_t batch;         /* < 2^31; at most 65535 when length > 1 or width > 2048 (f32) / 4096 */
+    int64_t batch;         /* < 2^31 */
     int64_t length;        /* 1 .. 2^31 - 1 */
     int32_t groups, width;
     int32_t dtype, act;
