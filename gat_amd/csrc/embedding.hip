@@ -59,6 +59,20 @@ template <class T, int V> __global__ __launch_bounds__(256) void emb_fwd_kernel(
     }
 }
 
+// ---- gradient --------------------------------------------------------------------------------
+// `bytes` at p set to zero, by `blocks` blocks of which this is number `b`: the aligned middle in 16-byte
+// stores, the few bytes around it one by one
+__device__ __forceinline__ void zero_fill(char *p, long long bytes, int b, int blocks) {
+    const long long lead = (16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15, head = lead < bytes ? lead : bytes;
+    const long long n16 = (bytes - head) / 16, rest = bytes - head - n16 * 16;
+    uint4 *q = reinterpret_cast<uint4 *>(p + head);
+    for (long long i = b * 256ll + threadIdx.x; i < n16; i += blocks * 256ll) q[i] = make_uint4(0, 0, 0, 0);
+    if (b == 0 && threadIdx.x < 16) {
+        if ((long long)threadIdx.x < head) p[threadIdx.x] = 0;
+        if ((long long)threadIdx.x < rest) p[head + n16 * 16 + threadIdx.x] = 0;
+    }
+}
+
 // ---- stable radix sort of (id, position) ---------------------------------------------------------
 // `bits` (at most 9) of the key a pass: with more, a tile's runs of equal digits get shorter than a cache
 // line and the scattered stores cost more than the pass saved.  A block owns a
@@ -222,8 +236,12 @@ template <int ITEMS> __global__ __launch_bounds__(256) void sort_scatter_kernel(
     }
 }
 
-// at most kSmallSort items: all passes in one block, through LDS
-__global__ __launch_bounds__(256) void sort_small_kernel(const SortArgs A) {
+// at most kSmallSort items: all passes in one block, through LDS.  The grid's other blocks clear the gradient.
+__global__ __launch_bounds__(256) void sort_small_kernel(const SortArgs A, char *clear, long long bytes) {
+    if (blockIdx.x > 0) {
+        zero_fill(clear, bytes, blockIdx.x - 1, gridDim.x - 1);
+        return;
+    }
     constexpr int ITEMS = kSmallSort / 256;
     __shared__ uint32_t skey[kSmallSort], spos[kSmallSort], scnt[4 * 256], wsum[4];
     volatile uint32_t *cnt = scnt;
@@ -294,15 +312,13 @@ struct SegArgs {
     long long n;
     uint32_t vocab;
     int dim, chunk, W, w_log;
+    int own_entries;              // every block of columns writes the entries (to a place of its own)
     float scale;
 };
 
 template <class T, class S, int V, bool LEAF>
-__global__ __launch_bounds__(256) void seg_sum_kernel(const SegArgs A) {
-    const int lane = threadIdx.x & (A.W - 1);
-    const long long c = (long long)blockIdx.x * (256 >> A.w_log) + (threadIdx.x >> A.w_log);
+__device__ __forceinline__ void seg_chunk(const SegArgs &A, long long c, int lane) {
     const long long e0 = c * A.chunk;
-    if (e0 >= A.n) return;
     const long long e1 = e0 + A.chunk < A.n ? e0 + A.chunk : A.n;
     const int j0 = (blockIdx.y * A.W + lane) * V;
     const bool on = j0 < A.dim;
@@ -384,16 +400,42 @@ __global__ __launch_bounds__(256) void seg_sum_kernel(const SegArgs A) {
             stv<T, V>(out + (long long)cur * A.dim, acc);
         }
     }
-    if (lane == 0 && blockIdx.y == 0 && A.nentry) {
+    if (lane == 0 && (A.own_entries || blockIdx.y == 0) && A.nentry) {
         A.nentry[2 * c] = make_uint2(k0, f0);
         A.nentry[2 * c + 1] = make_uint2(k1, f1);
     }
 }
 
-__global__ __launch_bounds__(256) void emb_zero_kernel(uint4 *p16, long long n16, uint8_t *tail, int ntail) {
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n16; i += gridDim.x * 256ll) p16[i] = make_uint4(0, 0, 0, 0);
-    if (blockIdx.x == 0 && (int)threadIdx.x < ntail) tail[threadIdx.x] = 0;
+template <class T, class S, int V, bool LEAF> __global__ __launch_bounds__(256) void seg_sum_kernel(const SegArgs A) {
+    const long long c = (long long)blockIdx.x * (256 >> A.w_log) + (threadIdx.x >> A.w_log);
+    if (c * A.chunk < A.n) seg_chunk<T, S, V, LEAF>(A, c, threadIdx.x & (A.W - 1));
 }
+
+// All levels from one of at most kTailEntries entries on, in one block per block of columns: they are a few
+// chunks each and a launch apiece would cost more than the sums.  Two sets of entries and rows take turns;
+// every block of columns keeps its own copy of the entries (the same in all).
+constexpr int kTailEntries = 1024;
+struct SegTail {
+    uint2 *entry[2];      // [column blocks][2 * chunks of the first level]
+    float *src[2];
+};
+template <class T, int V> __global__ __launch_bounds__(256) void seg_tail_kernel(SegArgs A, const SegTail B) {
+    const int lane = threadIdx.x & (A.W - 1), groups = 256 >> A.w_log;
+    const long long most = 2 * ((A.n + A.chunk - 1) / A.chunk);
+    for (int l = 0;; l ^= 1) {
+        const long long chunks = (A.n + A.chunk - 1) / A.chunk;
+        A.nentry = chunks > 1 ? B.entry[l] + blockIdx.y * most : nullptr;
+        A.nsrc = B.src[l];
+        for (long long c = threadIdx.x >> A.w_log; c < chunks; c += groups) seg_chunk<T, float, V, false>(A, c, lane);
+        if (chunks <= 1) return;
+        __syncthreads();          // the next level reads what this block stored
+        A.entry = A.nentry;
+        A.src = A.nsrc;
+        A.n = 2 * chunks;
+    }
+}
+
+__global__ __launch_bounds__(256) void emb_zero_kernel(char *p, long long bytes) { zero_fill(p, bytes, blockIdx.x, gridDim.x); }
 
 constexpr int kMaxLevels = 10;
 struct EmbGeom {
@@ -422,6 +464,7 @@ static EmbGeom emb_geom(long long n, long long vocab) {
     for (long long c = (n + G.chunk0 - 1) / G.chunk0; c > 1; c = (2 * c + G.chunk - 1) / G.chunk) {
         G.entries[G.levels] = 2 * c;
         ++G.levels;
+        if (2 * c <= kTailEntries) break;      // the tail kernel takes it from here
     }
     return G;
 }
@@ -470,9 +513,9 @@ extern "C" int gatmi_embedding_fwd(int32_t dtype, int64_t n, int64_t vocab, int6
 }
 
 struct EmbWs {
-    uint2 *pair[2], *lentry[2];
+    uint2 *pair[2], *lentry[2], *tentry[2];
     uint32_t *hist, *total;
-    float *lsrc[2];
+    float *lsrc[2], *tsrc[2];
     size_t bytes;
 };
 static EmbWs emb_carve(const EmbGeom &G, long long dim, void *ws) {
@@ -485,6 +528,10 @@ static EmbWs emb_carve(const EmbGeom &G, long long dim, void *ws) {
         const long long m = G.levels > 1 + i ? G.entries[1 + i] : 0;
         w.lentry[i] = cv.take<uint2>(m);
         w.lsrc[i] = cv.take<float>(m * dim);
+        // the tail's own: what its first level leaves is the most
+        const long long t = G.levels > 1 ? 2 * ((G.entries[G.levels - 1] + G.chunk - 1) / G.chunk) : 0;
+        w.tentry[i] = cv.take<uint2>(t * ((dim + 63) / 64));
+        w.tsrc[i] = cv.take<float>(t * dim);
     }
     w.bytes = cv.off + 256;
     return w;
@@ -508,20 +555,12 @@ extern "C" int gatmi_embedding_bwd(int32_t dtype, int64_t n, int64_t vocab, int6
         return GATMI_ERR_WS;
     }
     hipStream_t st = static_cast<hipStream_t>(stream);
-    {   // every row, then the rows that have ids
+    // every row is cleared, then the rows that have ids are stored
+    const long long clear = vocab * dim * (dtype == GATMI_F32 ? 4 : 2);
+    const unsigned clear_blocks = (unsigned)(clear / 16384 < 1 ? 1 : (clear / 16384 > 8192 ? 8192 : clear / 16384));
+    if (n == 0 || n > kSmallSort) {
         ProfScope ps("embedding_zero", st);
-        const long long bytes = vocab * dim * (dtype == GATMI_F32 ? 4 : 2);
-        char *p = static_cast<char *>(grad_table);
-        const long long lead = (16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15;
-        // the aligned middle in 16-byte stores; the few bytes around it one by one
-        const long long head = lead < bytes ? lead : bytes, n16 = (bytes - head) / 16, rest = bytes - head - n16 * 16;
-        const long long b = (n16 + 1023) / 1024;
-        hipLaunchKernelGGL(emb_zero_kernel, dim3((unsigned)(b < 1 ? 1 : (b > 8192 ? 8192 : b))), dim3(256), 0, st,
-                           reinterpret_cast<uint4 *>(p + head), n16, reinterpret_cast<uint8_t *>(p + head + n16 * 16),
-                           (int)rest);
-        if (head)
-            hipLaunchKernelGGL(emb_zero_kernel, dim3(1), dim3(256), 0, st, nullptr, 0ll,
-                               reinterpret_cast<uint8_t *>(p), (int)head);
+        hipLaunchKernelGGL(emb_zero_kernel, dim3(clear_blocks), dim3(256), 0, st, static_cast<char *>(grad_table), clear);
         GATMI_HIP(hipGetLastError());
     }
     if (n == 0) return GATMI_OK;
@@ -539,7 +578,8 @@ extern "C" int gatmi_embedding_bwd(int32_t dtype, int64_t n, int64_t vocab, int6
         if (n <= kSmallSort) {
             S.ids = ids;
             S.out = w.pair[(G.passes - 1) & 1];
-            hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(256), 0, st, S);
+            hipLaunchKernelGGL(sort_small_kernel, dim3(1 + clear_blocks), dim3(256), 0, st, S,
+                               static_cast<char *>(grad_table), clear);
         }
         for (int p = 0; n > kSmallSort && p < G.passes; ++p) {
             const size_t bins = (size_t)1 << G.bits;
@@ -568,7 +608,7 @@ extern "C" int gatmi_embedding_bwd(int32_t dtype, int64_t n, int64_t vocab, int6
         A.chunk = l == 0 ? G.chunk0 : G.chunk;
         A.entry = l == 0 ? w.pair[last] : w.lentry[(l - 1) & 1];
         A.src = l == 0 ? grad_y : w.lsrc[(l - 1) & 1];
-        const bool more = l + 1 < G.levels;
+        const bool more = l + 1 < G.levels, tail = l > 0 && !more;
         A.nentry = more ? w.lentry[l & 1] : nullptr;
         A.nsrc = w.lsrc[l & 1];
         // f32 partial rows take vectors of their own width
@@ -577,8 +617,14 @@ extern "C" int gatmi_embedding_bwd(int32_t dtype, int64_t n, int64_t vocab, int6
         A.w_log = ilog2(A.W);
         const long long chunks = (A.n + A.chunk - 1) / A.chunk, per = 256 >> A.w_log;
         const dim3 grid((unsigned)((chunks + per - 1) / per), (unsigned)((dim + (long long)A.W * v - 1) / ((long long)A.W * v)));
+        const SegTail B{{w.tentry[0], w.tentry[1]}, {w.tsrc[0], w.tsrc[1]}};
+        A.own_entries = tail;
         GATMI_WITH_TYPE(dtype, {
-            if (l == 0)
+            if (tail)
+                with_vec<float>(v, [&](auto V) {
+                    hipLaunchKernelGGL((seg_tail_kernel<T, decltype(V)::value>), dim3(1, grid.y), dim3(256), 0, st, A, B);
+                });
+            else if (l == 0)
                 with_vec<T>(v, [&](auto V) {
                     hipLaunchKernelGGL((seg_sum_kernel<T, T, decltype(V)::value, true>), grid, dim3(256), 0, st, A);
                 });
