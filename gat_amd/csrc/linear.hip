@@ -145,7 +145,7 @@ template <class T, int R> struct Tile {
     }
 };
 
-constexpr int kBM = 128, kBN = 128;      // tiles of dW
+constexpr int kBM = 128;      // rows of dW's tiles
 
 struct LinArgs {
     const void *A, *B;        // [M, K] and [N, K], rows of K elements (B: of ldb)
@@ -160,6 +160,7 @@ struct LinArgs {
     int N, K, ldb, act;
     long long tiles_n, tiles;
     long long per_split;      // dW: rows of one split
+    int splits;
 };
 
 // Granule of A as it enters the products: dy * slope, rounded to the tensor's type
@@ -511,15 +512,17 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
 
 // A tile of the transposed product in LDS, as it lies in memory: contraction steps (rows of the matrix) by
 // C channels, PIECES planes.  Fragments are read with the transposing LDS load: 16 lanes fetch a block of
-// 4 steps x 16 channels, four channels each, and every lane comes back with one channel's four steps.  Rows are
-// 64 bytes apart from a multiple of 256, so that the four rows of a block lie in different banks.
+// 4 steps x 16 channels, four channels each, and every lane comes back with one channel's four steps.  The
+// 64-byte pieces of a row change places by the row's last two bits, so that the four rows of a block lie in
+// different banks.  (Rows padded by 64 bytes do the same, but then two blocks of f32 tiles miss fitting a CU.)
 template <class T, int C> struct TileT {
     static constexpr int BK = Mul<T>::BK, P = Mul<T>::PIECES;
-    static constexpr int STRIDE = C * 2 + 64, PLANE = BK * STRIDE, BYTES = PLANE * P;
+    static constexpr int STRIDE = C * 2, PLANE = BK * STRIDE, BYTES = PLANE * P;
+    static __device__ __forceinline__ int at(int row, int col) { return row * STRIDE + ((col * 2) ^ ((row & 3) << 6)); }
     static __device__ __forceinline__ void put(char *lds, int row, int col, const Gran<T> &v) {
-        char *at = lds + row * STRIDE + col * 2;
+        char *to = lds + at(row, col);
         if constexpr (P == 1) {
-            *reinterpret_cast<u32x4 *>(at) = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
+            *reinterpret_cast<u32x4 *>(to) = u32x4{v.w[0], v.w[1], v.w[2], v.w[3]};
         } else {
             uint32_t q[3][4];
 #pragma unroll
@@ -527,7 +530,7 @@ template <class T, int C> struct TileT {
                 cut3(__uint_as_float(v.w[2 * i]), __uint_as_float(v.w[2 * i + 1]), q[0][i], q[1][i], q[2][i]);
 #pragma unroll
             for (int p = 0; p < 3; ++p)
-                *reinterpret_cast<u32x4 *>(at + p * PLANE) = u32x4{q[p][0], q[p][1], q[p][2], q[p][3]};
+                *reinterpret_cast<u32x4 *>(to + p * PLANE) = u32x4{q[p][0], q[p][1], q[p][2], q[p][3]};
         }
     }
     // channels col0 .. col0 + 31, steps 16 s + 8 half .. + 7 of this lane's channel
@@ -535,9 +538,9 @@ template <class T, int C> struct TileT {
         typedef short v4s __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) v4s *lds_ptr;
         const int row = 16 * s + (lane >> 5) * 8 + ((lane & 15) >> 2), col = col0 + (lane & 16) + (lane & 3) * 4;
-        const char *at = lds + p * PLANE + row * STRIDE + col * 2;
-        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at));
-        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 4 * STRIDE));
+        const char *from = lds + p * PLANE + at(row, col);
+        const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(from));
+        const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(from + 4 * STRIDE));
         return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 };
@@ -552,8 +555,12 @@ template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void
     __shared__ __attribute__((aligned(16))) char smem[TA::BYTES + TB::BYTES];
     static_assert(TA::BYTES + TB::BYTES >= RA * kBM * 4, "the column sums fit");
     char *la = smem, *lb = smem + TA::BYTES;
-    const long long split = blockIdx.x / A.tiles;
-    const int tile = (int)(blockIdx.x - split * A.tiles);
+    // the tiles of a split read the same rows: each XCD (block index mod 8) has a contiguous range of
+    // (split, tile), so that they meet in its L2
+    const long long item = (long long)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    if (item >= A.tiles * A.splits) return;
+    const long long split = item / A.tiles;
+    const int tile = (int)(item - split * A.tiles);
     const int n0 = tile / (int)A.tiles_n * kBM, k0 = tile % (int)A.tiles_n * BN;
     const long long r0 = split * A.per_split, r1 = r0 + A.per_split < A.M ? r0 + A.per_split : A.M;
     const T *pa = static_cast<const T *>(A.A), *pb = static_cast<const T *>(A.B);
@@ -561,8 +568,10 @@ template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void
     const int wm = (wave / WN) * 64, wn = (wave % WN) * 64;
     typedef typename SlopeOf<T>::type ST;
     const bool sloped = A.aslope, sums = (A.dbpart || A.db) && k0 == 0;
-    Gran<T> ga[NA], gb[NB];
-    SlopeGran<T> gs[NA];
+    // Two steps' pieces where the registers are there: while one is stored, the other is on its way.
+    constexpr int SETS = !IsF32<T>::value && BN == 256 ? 2 : 1;
+    Gran<T> ga_[SETS][NA], gb_[SETS][NB];
+    SlopeGran<T> gs_[SETS][NA];
     VecF<8> db;
 #pragma unroll
     for (int k = 0; k < 8; ++k) db.e[k] = 0.f;
@@ -579,7 +588,10 @@ template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void
         over_b = cb - (A.K - 8);
         cb = A.K - 8;
     }
-    auto fetch = [&](long long r) {
+    auto fetch = [&](auto set, long long r) {
+        Gran<T>(&ga)[NA] = ga_[decltype(set)::value], (&gb)[NB] = gb_[decltype(set)::value];
+        SlopeGran<T>(&gs)[NA] = gs_[decltype(set)::value];
+        if (r > r1 - 1) r = r1 - 1;          // behind the end: loaded all the same, never used
         const T *ra = pa + r * A.N, *rb = pb + r * A.K;
         const ST *rs = static_cast<const ST *>(A.aslope) + r * A.N;
         const int left = (int)(r1 - 1 - r < TA::BK ? r1 - 1 - r : TA::BK);      // rows behind the last repeat it
@@ -608,8 +620,9 @@ template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
-    if (r0 < r1) fetch(r0);
-    for (long long r = r0; r < r1; r += TA::BK) {
+    auto step = [&](auto set, long long r) {
+        Gran<T>(&ga)[NA] = ga_[decltype(set)::value], (&gb)[NB] = gb_[decltype(set)::value];
+        SlopeGran<T>(&gs)[NA] = gs_[decltype(set)::value];
         const bool end = r + TA::BK > r1;
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
@@ -641,7 +654,7 @@ template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void
             TB::put(lb, tb + i * RB, jb, gb[i]);
         }
         __syncthreads();
-        if (r + TA::BK < r1) fetch(r + TA::BK);
+        fetch(set, r + SETS * TA::BK);
 #pragma unroll
         for (int s = 0; s < TA::BK / 16; ++s) {
             u32x4 a[2][TA::P], b[2][TA::P];
@@ -655,6 +668,17 @@ template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void
             mma_pieces<T, 2, 2>(a, b, acc);
         }
         __syncthreads();
+    };
+    if (r0 < r1) {
+        typedef std::integral_constant<int, 0> First;
+        typedef std::integral_constant<int, SETS - 1> Second;
+        fetch(First{}, r0);
+        if constexpr (SETS == 2) fetch(Second{}, r0 + TA::BK);
+        for (long long r = r0; r < r1; r += SETS * TA::BK) {
+            step(First{}, r);
+            if constexpr (SETS == 2)
+                if (r + TA::BK < r1) step(Second{}, r + TA::BK);
+        }
     }
     if (sums) {      // [RA][128] partial sums, added in order
         float *red = reinterpret_cast<float *>(smem);
@@ -807,6 +831,7 @@ static int lin_check(const gatmi_linear *l) {
 
 struct LinGeom {
     int splits;
+    bool wide;                      // dW's tiles: 256 columns of x, for which dz is made once, instead of 128
     long long per_split;
     int ldf, ldb;                   // row lengths of the weight images, forward and transposed
     size_t image_f, image_b, slabs, dbpart;     // bytes
@@ -816,16 +841,33 @@ struct LinGeom {
 constexpr long long kCutRows = 2048;
 constexpr int kFewRows = 16;
 
+static long long lin_dw_tiles(const gatmi_linear *l, bool wide) {
+    const int bn = wide ? 256 : 128;
+    return ((l->out_features + kBM - 1ll) / kBM) * ((l->in_features + bn - 1ll) / bn);
+}
+
 static LinGeom lin_geom(const gatmi_linear *l) {
     LinGeom G;
     memset(&G, 0, sizeof(G));
     const size_t el = l->dtype == GATMI_F32 ? 6 : 2;
-    const long long tiles = ((l->out_features + kBM - 1ll) / kBM) * ((l->in_features + kBN - 1ll) / kBN);
-    // enough splits of the rows for two blocks a CU, at least 256 rows each
-    long long s = (2ll * device_cus() + tiles - 1) / tiles;
-    const long long most = (l->rows + 255) / 256;
-    if (s > most) s = most;
-    if (s < 1) s = 1;
+    G.wide = l->in_features > 128;
+    const long long tiles = lin_dw_tiles(l, G.wide);
+    // The rows are split so that the blocks fill the chip a whole number of times: a wide block's registers
+    // leave room for no second one on its CU, of narrow ones two fit.  In units of a row of one block: a round
+    // of blocks takes its rows and about 256 more for its start and its slab, a slab's way through memory
+    // N K / 2^14.  At least 256 rows a split.
+    const long long slots = device_cus() * (G.wide ? 1ll : 2ll), most = (l->rows + 255) / 256;
+    long long s = 1, best = -1;
+    for (long long rounds = 1; rounds <= 4; ++rounds) {
+        long long c = rounds * slots / tiles;
+        c = c < 1 ? 1 : (c > most && most > 0 ? most : c);
+        const long long t = (c * tiles + slots - 1) / slots * (l->rows / c + 256) +
+                            c * ((long long)l->out_features * l->in_features >> 14);
+        if (best < 0 || t < best) {
+            best = t;
+            s = c;
+        }
+    }
     const int bk = l->dtype == GATMI_F32 ? 32 : 64;
     G.per_split = ((l->rows + s - 1) / s + bk - 1) / bk * bk;
     if (G.per_split < bk) G.per_split = bk;
@@ -979,13 +1021,14 @@ extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void
         A.dw = one ? grad_weight : nullptr;
         A.db = one ? grad_bias : nullptr;
         A.per_split = G.per_split;
+        A.splits = G.splits;
         GATMI_WITH_TYPE(l->dtype, {
-            const bool wide = K > 128;      // dz is made once for twice the columns of x
+            const bool wide = G.wide;
             A.tiles_n = (K + (wide ? 255 : 127)) / (wide ? 256 : 128);
-            A.tiles = (long long)((N + kBM - 1) / kBM) * A.tiles_n;
+            A.tiles = lin_dw_tiles(l, wide);
             auto tn = N < 8 || K < 8 ? (wide ? lin_tn_kernel<T, 256, true> : lin_tn_kernel<T, 128, true>)
                                      : (wide ? lin_tn_kernel<T, 256, false> : lin_tn_kernel<T, 128, false>);
-            hipLaunchKernelGGL(tn, dim3((unsigned)(A.tiles * G.splits)), dim3(wide ? 512 : 256), 0, st, A);
+            hipLaunchKernelGGL(tn, dim3((unsigned)((A.tiles * G.splits + 7) / 8 * 8)), dim3(wide ? 512 : 256), 0, st, A);
             const long long size = (long long)N * K;
             if (grad_weight && !one)
                 hipLaunchKernelGGL((lin_slabs_kernel<T>), dim3((unsigned)((size + 63) / 64)), dim3(256), 0, st, slabs,
