@@ -160,7 +160,8 @@ struct LinArgs {
     int N, K, ldb, act;
     long long tiles_n, tiles;
     long long per_split;      // dW: rows of one split
-    int splits;
+    int splits;               // dW: of the rows; PART: of the contraction, in pieces of k_split
+    int k_split;
 };
 
 // Granule of A as it enters the products: dy * slope, rounded to the tensor's type
@@ -334,8 +335,9 @@ template <bool FWD> __device__ __forceinline__ float plain_dot(const LinArgs &A,
 
 // C[m][n] = epilogue(sum_k A[m][k] B[n][k]).  FWD: bias, activation, residual, slope; else A = dy * aslope
 // when given.  CUT (f32): B comes as three planes of bf16 pieces, rows of ldb (a multiple of 8, zeros behind K).
-// SHORT: K < 8; SHORT_N: N < 8.
-template <class T, int BM, int BN, int WM, int WN, bool FWD, bool CUT, bool SHORT, bool SHORT_N>
+// SHORT: K < 8; SHORT_N: N < 8.  PART: a block takes one piece of the contraction and leaves its sums in
+// part [splits][M][N], for lin_join_kernel.
+template <class T, int BM, int BN, int WM, int WN, bool FWD, bool CUT, bool SHORT, bool SHORT_N, bool PART>
 __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void lin_nt_kernel(const LinArgs A) {
     typedef Tile<T, BM> TA;
     typedef Tile<T, BN> TB;
@@ -345,8 +347,11 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
     __shared__ __attribute__((aligned(16))) char smem[kLoop > kEpi ? kLoop : kEpi];
     char *la = smem, *lb = smem + TA::BYTES;
     // consecutive tiles share rows of A: give each XCD (block index mod 8) a contiguous range of them
-    const long long tile = (long long)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-    if (tile >= A.tiles) return;
+    const long long item = (long long)(blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    if (item >= (PART ? A.tiles * A.splits : A.tiles)) return;
+    const long long split = PART ? item / A.tiles : 0, tile = item - split * A.tiles;
+    const int k_first = PART ? (int)split * A.k_split : 0;
+    const int k_end = PART && k_first + A.k_split < A.K ? k_first + A.k_split : A.K;
     const long long m0 = tile / A.tiles_n * BM;
     const int n0 = (int)(tile % A.tiles_n) * BN;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -411,8 +416,8 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
         for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
-    fetch(0);
-    for (int k0 = 0; k0 < A.K; k0 += TA::BK) {
+    fetch(k_first);
+    for (int k0 = k_first; k0 < k_end; k0 += TA::BK) {
         // the row's last, partial step: what a granule holds of the one before it is dropped.  An image has
         // zeros behind K instead of a step back, in its place: A must line up, so it is moved down there.
         const bool end = !SHORT && k0 + TA::BK > A.K;
@@ -439,9 +444,23 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
             }
         }
         __syncthreads();
-        if (k0 + TA::BK < A.K) fetch(k0 + TA::BK);
+        if (k0 + TA::BK < k_end) fetch(k0 + TA::BK);
         tile_mma<T, BM, BN, MI, NI>(la, lb, wm, wn, lane, acc);
         __syncthreads();
+    }
+    if constexpr (PART) {
+        float *part = A.part + split * A.M * A.N;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) {
+                    const long long m = m0 + wm + i * 32 + acc_row(q, lane >> 5);
+                    const int n = n0 + wn + j * 32 + (lane & 31);
+                    if (m < A.M && n < A.N) part[m * A.N + n] = acc[i][j][q];
+                }
+        return;
     }
     // epilogue: a wave turns its blocks 16 rows at a time through LDS of its own into row pieces of 8
     float *le = reinterpret_cast<float *>(smem) + wave * 16 * LD;
@@ -508,6 +527,26 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
             }
         }
     }
+}
+
+// The sums of a split contraction, joined in order, and what the product's own epilogue would have done
+template <class T, bool FWD> __global__ __launch_bounds__(256) void lin_join_kernel(const LinArgs A) {
+    const long long at = blockIdx.x * 256ll + threadIdx.x, size = A.M * A.N;
+    if (at >= size) return;
+    float v = 0.f;
+#pragma unroll 8
+    for (int q = 0; q < A.splits; ++q) v += A.part[q * size + at];
+    const long long m = at / A.N;
+    const int n = (int)(at - m * A.N);
+    if (IsF32<T>::value && !(fabsf(v) < INFINITY)) v = plain_dot<FWD>(A, m, n);
+    if constexpr (FWD) {
+        const float z = v + (A.bias ? (float)static_cast<const T *>(A.bias)[n] : 0.f);
+        float d = 1.f;
+        GATMI_WITH_ACT(A.act, v = (act_both<ACT, IsF32<T>::value>(z, d)));
+        if (A.slope) static_cast<typename SlopeOf<T>::type *>(A.slope)[at] = slope_out<T>(d);
+        if (A.res) v += (float)static_cast<const T *>(A.res)[at];
+    }
+    static_cast<T *>(A.C)[at] = (T)v;
 }
 
 // A tile of the transposed product in LDS, as it lies in memory: contraction steps (rows of the matrix) by
@@ -829,17 +868,46 @@ static int lin_check(const gatmi_linear *l) {
     return GATMI_OK;
 }
 
+// From this many rows on the f32 forward reads its weights as pieces cut once, not by every block
+constexpr long long kCutRows = 2048;
+// Up to this many rows go without the matrix cores, but 16-bit ones above four where the contraction is split:
+// 16 rows of [1024, 1024] bf16 take 8.0 us so and 5.9 in pieces, f32 5.5 and 7.3
+constexpr int kFewRows = 16;
+
+// Few tiles and a long contraction: a step of it takes a lone block 0.5 us (f32: 0.7), most of that waiting on
+// itself, and the chip is empty beside it.  Pieces of at least two steps, as many as give two blocks a CU, and a
+// kernel that joins them (2 us): from six (f32) or eight steps saved on, while the tiles are at most half the CUs.
+// [64, 1024] x [1024, 1024] bf16 12.0 -> 6.8 us, f32 29.7 -> 8.8; [1024, 1024] x [1024, 1024], 256 tiles, bf16
+// 12.8 -> 16.3, so not there.
+struct LinSplitK {
+    int splits, k_split;
+    size_t bytes;
+};
+static LinSplitK lin_split_k(long long M, int N, int K, int dtype) {
+    LinSplitK S = {1, K, 0};
+    if (M < 1) return S;
+    const int bk = dtype == GATMI_F32 ? 32 : 64, steps = (K + bk - 1) / bk;
+    const long long tiles = (M + 63) / 64 * ((N + 63) / 64), room = 2ll * device_cus() / tiles;
+    const long long want = room < (steps + 1) / 2 ? room : (steps + 1) / 2;
+    if (want < 2 || room < 4) return S;
+    const int each = (int)((steps + want - 1) / want);
+    if (steps - each < (dtype == GATMI_F32 ? 6 : 8)) return S;
+    S.k_split = each * bk;
+    S.splits = (steps + each - 1) / each;
+    S.bytes = align_up((size_t)S.splits * M * N * 4);
+    return S;
+}
+
 struct LinGeom {
     int splits;
     bool wide;                      // dW's tiles: 256 columns of x, for which dz is made once, instead of 128
     long long per_split;
     int ldf, ldb;                   // row lengths of the weight images, forward and transposed
     size_t image_f, image_b, slabs, dbpart;     // bytes
+    LinSplitK fwd, dx;
     bool image_fwd;                 // the forward takes an image
+    bool few;                       // ... or the few-row kernel
 };
-// From this many rows on the f32 forward reads its weights as pieces cut once, not by every block
-constexpr long long kCutRows = 2048;
-constexpr int kFewRows = 16;
 
 static long long lin_dw_tiles(const gatmi_linear *l, bool wide) {
     const int bn = wide ? 256 : 128;
@@ -876,6 +944,10 @@ static LinGeom lin_geom(const gatmi_linear *l) {
     G.ldf = (l->in_features + 7) / 8 * 8;
     G.ldb = (l->out_features + 7) / 8 * 8;
     G.image_fwd = l->dtype == GATMI_F32 && l->rows >= kCutRows;
+    G.fwd = lin_split_k(l->rows, l->out_features, l->in_features, l->dtype);
+    G.few = l->rows <= 4 || (l->rows <= kFewRows && (l->dtype == GATMI_F32 || G.fwd.splits == 1));
+    if (G.few) G.fwd = {1, l->in_features, 0};
+    G.dx = lin_split_k(l->rows, l->in_features, l->out_features, l->dtype);
     G.image_f = G.image_fwd ? align_up((size_t)l->out_features * G.ldf * el) : 0;
     G.image_b = align_up((size_t)l->in_features * G.ldb * el);
     G.slabs = align_up((size_t)G.splits * l->in_features * l->out_features * 4);
@@ -900,12 +972,22 @@ static void lin_go(LinArgs &A, hipStream_t st) {
         S.slope = move(A.slope, m * A.N * sizeof(ST));
         S.tiles = (S.M + BM - 1) / BM * S.tiles_n;
         const unsigned grid = (unsigned)((S.tiles + 7) / 8 * 8);
-        hipLaunchKernelGGL((lin_nt_kernel<T, BM, BN, WM, WN, FWD, CUT, SHORT, SHORT_N>), dim3(grid), dim3(WM * WN * 64), 0,
+        hipLaunchKernelGGL((lin_nt_kernel<T, BM, BN, WM, WN, FWD, CUT, SHORT, SHORT_N, false>), dim3(grid), dim3(WM * WN * 64), 0,
                            st, S);
     }
 }
 // The tile: narrow ones for narrow results; 64 x 64 while larger ones would leave compute units idle
-template <class T, bool FWD, bool CUT> static void lin_launch_nt(LinArgs A, hipStream_t st) {
+template <class T, bool FWD, bool CUT> static void lin_launch_nt(LinArgs A, const LinSplitK &S, hipStream_t st) {
+    if (S.splits > 1) {
+        A.splits = S.splits;
+        A.k_split = S.k_split;
+        A.tiles_n = (A.N + 63) / 64;
+        A.tiles = (A.M + 63) / 64 * A.tiles_n;
+        const unsigned grid = (unsigned)((A.tiles * A.splits + 7) / 8 * 8);
+        hipLaunchKernelGGL((lin_nt_kernel<T, 64, 64, 2, 2, FWD, CUT, false, false, true>), dim3(grid), dim3(256), 0, st, A);
+        hipLaunchKernelGGL((lin_join_kernel<T, FWD>), dim3((unsigned)((A.M * A.N + 255) / 256)), dim3(256), 0, st, A);
+        return;
+    }
     const long long big = (A.M + 127) / 128 * ((A.N + 127) / 128);
     if (A.K < 8) lin_go<T, 64, 64, 2, 2, FWD, CUT, true, true>(A, st);
     else if (A.N < 8) lin_go<T, 128, 32, 4, 1, FWD, CUT, false, true>(A, st);
@@ -921,7 +1003,8 @@ using namespace gatmi;
 
 extern "C" size_t gatmi_linear_fwd_workspace_bytes(const gatmi_linear *l) {
     if (lin_check(l)) return 0;
-    return lin_geom(l).image_f;
+    const LinGeom G = lin_geom(l);
+    return G.image_f + G.fwd.bytes;
 }
 
 extern "C" int gatmi_linear_fwd(const gatmi_linear *l, const void *x, const void *weight, const void *bias,
@@ -930,8 +1013,9 @@ extern "C" int gatmi_linear_fwd(const gatmi_linear *l, const void *x, const void
     if (l->rows == 0) return GATMI_OK;
     GATMI_REQUIRE(x && weight && y, "linear_fwd: null argument");
     const LinGeom G = lin_geom(l);
-    if (ws_bytes < G.image_f || (G.image_f && !ws)) {
-        set_error("linear workspace too small: %zu < %zu", ws_bytes, G.image_f);
+    const size_t need = G.image_f + G.fwd.bytes;
+    if (ws_bytes < need || (need && !ws)) {
+        set_error("linear workspace too small: %zu < %zu", ws_bytes, need);
         return GATMI_ERR_WS;
     }
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -947,8 +1031,9 @@ extern "C" int gatmi_linear_fwd(const gatmi_linear *l, const void *x, const void
     A.M = l->rows;
     A.N = l->out_features;
     A.K = A.ldb = l->in_features;
+    A.part = reinterpret_cast<float *>(static_cast<char *>(ws) + G.image_f);
     ProfScope ps("linear_fwd", st);
-    if (l->rows <= kFewRows) {
+    if (G.few) {
         GATMI_WITH_TYPE(l->dtype, {
             auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((A.N + 3) / 4), dim3(256), 0, st, A); };
             if (A.M == 1) go(lin_rows_kernel<T, 1>);
@@ -960,9 +1045,9 @@ extern "C" int gatmi_linear_fwd(const gatmi_linear *l, const void *x, const void
                            static_cast<const float *>(weight), A.N, A.K, G.ldf, ws);
         A.B = ws;
         A.ldb = G.ldf;
-        lin_launch_nt<float, true, true>(A, st);
+        lin_launch_nt<float, true, true>(A, G.fwd, st);
     } else {
-        GATMI_WITH_TYPE(l->dtype, (lin_launch_nt<T, true, false>(A, st)));
+        GATMI_WITH_TYPE(l->dtype, (lin_launch_nt<T, true, false>(A, G.fwd, st)));
     }
     GATMI_HIP(hipGetLastError());
     return GATMI_OK;
@@ -971,7 +1056,7 @@ extern "C" int gatmi_linear_fwd(const gatmi_linear *l, const void *x, const void
 extern "C" size_t gatmi_linear_bwd_workspace_bytes(const gatmi_linear *l) {
     if (lin_check(l)) return 0;
     const LinGeom G = lin_geom(l);
-    return G.image_b + G.slabs + G.dbpart;
+    return G.image_b + (G.slabs + G.dbpart > G.dx.bytes ? G.slabs + G.dbpart : G.dx.bytes);
 }
 
 extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void *weight, const void *slope,
@@ -981,8 +1066,9 @@ extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void
     GATMI_REQUIRE(l->rows == 0 || (x && weight && grad_y), "linear_bwd: null argument");
     GATMI_REQUIRE(l->act == GATMI_ACT_NONE || slope || l->rows == 0, "linear_bwd: the activation's slope is missing");
     const LinGeom G = lin_geom(l);
-    if (!ws || ws_bytes < G.image_b + G.slabs + G.dbpart) {
-        set_error("linear workspace too small: %zu < %zu", ws_bytes, G.image_b + G.slabs + G.dbpart);
+    const size_t need = gatmi_linear_bwd_workspace_bytes(l);
+    if (!ws || ws_bytes < need) {
+        set_error("linear workspace too small: %zu < %zu", ws_bytes, need);
         return GATMI_ERR_WS;
     }
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -999,13 +1085,14 @@ extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void
         A.plain = weight;
         A.B = image;
         A.C = grad_x;
+        A.part = slabs;         // (dW's turn comes after)
         A.N = K;
         A.K = N;
         A.ldb = G.ldb;
         GATMI_WITH_TYPE(l->dtype, {
             hipLaunchKernelGGL((lin_image_kernel<T, true>), dim3((G.ldb + 31) / 32, (K + 31) / 32), dim3(256), 0, st,
                                static_cast<const T *>(weight), N, K, G.ldb, ws);
-            lin_launch_nt<T, false, IsF32<T>::value>(A, st);
+            lin_launch_nt<T, false, IsF32<T>::value>(A, G.dx, st);
         });
         GATMI_HIP(hipGetLastError());
     }

@@ -86,3 +86,39 @@ def test_dropout_off_with_residual(cuda, dtype):
         up = torch.randn_like(y)
         assert all(torch.equal(g, up) for g in torch.autograd.grad(y, (x, r), up))
     assert int(seed) == 5        # nothing drawn, not moved on
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("m,k,n", [(17, 1024, 64), (5, 700, 30), (16, 2050, 9), (64, 515, 1025), (300, 1001, 3),
+                                   (200, 40, 1500), (1, 33, 3001), (3000, 777, 7)])
+def test_linear_split_contraction(cuda, dtype, m, k, n):
+    """few tiles and a long contraction (of the forward's, the second half of the gradient's)"""
+    from test_gpu_dense import linear_case
+    linear_case(cuda, dtype, m, k, n, "silu", True, True)
+    linear_case(cuda, dtype, m, k, n, "none", False, False)
+
+
+def test_linear_split_contraction_not_finite(cuda):
+    """infinities and NaN in f32 as plain f32 sums have them, forward and backward, when the contraction is split"""
+    import gat_amd
+    g = torch.Generator().manual_seed(4)
+    x, w = torch.randn(40, 1024, generator=g), torch.randn(70, 1024, generator=g)
+    x[3, 5], x[7, 900], w[11, 2], x[9, 9], w[20, 9] = float("inf"), float("nan"), float("-inf"), 3.0e38, 0.999
+    x[12, :2], w[12, :2] = torch.tensor([3.0e38, -3.0e38]), 1.0
+    xd, wd = x.to(cuda).requires_grad_(True), w.to(cuda).requires_grad_(True)
+    y = gat_amd.linear_act(xd, wd)
+    want = x.double() @ w.double().t()
+    # where the terms' sizes sum up to a float, every partial sum is one, whatever the order; elsewhere (3e38 * 2)
+    # plain f32 sums overflow too
+    same = x.double().abs() @ w.double().abs().t() < 3.4e38
+    got = y.detach().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got[torch.isinf(want)].double(), want[torch.isinf(want)])
+    assert bool(torch.isfinite(got[same]).all())
+    dy = torch.randn(40, 70, generator=g)
+    dy[2, 8] = float("inf")
+    gx, gw = torch.autograd.grad(y, (xd, wd), dy.to(cuda))
+    for got, want in ((gx, dy.double() @ w.double()), (gw, dy.double().t() @ x.double())):
+        assert torch.equal(torch.isnan(got.cpu()), torch.isnan(want))
+        inf = torch.isinf(want)
+        assert torch.equal(got.cpu().double()[inf], want[inf])
