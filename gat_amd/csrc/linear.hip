@@ -272,24 +272,24 @@ __device__ __forceinline__ void tile_mma(const char *la, const char *lb, int ra,
 __device__ __forceinline__ int acc_row(int q, int half) { return (q >> 2) * 8 + half * 4 + (q & 3); }
 
 // eight columns of one row on their way out: bias, activation, residual, slope
-template <class T, int ACT> __device__ __forceinline__ void epi_values(float (&v)[8], const float (&bias)[8],
+template <class T, int ACT> __device__ __forceinline__ void epi_values(float (&v)[8], const VecF<8> &bias,
                                                                      typename SlopeOf<T>::type (&sl)[8]) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         float d;
-        v[k] = act_both<ACT, IsF32<T>::value>(v[k] + bias[k], d);
+        v[k] = act_both<ACT, IsF32<T>::value>(v[k] + bias.e[k], d);
         sl[k] = slope_out<T>(d);
     }
 }
 template <class T, bool FWD>
 __device__ __forceinline__ void epi_piece(const LinArgs &A, long long m, int n, int have, float (&v)[8],
-                                          const float (&bias)[8], const Gran<T> &res) {
+                                          const Gran<T> &bias, const Gran<T> &res) {
     typedef typename SlopeOf<T>::type ST;
     const long long at = m * A.N + n;
     T *out = static_cast<T *>(A.C) + at;
     ST sl[8];
     if constexpr (FWD) {
-        GATMI_WITH_ACT(A.act, epi_values<T, ACT>(v, bias, sl));
+        GATMI_WITH_ACT(A.act, epi_values<T, ACT>(v, gran_values<T>(bias), sl));
         if (A.slope) {
             ST *so = static_cast<ST *>(A.slope) + at;
             if (have >= 8) {
@@ -371,29 +371,24 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
     const ST *bs = static_cast<const ST *>(A.aslope) + m0 * A.K;
     const char *bb = static_cast<const char *>(A.B) + (long long)n0 * A.ldb * (CUT ? 2 : (int)sizeof(T));
     const long long plane = (long long)A.N * A.ldb * 2;
-    uint32_t ra[NA], rb[NB];        // row offsets in elements
-#pragma unroll
-    for (int i = 0; i < NA; ++i) {
-        const long long left = A.M - 1 - m0;
-        const int r = row + i * RP;
-        ra[i] = (uint32_t)(r < left ? r : (int)left) * (uint32_t)A.K;
-    }
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-        const int left = A.N - 1 - n0, r = row + i * RP;
-        rb[i] = (uint32_t)(r < left ? r : left) * (uint32_t)A.ldb;
-    }
+    const int left_a = A.M - 1 - m0 < BM ? (int)(A.M - 1 - m0) : BM, left_b = A.N - 1 - n0;
     const int last = CUT ? A.ldb - 8 : A.K - 8;     // B's last whole granule
     auto fetch = [&](int k0) {
         const int k = k0 + g * 8, ka = SHORT ? k : (k < A.K - 8 ? k : A.K - 8), kb = SHORT && !CUT ? k : (k < last ? k : last);
+        // Rows' offsets in elements, made again at every step: kept, they are the registers that do not fit and
+        // went to scratch memory.  The compiler must not know that they are the same each time.
+        int row_ = row;
+        asm volatile("" : "+v"(row_));
+        auto row_a = [&](int i) { return __umul24(row_ + i * RP < left_a ? row_ + i * RP : left_a, A.K); };
+        auto row_b = [&](int i) { return __umul24(row_ + i * RP < left_b ? row_ + i * RP : left_b, A.ldb); };
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
             if constexpr (SHORT) {
-                ga[i] = ld_gran_short<T>(ba, (ra[i] + ka) * (uint32_t)sizeof(T), A.K - k);
-                if (!FWD && sloped) gs[i] = ld_slope_short<T>(bs, (ra[i] + ka) * (uint32_t)sizeof(ST), A.K - k);
+                ga[i] = ld_gran_short<T>(ba, (row_a(i) + ka) * (uint32_t)sizeof(T), A.K - k);
+                if (!FWD && sloped) gs[i] = ld_slope_short<T>(bs, (row_a(i) + ka) * (uint32_t)sizeof(ST), A.K - k);
             } else {
-                ga[i] = ld_gran<T>(ba, (ra[i] + ka) * (uint32_t)sizeof(T));
-                if (!FWD && sloped) gs[i] = ld_slope<T>(bs, (ra[i] + ka) * (uint32_t)sizeof(ST));
+                ga[i] = ld_gran<T>(ba, (row_a(i) + ka) * (uint32_t)sizeof(T));
+                if (!FWD && sloped) gs[i] = ld_slope<T>(bs, (row_a(i) + ka) * (uint32_t)sizeof(ST));
             }
         }
 #pragma unroll
@@ -401,11 +396,11 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
             if constexpr (CUT) {
 #pragma unroll
                 for (int p = 0; p < 3; ++p)
-                    gc[i][p] = *reinterpret_cast<const u32x4 *>(bb + p * plane + (rb[i] + kb) * 2u);
+                    gc[i][p] = *reinterpret_cast<const u32x4 *>(bb + p * plane + (row_b(i) + kb) * 2u);
             } else if constexpr (SHORT) {
-                gb[i] = ld_gran_short<T>(bb, (rb[i] + kb) * (uint32_t)sizeof(T), A.K - k);
+                gb[i] = ld_gran_short<T>(bb, (row_b(i) + kb) * (uint32_t)sizeof(T), A.K - k);
             } else {
-                gb[i] = ld_gran<T>(bb, (rb[i] + kb) * (uint32_t)sizeof(T));
+                gb[i] = ld_gran<T>(bb, (row_b(i) + kb) * (uint32_t)sizeof(T));
             }
         }
     };
@@ -468,33 +463,32 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
     const int half = lane >> 5, c8 = (lane % PR) * 8, rr = lane / PR;
     const int n = n0 + wn + c8;
     const int have = A.N - n;                       // columns of this piece that exist
-    // the residual's pieces of a 32-row block are on their way before the first of them is used
-    constexpr int PP = 16 / RI;
-    Gran<T> res[2][PP];
-    auto fetch_res = [&](int i) {
+    // the residual's pieces are on their way before they are used: of a 32-row block for f32, of 16 rows for
+    // 16-bit types, whose four waves a SIMD have no registers for more
+    constexpr int PP = 16 / RI, AHEAD = IsF32<T>::value ? 2 : 1;
+    Gran<T> res[AHEAD][PP];
+    auto fetch_res = [&](int i, int h0) {
         const T *br = static_cast<const T *>(A.res) + (m0 + wm) * A.N;
         const long long left = A.M - 1 - (m0 + wm);
         const int nc = SHORT_N || n <= A.N - 8 ? n : A.N - 8;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < AHEAD; ++h)
 #pragma unroll
             for (int p = 0; p < PP; ++p) {
-                const int r = i * 32 + h * 16 + p * RI + rr;
+                const int r = i * 32 + (h0 + h) * 16 + p * RI + rr;
                 // a wave whose rows all lie behind the matrix reads the row before them
                 const long long at = (r < left ? r : left) * (long long)A.N + nc;
                 if constexpr (SHORT_N) res[h][p] = ld_gran_short<T>(br + at, 0, have);
                 else res[h][p] = ld_gran<T>(br + at, 0);
             }
     };
-    float bias[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-        bias[k] = FWD && A.bias && k < have ? (float)static_cast<const T *>(A.bias)[n + k] : 0.f;
+    Gran<T> bias;       // (as it lies in memory: half the registers of f32 ones for 16-bit types)
+    if (FWD) bias = ld_gran_short<T>(A.bias, (uint32_t)n * sizeof(T), A.bias ? have : 0);
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-        if (FWD && A.res) fetch_res(i);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            if (FWD && A.res && h % AHEAD == 0) fetch_res(i, h);
             // the wave's own LDS, in order: what it stored before is read before it stores again
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
@@ -522,8 +516,8 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
                         for (int k = 0; k < 8; ++k) v[k] = row[k];
                     }
                 }
-                if (FWD && !SHORT_N && have < 8 && A.res) shift_down<T>(res[h][p].w, 8 - have);
-                epi_piece<T, FWD>(A, m, n, have, v, bias, res[h][p]);
+                if (FWD && !SHORT_N && have < 8 && A.res) shift_down<T>(res[h % AHEAD][p].w, 8 - have);
+                epi_piece<T, FWD>(A, m, n, have, v, bias, res[h % AHEAD][p]);
             }
         }
     }
