@@ -98,6 +98,14 @@ def test_linear_split_contraction(cuda, dtype, m, k, n):
     linear_case(cuda, dtype, m, k, n, "none", False, False)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("m,k,n", [(33000, 256, 192), (32769, 192, 200), (66001, 64, 72)])
+def test_linear_whole_steps(cuda, dtype, m, k, n):
+    """contractions of whole steps over many large tiles, the last of them partial"""
+    from test_gpu_dense import linear_case
+    linear_case(cuda, dtype, m, k, n, "elu", True, True)
+
+
 def test_linear_split_contraction_not_finite(cuda):
     """infinities and NaN in f32 as plain f32 sums have them, forward and backward, when the contraction is split"""
     import gat_amd
