@@ -837,29 +837,29 @@ template <class T, int MR> __global__ __launch_bounds__(256) void lin_rows_kerne
     static_cast<T *>(A.C)[at] = (T)y;
 }
 
-// dW = sum of the slabs, in order.  64 values by 4 groups of slabs a block: few values and hundreds of slabs
-// still make many loads
-template <class T> __global__ __launch_bounds__(256) void lin_slabs_kernel(const float *part, int splits, long long size, T *out) {
-    __shared__ float red[256];
-    const int lane = threadIdx.x & 63, grp = threadIdx.x >> 6;
-    const long long i = blockIdx.x * 64ll + lane;
-    float s = 0.f;
-    if (i < size)
-#pragma unroll 8
-        for (int q = grp; q < splits; q += 4) s += part[q * size + i];
-    red[threadIdx.x] = s;
-    __syncthreads();
-    if (grp == 0 && i < size) out[i] = (T)(((s + red[64 + lane]) + red[128 + lane]) + red[192 + lane]);
-}
-
-// db = sum of the splits' column sums, in order
-template <class T> __global__ __launch_bounds__(256) void lin_db_kernel(const float *part, int splits, int N, T *db) {
+// dW = sum of the slabs and db = sum of the splits' column sums, in order: the first `dw_blocks` blocks and the
+// others.  64 values by 4 groups of slabs a block (8 by 32 for db): few values and hundreds of slabs still make
+// many loads
+template <class T> __global__ __launch_bounds__(256) void lin_slabs_kernel(const float *part, int splits, long long size, T *dw,
+                                                                          int dw_blocks, const float *dbpart, int N, T *db) {
     __shared__ double red[256];
-    const int c = blockIdx.x * 8 + (threadIdx.x & 7), rg = threadIdx.x >> 3;
+    if ((int)blockIdx.x < dw_blocks) {
+        const int lane = threadIdx.x & 63, grp = threadIdx.x >> 6;
+        const long long i = blockIdx.x * 64ll + lane;
+        float s = 0.f;
+        if (i < size)
+#pragma unroll 8
+            for (int q = grp; q < splits; q += 4) s += part[q * size + i];
+        red[threadIdx.x] = s;
+        __syncthreads();
+        if (grp == 0 && i < size) dw[i] = (T)(float)(((s + red[64 + lane]) + red[128 + lane]) + red[192 + lane]);
+        return;
+    }
+    const int c = (blockIdx.x - dw_blocks) * 8 + (threadIdx.x & 7), rg = threadIdx.x >> 3;
     double s = 0.0;
     if (c < N)
 #pragma unroll 4
-        for (int b = rg; b < splits; b += 32) s += part[(long long)b * N + c];
+        for (int b = rg; b < splits; b += 32) s += dbpart[(long long)b * N + c];
     red[threadIdx.x] = s;
     __syncthreads();
     if (rg == 0 && c < N) {
@@ -1155,18 +1155,17 @@ extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void
         A.splits = G.splits;
         GATMI_WITH_TYPE(l->dtype, {
             const bool wide = G.wide;
-            A.tiles_n = (K + (wide ? 255 : 127)) / (wide ? 256 : 128);
-            A.tiles = lin_dw_tiles(l, wide);
+            // (without dW the first column of tiles does: its blocks leave the column sums)
+            A.tiles_n = grad_weight ? (K + (wide ? 255 : 127)) / (wide ? 256 : 128) : 1;
+            A.tiles = grad_weight ? lin_dw_tiles(l, wide) : (N + kBM - 1) / kBM;
             auto tn = N < 8 || K < 8 ? (wide ? lin_tn_kernel<T, 256, true> : lin_tn_kernel<T, 128, true>)
                                      : (wide ? lin_tn_kernel<T, 256, false> : lin_tn_kernel<T, 128, false>);
             hipLaunchKernelGGL(tn, dim3((unsigned)((A.tiles * G.splits + 7) / 8 * 8)), dim3(wide ? 512 : 256), 0, st, A);
             const long long size = (long long)N * K;
-            if (grad_weight && !one)
-                hipLaunchKernelGGL((lin_slabs_kernel<T>), dim3((unsigned)((size + 63) / 64)), dim3(256), 0, st, slabs,
-                                   G.splits, size, static_cast<T *>(grad_weight));
-            if (grad_bias && !one)
-                hipLaunchKernelGGL((lin_db_kernel<T>), dim3((N + 7) / 8), dim3(256), 0, st, dbpart, G.splits, N,
-                                   static_cast<T *>(grad_bias));
+            const int dw_blocks = grad_weight ? (int)((size + 63) / 64) : 0, db_blocks = grad_bias ? (N + 7) / 8 : 0;
+            if (!one)
+                hipLaunchKernelGGL((lin_slabs_kernel<T>), dim3(dw_blocks + db_blocks), dim3(256), 0, st, slabs, G.splits, size,
+                                   static_cast<T *>(grad_weight), dw_blocks, dbpart, N, static_cast<T *>(grad_bias));
         });
         GATMI_HIP(hipGetLastError());
     }

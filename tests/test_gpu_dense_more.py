@@ -130,3 +130,15 @@ def test_linear_split_contraction_not_finite(cuda):
         assert torch.equal(torch.isnan(got.cpu()), torch.isnan(want))
         inf = torch.isinf(want)
         assert torch.equal(got.cpu().double()[inf], want[inf])
+
+
+def test_linear_gradient_of_the_bias_alone(cuda):
+    """weights frozen, many splits of the rows, more columns of x than one tile"""
+    import gat_amd
+    g = torch.Generator().manual_seed(9)
+    x, w, b = torch.randn(9000, 300, generator=g), torch.randn(140, 300, generator=g) / 17, torch.randn(140, generator=g)
+    dy = torch.randn(9000, 140, generator=g)
+    ref = R.Linear(x, w, b, None, "gelu", dy, F32)
+    bd = b.to(cuda).requires_grad_(True)
+    (db,) = torch.autograd.grad(gat_amd.linear_act(x.to(cuda), w.to(cuda), bd, "gelu"), bd, dy.to(cuda))
+    R.check(db, ref.db, "db")
