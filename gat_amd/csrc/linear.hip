@@ -12,11 +12,12 @@
 //    rounding to 16 bits, its own.
 //
 // What bounds it.  Layers of a few hundred columns are bound by memory for 16-bit types: [2449029, 256] x
-// [256, 256] bf16 with GELU and residual takes 1.23 ms forward (5.0 GB, 4.1 TB/s), 0.86 ms for dx (3.8 GB,
-// 4.4 TB/s) and 0.71 ms for dW (3.8 GB, 5.3 TB/s), where a copy runs at 4.9 TB/s.  Wide ones are bound by the
-// matrix cores: [65537, 1024] x [1024, 1001] f16 in 0.186 ms, 720 TFLOP/s.  f32 is between the two: [100000, 240] x
-// [240, 240] takes 0.142 ms forward, of which the matrix cores are busy for 0.031, the vector units (cutting the
-// operands, the activation) for 0.037, and 384 MB at the copy's rate are 0.078; dx 0.123, dW 0.104.
+// [256, 256] bf16 with GELU and residual takes 1.18 ms forward (5.0 GB, 4.3 TB/s), 0.85 ms for dx (3.8 GB,
+// 4.4 TB/s) and 0.71 ms for dW (3.8 GB, 5.3 TB/s), where a copy runs at 4.9 TB/s.  Wide ones are bound by what
+// feeds the matrix cores: [65537, 1024] x [1024, 1001] f16 in 0.182 ms, 740 TFLOP/s, with the matrix cores, LDS and
+// the vector units busy for a third of it each.  f32 is between the two: [100000, 240] x [240, 240] takes 0.140 ms
+// forward, of which the matrix cores are busy for 0.031, the vector units (cutting the operands, the activation)
+// for 0.037, and 384 MB at the copy's rate are 0.078; dx 0.122, dW 0.104.
 #include "attn_device.h"
 #include "common.h"
 #include "dense_device.h"
