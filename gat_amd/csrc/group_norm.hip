@@ -28,7 +28,7 @@ constexpr int kGnFwdBlocks = 4096, kGnBwdBlocks = 1024;
 // Blocks of the length > 1 form, over all samples: of the passes that leave sums (each block's are read again)
 // and of those that only apply.  Twelve blocks a CU for the sums: 158 -> 137 us for the backward's at
 // [3, 169343, 256] bf16 against six; the forward's does not care.
-constexpr int kGnChunks = 3072, kGnApply = 6144;
+constexpr int kGnChunks = 12 * 256, kGnApply = 24 * 256;
 constexpr int kGnJoin = 1024;      // most threads of a block that joins a group's chunks
 constexpr int kGnSamples = 65535;  // samples of one launch
 constexpr int kGnSlabs = 64;       // row slabs of the column sums
