@@ -142,3 +142,113 @@ def test_linear_gradient_of_the_bias_alone(cuda):
     bd = b.to(cuda).requires_grad_(True)
     (db,) = torch.autograd.grad(gat_amd.linear_act(x.to(cuda), w.to(cuda), bd, "gelu"), bd, dy.to(cuda))
     R.check(db, ref.db, "db")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_one_axis_and_empty_axes(cuda, dtype):
+    import gat_amd
+    g = torch.Generator().manual_seed(3)
+    x, w, b, dy = (torch.randn(*s, generator=g).to(dtype) for s in ((30,), (11, 30), (11,), (11,)))
+    ref = R.Linear(x[None], w, b, None, "silu", dy[None], dtype)
+    xd, wd = x.to(cuda).requires_grad_(True), w.to(cuda).requires_grad_(True)
+    y = gat_amd.linear_act(xd, wd, b.to(cuda), "silu")
+    y.backward(dy.to(cuda))
+    R.check(y[None], ref.y, "y")
+    R.check(xd.grad[None], ref.dx, "dx")
+    R.check(wd.grad, ref.dw, "dw")
+    e = torch.zeros(4, 0, 30, device=cuda, dtype=dtype, requires_grad=True)
+    z = gat_amd.linear_act(e, wd, b.to(cuda))
+    assert z.shape == (4, 0, 11)
+    ge, gw = torch.autograd.grad(z, (e, wd), torch.zeros_like(z))
+    assert ge.shape == e.shape and not gw.any()
+    d = gat_amd.dropout(x.to(cuda), 0.5, seed=4)
+    assert torch.equal(d, gat_amd.dropout(x.to(cuda)[None], 0.5, seed=4)[0])
+    for shape in ((3, 0), (0, 3), (2, 0, 5)):
+        assert gat_amd.dropout(torch.zeros(*shape, device=cuda, dtype=dtype), 0.5).shape == shape
+
+
+def test_an_operand_used_twice(cuda):
+    """x as its own residual, one weight in two products, weight and bias of a norm the same tensor"""
+    import gat_amd
+    g = torch.Generator().manual_seed(5)
+    x, w, v, dy = (torch.randn(*s, generator=g) for s in ((70, 24), (24, 24), (24,), (70, 24)))
+    xd, wd, vd = (t.to(cuda).requires_grad_(True) for t in (x, w, v))
+    h = gat_amd.linear_act(xd, wd, vd, "elu", xd)
+    y = gat_amd.group_norm_act(gat_amd.linear_act(h, wd, None, "none", h), 4, vd, vd)
+    got = torch.autograd.grad(y, (xd, wd, vd), dy.to(cuda))
+    X, W, V = (t.double().requires_grad_(True) for t in (x, w, v))
+    H = torch.nn.functional.elu(X @ W.t() + V) + X
+    H = H @ W.t() + H
+    Y = torch.nn.functional.group_norm(H, 4, V, V, 1e-5)
+    # four f32 operators in a row, sums of at most 70 x 24 terms: each a few dozen steps of its summands, under
+    # 100 U = 6e-6 of the largest value together
+    for a, r in zip(got, torch.autograd.grad(Y, (X, W, V), dy.double())):
+        assert float((a.cpu().double() - r).abs().max()) < 1e-5 * float(r.abs().max())
+
+
+def test_backward_twice_and_checkpointed(cuda):
+    """a retained graph gives the same gradients again; a checkpointed block draws the same mask again"""
+    import gat_amd
+    from torch.utils.checkpoint import checkpoint
+    x = torch.randn(300, 64, device=cuda, requires_grad=True)
+    w = torch.randn(64, 64, device=cuda, requires_grad=True)
+
+    def block(x, w):
+        return gat_amd.linear_act(gat_amd.dropout(x, 0.4), w, None, "gelu")
+
+    torch.manual_seed(8)
+    y = block(x, w)
+    dy = torch.randn_like(y)
+    first = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    again = torch.autograd.grad(y, (x, w), dy)
+    torch.manual_seed(8)
+    z = checkpoint(block, x, w, use_reentrant=False)
+    torch.manual_seed(9)
+    other = torch.autograd.grad(z, (x, w), dy)
+    assert torch.equal(y, z)
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(first, again, other))
+
+
+def test_changed_in_place_before_the_backward(cuda):
+    """what the backward needs is guarded as by torch's own operators"""
+    import gat_amd
+    x = torch.randn(40, 16, device=cuda)
+    w = torch.randn(8, 16, device=cuda, requires_grad=True)
+    y = gat_amd.linear_act(x, w)
+    x.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+
+
+def test_two_streams_at_once(cuda):
+    """long calls that overlap on two streams, each with workspaces of its own"""
+    import gat_amd
+    g = torch.Generator().manual_seed(6)
+    sets = []
+    for i in range(2):
+        x = torch.randn(60000, 200, generator=g).to(cuda).requires_grad_(True)
+        w = (torch.randn(96, 200, generator=g) / 14).to(cuda).requires_grad_(True)
+        ids = torch.randint(0, 5000, (60000,), generator=g).to(cuda)
+        t = torch.randn(5000, 96, generator=g).to(cuda).requires_grad_(True)
+        v = torch.randn(96, generator=g).to(cuda)
+        dy = torch.randn(60000, 96, generator=g).to(cuda)
+        sets.append((x, w, ids, t, v, dy))
+
+    def work(s):
+        x, w, ids, t, v, dy = s
+        y = gat_amd.linear_act(x, w, v, "silu", gat_amd.embedding(ids, t))
+        y = gat_amd.group_norm_act(y.view(6, 10000, 96), 3, v, v, act="elu").view(60000, 96)
+        return [y.detach(), *torch.autograd.grad(y, (x, w, t), dy)]
+
+    want = [work(s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for turn in range(3):
+        got = []
+        for s, st in zip(sets, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                got.append(work(s))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b)), turn
