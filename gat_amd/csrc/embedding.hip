@@ -200,6 +200,16 @@ template <int ITEMS> __global__ __launch_bounds__(256) void sort_scatter_kernel(
         pos[k] = e.y;
         digit[k] = (key[k] >> A.shift) & (bins - 1);
     }
+    // this thread's digits, at most two: their counts are on their way while the wave ranks its items
+    constexpr int kDigits = (1 << kSortMaxBits) / 256;
+    const int per = bins > 256 ? kDigits : 1, d0 = threadIdx.x * per;
+    uint32_t total[kDigits], before[kDigits];
+#pragma unroll
+    for (int q = 0; q < kDigits; ++q) {
+        const bool on = q < per && d0 + q < bins;
+        total[q] = on ? A.total[d0 + q] : 0u;
+        before[q] = on ? A.hist[(long long)(d0 + q) * A.blocks + blockIdx.x] : 0u;
+    }
     wave_ranks<ITEMS>(cnt + wave * bins, digit, have, A.bits, lane, rank);
     __syncthreads();
     // the tile's own order first, in LDS: neighbours in it go to neighbouring places, and the stores of a wave
@@ -207,19 +217,20 @@ template <int ITEMS> __global__ __launch_bounds__(256) void sort_scatter_kernel(
     uint2 *tile = reinterpret_cast<uint2 *>(smem + 5 * bins);
     uint32_t *shift = smem + 4 * bins;       // [bins]: a digit's place in the output less its place in the tile
     {
-        const int per = bins > 256 ? bins / 256 : 1, d0 = threadIdx.x * per;
         uint32_t mine = 0, all = 0;
-        for (int q = 0; q < per; ++q)
-            if (d0 + q < bins) {
+#pragma unroll
+        for (int q = 0; q < kDigits; ++q)
+            if (q < per && d0 + q < bins) {
                 for (int w = 0; w < 4; ++w) mine += cnt[w * bins + d0 + q];
-                all += A.total[d0 + q];
+                all += total[q];
             }
         uint32_t here = block_scan(mine, wsum), there = block_scan(all, wsum);
-        for (int q = 0; q < per; ++q) {
+#pragma unroll
+        for (int q = 0; q < kDigits; ++q) {
             const int d = d0 + q;
-            if (d >= bins) break;
-            shift[d] = there + A.hist[(long long)d * A.blocks + blockIdx.x] - here;
-            there += A.total[d];
+            if (q >= per || d >= bins) break;
+            shift[d] = there + before[q] - here;
+            there += total[q];
             for (int w = 0; w < 4; ++w) {
                 const uint32_t c = cnt[w * bins + d];
                 cnt[w * bins + d] = here;
