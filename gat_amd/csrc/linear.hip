@@ -8,8 +8,12 @@
 //    multiply rounds, at 16/6 of the f32 MFMA's rate.  A sum that comes out infinite or NaN (an operand
 //    was, or a piece rounded up to infinity next to the largest float) is taken again in plain f32.
 //  * act'(z) is written by the forward when a backward follows: f32 for f32 tensors, for 16-bit ones as a
-//    16-bit fixed-point number of step 2^-15 (0 and 1 are exact), so that dz = dy act'(z) carries one
-//    rounding to 16 bits, its own.
+//    16-bit fixed-point number of step 2^-15 (0 and 1 are exact).
+//  * dz = dy act'(z) of 16-bit tensors does not fit their type.  It enters the products as two numbers of it,
+//    dz = hi + lo, lo what hi's rounding left: a product more a step, and dx and dW are rounded once, as they
+//    are stored.  (One number: every dz off by up to half a step, and the error of dx and dW larger by sqrt 2.)
+//    ReLU's slopes are 0 and 1, dz is dy or nothing, and one number is enough.  An infinite or NaN factor on the
+//    other side would meet a zero lo or one of the other sign: see `redo`.
 //
 // What bounds it.  Layers of a few hundred columns are bound by memory for 16-bit types: [2449029, 256] x
 // [256, 256] bf16 with GELU and residual takes 1.18 ms forward (5.0 GB, 4.3 TB/s), 0.85 ms for dx (3.8 GB,
@@ -125,11 +129,43 @@ __device__ __forceinline__ void cut3(float a, float b, uint32_t &p0, uint32_t &p
     p2 = pack_bf16(a, b);
 }
 
+// the eight values of a granule in f32
+template <class T> __device__ __forceinline__ VecF<8> gran_values(const Gran<T> &g) {
+    VecF<8> v;
+    T e[8];
+    __builtin_memcpy(e, g.w, sizeof(e));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.e[i] = (float)e[i];
+    return v;
+}
+template <class T> __device__ __forceinline__ Gran<T> to_gran(const VecF<8> &v) {
+    Gran<T> g;
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = (T)v.e[i];
+    __builtin_memcpy(g.w, e, sizeof(e));
+    return g;
+}
+
+// v = hi + lo, both of the tensor's type.  hi stays finite, so that lo is v - hi for every v: infinite where v is
+// (v_med3), NaN where v is.
+template <class T> __device__ __forceinline__ void split2(const VecF<8> &v, Gran<T> &hi, Gran<T> &lo) {
+    const float top = std::is_same<T, f16_t>::value ? 65504.f : 3.3895313892515355e38f;
+    VecF<8> h, l;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h.e[i] = __builtin_amdgcn_fmed3f(v.e[i], -top, top);
+    hi = to_gran<T>(h);
+    h = gran_values<T>(hi);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) l.e[i] = v.e[i] - h.e[i];
+    lo = to_gran<T>(l);
+}
+
 // A tile of R rows x BK contraction elements in LDS, PIECES planes of 16-bit elements.  16-byte granules
 // are XOR-swizzled so that sixteen lanes reading one granule column of sixteen rows hit all 64 banks: rows of
 // 128 bytes lie in halves of the banks by their parity, rows of 64 bytes in quarters.
-template <class T, int R> struct Tile {
-    static constexpr int BK = Mul<T>::BK, G = BK / 8, P = Mul<T>::PIECES;
+template <class T, int R, int PIECES = Mul<T>::PIECES> struct Tile {
+    static constexpr int BK = Mul<T>::BK, G = BK / 8, P = PIECES;
     static constexpr int PLANE = R * BK * 2, BYTES = PLANE * P;
     static __device__ __forceinline__ int at(int row, int g) {
         const int s = G == 8 ? ((row >> 1) & 7) : ((row >> 2) & 3);
@@ -148,10 +184,19 @@ template <class T, int R> struct Tile {
                 *reinterpret_cast<u32x4 *>(lds + p * PLANE + at(row, g)) = u32x4{q[p][0], q[p][1], q[p][2], q[p][3]};
         }
     }
+    static __device__ __forceinline__ void put2(char *lds, int row, int g, const VecF<8> &v) {
+        static_assert(P == 2, "a tile of halves");
+        Gran<T> q[2];
+        split2<T>(v, q[0], q[1]);
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+            *reinterpret_cast<u32x4 *>(lds + p * PLANE + at(row, g)) = u32x4{q[p].w[0], q[p].w[1], q[p].w[2], q[p].w[3]};
+    }
     static __device__ __forceinline__ u32x4 frag(const char *lds, int p, int row, int g) {
         return *reinterpret_cast<const u32x4 *>(lds + p * PLANE + at(row, g));
     }
 };
+
 
 constexpr int kBM = 128;      // rows of dW's tiles
 
@@ -196,15 +241,6 @@ template <class T> __device__ __forceinline__ SlopeGran<T> ld_slope_short(const 
     __builtin_memcpy(s.w, e, sizeof(e));
     return s;
 }
-// the eight values of a granule in f32
-template <class T> __device__ __forceinline__ VecF<8> gran_values(const Gran<T> &g) {
-    VecF<8> v;
-    T e[8];
-    __builtin_memcpy(e, g.w, sizeof(e));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v.e[i] = (float)e[i];
-    return v;
-}
 template <class T> __device__ __forceinline__ VecF<8> with_slope(const Gran<T> &g, const SlopeGran<T> &s) {
     VecF<8> v = gran_values<T>(g);
     if constexpr (IsF32<T>::value) {
@@ -225,24 +261,22 @@ template <class T> __device__ __forceinline__ VecF<8> with_slope(const Gran<T> &
     }
     return v;
 }
-template <class T> __device__ __forceinline__ Gran<T> to_gran(const VecF<8> &v) {
-    Gran<T> g;
-    T e[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = (T)v.e[i];
-    __builtin_memcpy(g.w, e, sizeof(e));
-    return g;
+// one value of A as it enters the products, in f32
+template <class T> __device__ __forceinline__ float one_slope(const typename SlopeOf<T>::type s) {
+    if constexpr (IsF32<T>::value) return s;
+    else return s == 65535 ? __uint_as_float(0x7fc00000u) : fmaf((float)s, 1.0f / 32768.f, -0.25f);
 }
 
 // acc (32x32 blocks of a wave) += one contraction step of 16, all pieces
-template <class T, int MI, int NI>
-__device__ __forceinline__ void mma_pieces(const u32x4 (&a)[MI][Mul<T>::PIECES], const u32x4 (&b)[NI][Mul<T>::PIECES],
+template <class T, int PA, int MI, int NI>
+__device__ __forceinline__ void mma_pieces(const u32x4 (&a)[MI][PA], const u32x4 (&b)[NI][Mul<T>::PIECES],
                                            f32x16v (&acc)[MI][NI]) {
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
             if constexpr (Mul<T>::PIECES == 1) {
+                if constexpr (PA == 2) acc[i][j] = Mul<T>::mma(a[i][1], b[j][0], acc[i][j]);
                 acc[i][j] = Mul<T>::mma(a[i][0], b[j][0], acc[i][j]);
             } else {   // the small products first
                 acc[i][j] = Mul<T>::mma(a[i][0], b[j][2], acc[i][j]);
@@ -256,23 +290,22 @@ __device__ __forceinline__ void mma_pieces(const u32x4 (&a)[MI][Mul<T>::PIECES],
 }
 
 // acc += A-tile rows ra.. x B-tile rows rb..
-template <class T, int BM, int BN, int MI, int NI>
+template <class T, class TA, class TB, int MI, int NI>
 __device__ __forceinline__ void tile_mma(const char *la, const char *lb, int ra, int rb, int lane,
                                          f32x16v (&acc)[MI][NI]) {
-    typedef Tile<T, BM> TA;
-    typedef Tile<T, BN> TB;
     const int r = lane & 31, half = lane >> 5;
 #pragma unroll
     for (int s = 0; s < TA::BK / 16; ++s) {
-        u32x4 a[MI][TA::P], b[NI][TA::P];
+        u32x4 a[MI][TA::P], b[NI][TB::P];
 #pragma unroll
         for (int p = 0; p < TA::P; ++p) {
 #pragma unroll
             for (int i = 0; i < MI; ++i) a[i][p] = TA::frag(la, p, ra + i * 32 + r, 2 * s + half);
+            if (p >= TB::P) continue;
 #pragma unroll
             for (int j = 0; j < NI; ++j) b[j][p] = TB::frag(lb, p, rb + j * 32 + r, 2 * s + half);
         }
-        mma_pieces<T, MI, NI>(a, b, acc);
+        mma_pieces<T, TA::P, MI, NI>(a, b, acc);
     }
 }
 
@@ -329,16 +362,36 @@ __device__ __forceinline__ void epi_piece(const LinArgs &A, long long m, int n, 
     }
 }
 
-// the sum in plain f32, an element at a time: what the pieces cannot say (f32 only)
-template <bool FWD> __device__ __forceinline__ float plain_dot(const LinArgs &A, long long m, int n) {
-    const float *a = static_cast<const float *>(A.A) + m * A.K;
-    const float *sl = FWD || !A.aslope ? nullptr : static_cast<const float *>(A.aslope) + m * A.K;
-    const float *w = static_cast<const float *>(A.plain) + (FWD ? (long long)n * A.K : n);
+// the sum in plain f32, an element at a time: what the pieces cannot say
+template <class T, bool FWD> __device__ __forceinline__ float plain_dot(const LinArgs &A, long long m, int n) {
+    typedef typename SlopeOf<T>::type ST;
+    const T *a = static_cast<const T *>(A.A) + m * A.K;
+    const ST *sl = FWD || !A.aslope ? nullptr : static_cast<const ST *>(A.aslope) + m * A.K;
+    const T *w = static_cast<const T *>(A.plain) + (FWD ? (long long)n * A.K : n);
     const long long step = FWD ? 1 : A.N;
     float s = 0.f;
 #pragma unroll 1
-    for (int k = 0; k < A.K; ++k) s = fmaf(sl ? a[k] * sl[k] : a[k], w[k * step], s);
+    for (int k = 0; k < A.K; ++k) s = fmaf(sl ? (float)a[k] * one_slope<T>(sl[k]) : (float)a[k], (float)w[k * step], s);
     return s;
+}
+
+// Whether this block's sums need the plain ones after all, where dz is two numbers: some sum is not finite, and so
+// is some factor of the other side among `rows` rows (`stride` apart) of `cols` columns.  An infinity of dz alone
+// comes out right.
+template <class T, int MI, int NI>
+__device__ __forceinline__ bool redo(const f32x16v (&acc)[MI][NI], const T *b, long long rows, long long stride, int cols) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) s = fmaf(acc[i][j][q], 0.f, s);       // NaN once one is not finite
+    if (!__syncthreads_or(s != 0.f)) return false;
+    bool bad = false;
+    for (long long r = 0; r < rows; ++r)
+        for (int c = threadIdx.x; c < cols; c += blockDim.x) bad = bad || !(fabsf((float)b[r * stride + c]) < INFINITY);
+    return __syncthreads_or(bad);
 }
 
 // One block a tile, through registers into one LDS buffer: the next step's loads are on their way while this
@@ -352,10 +405,11 @@ template <bool FWD> __device__ __forceinline__ float plain_dot(const LinArgs &A,
 // part [splits][M][N], for lin_join_kernel.  WHOLE: K is a multiple of a step, and the last tile of rows starts
 // early instead of running over (M >= BM; what it shares with the tile before, that one stores): no address but
 // B's rows needs vector arithmetic in the loop, and nothing is dropped.  16-bit types gain 3 to 8% ([65536, 1024] x
-// [1024, 1024] bf16 206 -> 192 us); f32, busy with its cuts, loses 2.
-template <class T, int BM, int BN, int WM, int WN, bool FWD, bool CUT, bool SHORT, bool SHORT_N, bool PART, bool WHOLE>
+// [1024, 1024] bf16 206 -> 192 us); f32, busy with its cuts, loses 2.  TWO (16 bits, backward): dz as two numbers.
+template <class T, int BM, int BN, int WM, int WN, bool FWD, bool CUT, bool SHORT, bool SHORT_N, bool PART, bool WHOLE, bool TWO>
 __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void lin_nt_kernel(const LinArgs A) {
-    typedef Tile<T, BM> TA;
+    static_assert(!TWO || (!FWD && !IsF32<T>::value), "dz of 16-bit tensors");
+    typedef Tile<T, BM, TWO ? 2 : Mul<T>::PIECES> TA;
     typedef Tile<T, BN> TB;
     constexpr int THREADS = WM * WN * 64, MI = BM / WM / 32, NI = BN / WN / 32;
     constexpr int LD = NI * 32 + 4;
@@ -380,7 +434,7 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
     Gran<T> gb[CUT ? 1 : NB];
     u32x4 gc[CUT ? NB : 1][3];
     const int g = threadIdx.x % G, row = threadIdx.x / G;
-    const bool sloped = !FWD && A.aslope;
+    const bool sloped = TWO || (!FWD && A.aslope);
     // wave-uniform tile bases, 32-bit offsets from there (a tile spans at most 256 rows of 256 KB); rows behind
     // the matrix repeat its last one, their results are not stored
     const T *ba = static_cast<const T *>(A.A) + m0 * A.K;
@@ -461,12 +515,18 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
         const int k = k0 + g * 8, over = k > A.K - 8 ? k - (A.K - 8) : 0;
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
-            if (!FWD && sloped) ga[i] = to_gran<T>(with_slope<T>(ga[i], gs[i]));
-            if (end) {
-                if constexpr (CUT) shift_down<T>(ga[i].w, over);
-                else drop(ga[i], over);
+            if constexpr (TWO) {
+                if (end) drop(ga[i], over);
+                TA::put2(la, row + i * RP, g, with_slope<T>(ga[i], gs[i]));
+                continue;
+            } else {
+                if (!FWD && sloped) ga[i] = to_gran<T>(with_slope<T>(ga[i], gs[i]));
+                if (end) {
+                    if constexpr (CUT) shift_down<T>(ga[i].w, over);
+                    else drop(ga[i], over);
+                }
+                TA::put(la, row + i * RP, g, ga[i]);
             }
-            TA::put(la, row + i * RP, g, ga[i]);
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
@@ -482,7 +542,7 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
         }
         __syncthreads();
         if (k0 + TA::BK < k_end) fetch(k0 + TA::BK);
-        tile_mma<T, BM, BN, MI, NI>(la, lb, wm, wn, lane, acc);
+        tile_mma<T, TA, TB, MI, NI>(la, lb, wm, wn, lane, acc);
         __syncthreads();
     }
     if constexpr (PART) {
@@ -499,6 +559,9 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
                 }
         return;
     }
+    bool again = IsF32<T>::value;
+    if constexpr (TWO)
+        again = redo<T, MI, NI>(acc, reinterpret_cast<const T *>(bb), A.N - n0 < BN ? A.N - n0 : BN, A.ldb, A.K);
     // epilogue: a wave turns its blocks 16 rows at a time through LDS of its own into row pieces of 8
     float *le = reinterpret_cast<float *>(smem) + wave * 16 * LD;
     constexpr int PR = NI * 4, RI = 64 / PR;        // pieces a row, rows at once
@@ -545,7 +608,7 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
                 float v[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[k] = le[(p * RI + rr) * LD + c8 + k];
-                if constexpr (IsF32<T>::value) {        // see the head of this file
+                if (again) {        // see the head of this file
                     bool fine = true;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) fine = fine && fabsf(v[k]) < INFINITY;
@@ -553,7 +616,7 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
                         float *row = le + (p * RI + rr) * LD + c8;      // this lane's own eight
 #pragma unroll 1
                         for (int k = 0; k < 8; ++k)
-                            if (k < have && !(fabsf(row[k]) < INFINITY)) row[k] = plain_dot<FWD>(A, m, n + k);
+                            if (k < have && !(fabsf(row[k]) < INFINITY)) row[k] = plain_dot<T, FWD>(A, m, n + k);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) v[k] = row[k];
                     }
@@ -574,7 +637,7 @@ template <class T, bool FWD> __global__ __launch_bounds__(256) void lin_join_ker
     for (int q = 0; q < A.splits; ++q) v += A.part[q * size + at];
     const long long m = at / A.N;
     const int n = (int)(at - m * A.N);
-    if (IsF32<T>::value && !(fabsf(v) < INFINITY)) v = plain_dot<FWD>(A, m, n);
+    if ((IsF32<T>::value || (!FWD && A.aslope)) && !(fabsf(v) < INFINITY)) v = plain_dot<T, FWD>(A, m, n);
     if constexpr (FWD) {
         const float z = v + (A.bias ? (float)static_cast<const T *>(A.bias)[n] : 0.f);
         float d = 1.f;
@@ -590,8 +653,8 @@ template <class T, bool FWD> __global__ __launch_bounds__(256) void lin_join_ker
 // 4 steps x 16 channels, four channels each, and every lane comes back with one channel's four steps.  The
 // 64-byte pieces of a row change places by the row's last two bits, so that the four rows of a block lie in
 // different banks.  (Rows padded by 64 bytes do the same, but then two blocks of f32 tiles miss fitting a CU.)
-template <class T, int C> struct TileT {
-    static constexpr int BK = Mul<T>::BK, P = Mul<T>::PIECES;
+template <class T, int C, int PIECES = Mul<T>::PIECES> struct TileT {
+    static constexpr int BK = Mul<T>::BK, P = PIECES;
     static constexpr int STRIDE = C * 2, PLANE = BK * STRIDE, BYTES = PLANE * P;
     static __device__ __forceinline__ int at(int row, int col) { return row * STRIDE + ((col * 2) ^ ((row & 3) << 6)); }
     static __device__ __forceinline__ void put(char *lds, int row, int col, const Gran<T> &v) {
@@ -607,6 +670,14 @@ template <class T, int C> struct TileT {
             for (int p = 0; p < 3; ++p)
                 *reinterpret_cast<u32x4 *>(to + p * PLANE) = u32x4{q[p][0], q[p][1], q[p][2], q[p][3]};
         }
+    }
+    static __device__ __forceinline__ void put2(char *lds, int row, int col, const VecF<8> &v) {
+        static_assert(P == 2, "a tile of halves");
+        Gran<T> q[2];
+        split2<T>(v, q[0], q[1]);
+#pragma unroll
+        for (int p = 0; p < 2; ++p)
+            *reinterpret_cast<u32x4 *>(lds + p * PLANE + at(row, col)) = u32x4{q[p].w[0], q[p].w[1], q[p].w[2], q[p].w[3]};
     }
     // channels col0 .. col0 + 31, steps 16 s + 8 half .. + 7 of this lane's channel
     static __device__ __forceinline__ u32x4 frag(const char *lds, int p, int s, int col0, int lane) {
@@ -626,8 +697,9 @@ template <class T, int C> struct TileT {
 //
 // dW slabs: part[split][n][k] = sum over the split's rows of dz[m][n] x[m][k], dz = A (* aslope) [M, N],
 // x = B [M, K]; the blocks of the first column of tiles also leave dz's column sums.  SHORT: N or K < 8.
-template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void lin_tn_kernel(const LinArgs A) {
-    typedef TileT<T, kBM> TA;
+template <class T, int BN, bool SHORT, bool TWO> __global__ __launch_bounds__(2 * BN) void lin_tn_kernel(const LinArgs A) {
+    static_assert(!TWO || !IsF32<T>::value, "dz of 16-bit tensors");
+    typedef TileT<T, kBM, TWO ? 2 : Mul<T>::PIECES> TA;
     typedef TileT<T, BN> TB;
     constexpr int THREADS = 2 * BN, WN = BN / 64, GA = kBM / 8, GB = BN / 8;
     constexpr int RA = THREADS / GA, RB = THREADS / GB, NA = TA::BK / RA, NB = TA::BK / RB;
@@ -646,7 +718,7 @@ template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = (wave / WN) * 64, wn = (wave % WN) * 64;
     typedef typename SlopeOf<T>::type ST;
-    const bool sloped = A.aslope, sums = (A.dbpart || A.db) && k0 == 0;
+    const bool sloped = TWO || A.aslope, sums = (A.dbpart || A.db) && k0 == 0;
     // Two steps' pieces where the registers are there: while one is stored, the other is on its way.
     constexpr int SETS = !IsF32<T>::value && BN == 256 ? 2 : 1;
     Gran<T> ga_[SETS][NA], gb_[SETS][NB];
@@ -718,13 +790,17 @@ template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void
                 if (sums)
 #pragma unroll
                     for (int k = 0; k < 8; ++k) db.e[k] += v.e[k];     // before the rounding
+                if constexpr (TWO) {
+                    TA::put2(la, ta + i * RA, ja, v);
+                    continue;
+                }
                 ga[i] = to_gran<T>(v);
             } else if (sums) {
                 const VecF<8> v = gran_values<T>(ga[i]);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) db.e[k] += v.e[k];
             }
-            TA::put(la, ta + i * RA, ja, ga[i]);
+            if constexpr (!TWO) TA::put(la, ta + i * RA, ja, ga[i]);
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
@@ -736,15 +812,15 @@ template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void
         fetch(set, r + SETS * TA::BK);
 #pragma unroll
         for (int s = 0; s < TA::BK / 16; ++s) {
-            u32x4 a[2][TA::P], b[2][TA::P];
+            u32x4 a[2][TA::P], b[2][TB::P];
 #pragma unroll
             for (int p = 0; p < TA::P; ++p)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     a[i][p] = TA::frag(la, p, s, wm + i * 32, lane);
-                    b[i][p] = TB::frag(lb, p, s, wn + i * 32, lane);
+                    if (p < TB::P) b[i][p < TB::P ? p : 0] = TB::frag(lb, p, s, wn + i * 32, lane);
                 }
-            mma_pieces<T, 2, 2>(a, b, acc);
+            mma_pieces<T, TA::P, 2, 2>(a, b, acc);
         }
         __syncthreads();
     };
@@ -771,6 +847,8 @@ template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void
             else A.dbpart[split * A.N + n0 + threadIdx.x] = s;
         }
     }
+    bool again = IsF32<T>::value;
+    if constexpr (TWO) again = redo<T, 2, 2>(acc, pb + r0 * A.K + k0, r1 - r0, A.K, A.K - k0 < BN ? A.K - k0 : BN);
     float *part = A.part + split * (long long)A.N * A.K;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -781,11 +859,11 @@ template <class T, int BN, bool SHORT> __global__ __launch_bounds__(2 * BN) void
                 const int n = n0 + wm + i * 32 + acc_row(q, lane >> 5), k = k0 + wn + j * 32 + (lane & 31);
                 if (n >= A.N || k >= A.K) continue;
                 float v = acc[i][j][q];
-                if (IsF32<T>::value && !(fabsf(v) < INFINITY)) {
+                if (again && !(fabsf(v) < INFINITY)) {
                     v = 0.f;
                     for (long long m = r0; m < r1; ++m) {
                         float d = (float)pa[m * A.N + n];
-                        if (sloped) d *= static_cast<const float *>(A.aslope)[m * A.N + n];
+                        if (sloped) d *= one_slope<T>(static_cast<const ST *>(A.aslope)[m * A.N + n]);
                         v = fmaf(d, (float)pb[m * A.K + k], v);
                     }
                 }
@@ -953,6 +1031,10 @@ static long long lin_dw_tiles(const gatmi_linear *l, bool wide) {
     const int bn = wide ? 256 : 128;
     return ((l->out_features + kBM - 1ll) / kBM) * ((l->in_features + bn - 1ll) / bn);
 }
+// dz as two numbers: where it does not fit the tensors' type
+static bool lin_two(const gatmi_linear *l) {
+    return l->dtype != GATMI_F32 && l->act != GATMI_ACT_NONE && l->act != GATMI_ACT_RELU;
+}
 
 static LinGeom lin_geom(const gatmi_linear *l) {
     LinGeom G;
@@ -995,7 +1077,7 @@ static LinGeom lin_geom(const gatmi_linear *l) {
     return G;
 }
 
-template <class T, int BM, int BN, int WM, int WN, bool FWD, bool CUT, bool SHORT = false, bool SHORT_N = false,
+template <class T, bool TWO, int BM, int BN, int WM, int WN, bool FWD, bool CUT, bool SHORT = false, bool SHORT_N = false,
           bool WHOLE = false>
 static void lin_go(LinArgs &A, hipStream_t st) {
     typedef typename SlopeOf<T>::type ST;
@@ -1014,32 +1096,41 @@ static void lin_go(LinArgs &A, hipStream_t st) {
         S.slope = move(A.slope, m * A.N * sizeof(ST));
         S.tiles = (S.M + BM - 1) / BM * S.tiles_n;
         const unsigned grid = (unsigned)((S.tiles + 7) / 8 * 8);
-        hipLaunchKernelGGL((lin_nt_kernel<T, BM, BN, WM, WN, FWD, CUT, SHORT, SHORT_N, false, WHOLE>), dim3(grid), dim3(WM * WN * 64), 0,
+        hipLaunchKernelGGL((lin_nt_kernel<T, BM, BN, WM, WN, FWD, CUT, SHORT, SHORT_N, false, WHOLE, TWO>), dim3(grid), dim3(WM * WN * 64), 0,
                            st, S);
     }
 }
 // The tile.  While 128 x 128 ones would be fewer than two a CU, 64 x 64: a lone block of the large ones waits
 // for itself ([4096, 64] x [64, 1024] f32 24.7 -> 16.7 us, bf16 11.1 -> 8.1; with 3 a CU [8192, 1024] x
-// [1024, 1024] f32 loses, 117 -> 134).  Narrow results take narrow tiles, 128 x 32 from one a CU on.
-template <class T, bool FWD, bool CUT> static void lin_launch_nt(LinArgs A, const LinSplitK &S, hipStream_t st) {
+// [1024, 1024] f32 loses, 117 -> 134).  Narrow results take narrow tiles, 128 x 32 from one a CU on.  Where dz is two
+// numbers a 128 x 128 tile's 48 KB of LDS and 184 registers leave two blocks a CU; half the rows leave three or four, and
+// up to 256 columns a tile make dz once: dx of [2449029, 256] x [256, 256] bf16 1.36 -> 1.02 ms, to 128 columns 0.77 -> 0.69.
+template <class T, bool FWD, bool CUT, bool TWO> static void lin_launch_nt(LinArgs A, const LinSplitK &S, hipStream_t st) {
     if (S.splits > 1) {
         A.splits = S.splits;
         A.k_split = S.k_split;
         A.tiles_n = (A.N + 63) / 64;
         A.tiles = (A.M + 63) / 64 * A.tiles_n;
         const unsigned grid = (unsigned)((A.tiles * A.splits + 7) / 8 * 8);
-        hipLaunchKernelGGL((lin_nt_kernel<T, 64, 64, 2, 2, FWD, CUT, false, false, true, false>), dim3(grid), dim3(256), 0, st, A);
+        hipLaunchKernelGGL((lin_nt_kernel<T, 64, 64, 2, 2, FWD, CUT, false, false, true, false, TWO>), dim3(grid), dim3(256), 0, st, A);
         hipLaunchKernelGGL((lin_join_kernel<T, FWD>), dim3((unsigned)((A.M * A.N + 255) / 256)), dim3(256), 0, st, A);
         return;
     }
     const long long big = (A.M + 127) / 128 * ((A.N + 127) / 128);
-    if (A.K < 8) lin_go<T, 64, 64, 2, 2, FWD, CUT, true, true>(A, st);
-    else if (A.N < 8) lin_go<T, 128, 32, 4, 1, FWD, CUT, false, true>(A, st);
-    else if (A.N <= 32 && big >= device_cus()) lin_go<T, 128, 32, 4, 1, FWD, CUT>(A, st);
-    else if (big < 2 * device_cus()) lin_go<T, 64, 64, 2, 2, FWD, CUT>(A, st);
-    else if (A.N <= 64) lin_go<T, 128, 64, 4, 1, FWD, CUT>(A, st);
-    else if (!IsF32<T>::value && A.K % Mul<T>::BK == 0 && A.M >= 128) lin_go<T, 128, 128, 2, 2, FWD, CUT, false, false, true>(A, st);
-    else lin_go<T, 128, 128, 2, 2, FWD, CUT>(A, st);
+    if (A.K < 8) lin_go<T, TWO, 64, 64, 2, 2, FWD, CUT, true, true>(A, st);
+    else if (A.N < 8) lin_go<T, TWO, 128, 32, 4, 1, FWD, CUT, false, true>(A, st);
+    else if (A.N <= 32 && big >= device_cus()) lin_go<T, TWO, 128, 32, 4, 1, FWD, CUT>(A, st);
+    else if (big < 2 * device_cus()) lin_go<T, TWO, 64, 64, 2, 2, FWD, CUT>(A, st);
+    else if (A.N <= 64) lin_go<T, TWO, 128, 64, 4, 1, FWD, CUT>(A, st);
+    else {
+        const bool whole = !IsF32<T>::value && A.K % Mul<T>::BK == 0 && A.M >= 128;
+        if constexpr (TWO) {
+            if (A.N <= 128) whole ? lin_go<T, TWO, 64, 128, 2, 2, FWD, CUT, false, false, true>(A, st) : lin_go<T, TWO, 64, 128, 2, 2, FWD, CUT>(A, st);
+            else whole ? lin_go<T, TWO, 64, 256, 1, 4, FWD, CUT, false, false, true>(A, st) : lin_go<T, TWO, 64, 256, 1, 4, FWD, CUT>(A, st);
+        } else {
+            whole ? lin_go<T, TWO, 128, 128, 2, 2, FWD, CUT, false, false, true>(A, st) : lin_go<T, TWO, 128, 128, 2, 2, FWD, CUT>(A, st);
+        }
+    }
 }
 
 }  // namespace gatmi
@@ -1090,9 +1181,9 @@ extern "C" int gatmi_linear_fwd(const gatmi_linear *l, const void *x, const void
                            static_cast<const float *>(weight), A.N, A.K, G.ldf, ws);
         A.B = ws;
         A.ldb = G.ldf;
-        lin_launch_nt<float, true, true>(A, G.fwd, st);
+        lin_launch_nt<float, true, true, false>(A, G.fwd, st);
     } else {
-        GATMI_WITH_TYPE(l->dtype, (lin_launch_nt<T, true, false>(A, G.fwd, st)));
+        GATMI_WITH_TYPE(l->dtype, (lin_launch_nt<T, true, false, false>(A, G.fwd, st)));
     }
     GATMI_HIP(hipGetLastError());
     return GATMI_OK;
@@ -1125,6 +1216,7 @@ extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void
     A.A = grad_y;
     A.aslope = l->act == GATMI_ACT_NONE ? nullptr : slope;
     A.M = l->rows;
+    const bool two = lin_two(l);
     if (grad_x && l->rows > 0) {
         ProfScope ps("linear_dx", st);
         A.plain = weight;
@@ -1137,7 +1229,9 @@ extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void
         GATMI_WITH_TYPE(l->dtype, {
             hipLaunchKernelGGL((lin_image_kernel<T, true>), dim3((G.ldb + 31) / 32, (K + 31) / 32), dim3(256), 0, st,
                                static_cast<const T *>(weight), N, K, G.ldb, ws);
-            lin_launch_nt<T, false, IsF32<T>::value>(A, G.dx, st);
+            constexpr bool cut = IsF32<T>::value;
+            if (two) lin_launch_nt<T, false, cut, !cut>(A, G.dx, st);
+            else lin_launch_nt<T, false, cut, false>(A, G.dx, st);
         });
         GATMI_HIP(hipGetLastError());
     }
@@ -1159,8 +1253,12 @@ extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void
             // (without dW the first column of tiles does: its blocks leave the column sums)
             A.tiles_n = grad_weight ? (K + (wide ? 255 : 127)) / (wide ? 256 : 128) : 1;
             A.tiles = grad_weight ? lin_dw_tiles(l, wide) : (N + kBM - 1) / kBM;
-            auto tn = N < 8 || K < 8 ? (wide ? lin_tn_kernel<T, 256, true> : lin_tn_kernel<T, 128, true>)
-                                     : (wide ? lin_tn_kernel<T, 256, false> : lin_tn_kernel<T, 128, false>);
+            auto pick = [&](auto t) {
+                constexpr bool b = decltype(t)::value;
+                return N < 8 || K < 8 ? (wide ? lin_tn_kernel<T, 256, true, b> : lin_tn_kernel<T, 128, true, b>)
+                                      : (wide ? lin_tn_kernel<T, 256, false, b> : lin_tn_kernel<T, 128, false, b>);
+            };
+            auto tn = two ? pick(std::integral_constant<bool, !IsF32<T>::value>{}) : pick(std::false_type{});
             hipLaunchKernelGGL(tn, dim3((unsigned)((A.tiles * G.splits + 7) / 8 * 8)), dim3(wide ? 512 : 256), 0, st, A);
             const long long size = (long long)N * K;
             const int dw_blocks = grad_weight ? (int)((size + 63) / 64) : 0, db_blocks = grad_bias ? (N + 7) / 8 : 0;

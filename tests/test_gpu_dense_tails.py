@@ -1,0 +1,110 @@
+"""The dense operators on the GPU where single roundings and saturated units show: every result here is ONE term (or
+one function value), so that no averaging over a sum hides what was lost on the way.  Bounds are relative
+(tests/dense_tails.py)."""
+import pytest
+import torch
+
+import dense_tails as T
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def uniform(shape, dtype, lo, hi, seed, scale=1.0):
+    """values in [lo, hi), and an upstream gradient"""
+    g = torch.Generator().manual_seed(seed)
+    return (torch.rand(*shape, generator=g) * (hi - lo) + lo).to(dtype), (torch.randn(*shape, generator=g) * scale).to(dtype)
+
+
+def pieces(dz, dtype):
+    """dz of a 16-bit tensor enters the products as two numbers of its type, the second what the first one's rounding
+    left: half a step of a half step, and f16's own smallest step"""
+    return T.u(dtype) ** 2 * dz.abs() + (2.0 ** -25 if dtype == F16 else 0.0)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("act", ["elu", "silu", "gelu"])
+@pytest.mark.parametrize("m,n", [(3, 64), (40, 64), (333, 72), (2500, 40), (40, 5), (700, 1200), (66000, 128)])
+def test_linear_dx_is_rounded_once(cuda, dtype, act, m, n):
+    """W = 1.7 on the diagonal: dx is one product, dy act'(z) W, of which only the result may be rounded to the type"""
+    import gat_amd
+    x, dy = uniform((m, n), dtype, -0.3, 1.2, m + n)
+    w = (torch.eye(n) * 1.7).to(dtype)
+    z = x.double() * float(w[0, 0])              # exact in f32 too: 8 by 8 or 11 by 11 bits
+    _, d, _, size = T.act(z, act)
+    dz = dy.double() * d
+    edz = dy.double().abs() * (T.own(z, dtype) * size + T.coding(d, dtype)) * 1.01 + pieces(dz, dtype) + 4 * T.U * dz.abs()
+    dx = dz * float(w[0, 0])
+    xd = x.to(cuda).requires_grad_(True)
+    y = gat_amd.linear_act(xd, w.to(cuda), act=act)
+    (gx,) = torch.autograd.grad(y, xd, dy.to(cuda))
+    T.within(gx, dx, edz * 1.75 + T.u(dtype) * dx.abs(), "dx")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("act", ["elu", "silu", "gelu"])
+@pytest.mark.parametrize("m,k,n", [(64, 40, 64), (333, 72, 30), (2500, 300, 140), (50, 5, 40), (50, 40, 3)])
+def test_linear_dw_is_rounded_once(cuda, dtype, act, m, k, n):
+    """W = 0, so z is the bias; one row of x for each of its columns: dW is one product, dy act'(z) x"""
+    import gat_amd
+    b, _ = uniform((n,), dtype, -0.3, 1.9, n)
+    v, dy = uniform((k, n), dtype, 0.6, 1.9, k)
+    dy = torch.cat([dy, torch.ones(m, n).to(dtype)])[:m]
+    x = torch.zeros(m, k, dtype=dtype)
+    x[torch.arange(min(k, m)), torch.arange(min(k, m))] = v[: min(k, m), 0]
+    z = b.double().expand(m, n)
+    _, d, _, size = T.act(z, act)
+    dz = dy.double() * d
+    edz = dy.double().abs() * (T.own(z, dtype) * size + T.coding(d, dtype)) * 1.01 + pieces(dz, dtype) + 4 * T.U * dz.abs()
+    wd = torch.zeros(n, k, dtype=dtype, device=cuda, requires_grad=True)
+    y = gat_amd.linear_act(x.to(cuda), wd, b.to(cuda), act)
+    (gw,) = torch.autograd.grad(y, wd, dy.to(cuda))
+    X = x.double()
+    dw = dz.t() @ X
+    T.within(gw, dw, edz.t() @ X + T.u(dtype) * dw.abs(), "dw")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("m,k,n", [(40, 50, 70), (2500, 140, 90), (64, 40, 1200), (30, 5, 6), (66000, 64, 72), (33000, 256, 64)])
+def test_linear_gradients_not_finite(cuda, dtype, m, k, n):
+    """an infinity or NaN in x, W or dy gives what the formula gives, where dz is two numbers as elsewhere: the same
+    infinities and NaN, and every other value as if they were not there"""
+    import gat_amd
+    g = torch.Generator().manual_seed(m + n)
+    base = [torch.randn(m, k, generator=g).to(dtype), (torch.randn(n, k, generator=g) / k ** 0.5).to(dtype),
+            torch.randn(m, n, generator=g).to(dtype)]
+    inf = float("inf")
+    for which, at, value in ((0, (3, 4), inf), (1, (5, 2), -inf), (2, (9, 1), inf), (2, (7, 0), float("nan")),
+                             (0, (m - 1, k - 1), float("nan")), (1, (n - 1, k - 1), inf)):
+        x, w, dy = (t.clone() for t in base)
+        (x, w, dy)[which][at] = value
+        xd, wd = x.to(cuda).requires_grad_(True), w.to(cuda).requires_grad_(True)
+        y = gat_amd.linear_act(xd, wd, act="elu")
+        got = torch.autograd.grad(y, (xd, wd), dy.to(cuda))
+        X, W, D = x.to(cuda).double(), w.to(cuda).double(), dy.to(cuda).double()
+        dz = D * T.act(X @ W.t(), "elu")[1]
+        for have, want in zip(got, (dz @ W, dz.t() @ X)):
+            have = have.double()
+            assert torch.equal(torch.isnan(have), torch.isnan(want)), (which, at)
+            assert torch.equal(have[torch.isinf(want)], want[torch.isinf(want)]), (which, at)
+            fine = torch.isfinite(want)
+            # (no more than: nothing else was touched)
+            if bool(fine.any()):
+                assert float((have - want)[fine].abs().max()) <= 2e-2 * float(want[fine].abs().max()), (which, at)
+
+
+def test_linear_gradient_past_the_range_of_f16(cuda):
+    """dz = dy act'(z) may be larger than any f16 where dx is not: GELU's slope goes up to 1.129"""
+    import gat_amd
+    for m in (40, 3):
+        x = torch.full((m, 64), 1.5, dtype=F16)
+        w = torch.eye(64, dtype=F16) * 0.25
+        dy = torch.full((m, 64), 65504.0, dtype=F16)
+        dy[1] *= -1
+        b = torch.full((64,), 1.0, dtype=F16)
+        xd = x.to(cuda).requires_grad_(True)
+        y = gat_amd.linear_act(xd, w.to(cuda), b.to(cuda), act="gelu")
+        (gx,) = torch.autograd.grad(y, xd, dy.to(cuda))
+        dx = dy.double() * T.act(x.double() * 0.25 + 1.0, "gelu")[1] * 0.25
+        assert float(dx.abs().min()) * 4 > 65520
+        T.within(gx, dx, dx.abs() * (T.u(F16) + 2.0 ** -11), "dx")
