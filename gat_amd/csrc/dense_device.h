@@ -74,8 +74,15 @@ template <bool EXACT> __device__ __forceinline__ float act_exp(float v) {
     return __builtin_amdgcn_exp2f(v * 1.44269502162933349609375f);
 }
 
-// exp(z) - 1 for z <= 0
-template <bool EXACT> __device__ __forceinline__ float act_expm1(float z) {
+// exp(z) for z <= 0, to a few of its own steps however small it is; NaN for NaN
+template <bool EXACT> __device__ __forceinline__ float act_exp_neg(float z) {
+    const float e = act_exp<false>(z);
+    if constexpr (EXACT) return z >= -87.0f ? exp_fast(z) : e;      // (exp_fast stops at -87)
+    return e;
+}
+
+// exp(z) - 1 for z <= 0, from exp(z)
+template <bool EXACT> __device__ __forceinline__ float act_expm1(float z, float e) {
     if constexpr (EXACT) {
         // above -0.35 the series to z^8 / 8! (what follows is below 2^-30 of the sum); below it exp(z) <= 0.705
         // and the subtraction leaves an error of exp's own 1.5 steps of at most 2^-24 against 0.295 or more
@@ -86,12 +93,11 @@ template <bool EXACT> __device__ __forceinline__ float act_expm1(float z) {
         s = fmaf(z, s, 1.6666667e-1f);
         s = fmaf(z, s, 0.5f);
         s = fmaf(z * z, s, z);
-        return z < -0.35f ? exp_fast(z) - 1.0f : s;      // NaN: s
+        return z < -0.35f ? e - 1.0f : s;      // NaN: s
     }
-    // next to 0 the subtraction would cancel: z + z^2/2 + z^3/6, off by z^3/24 relative (< 2^-20 there)
-    const float e = act_exp<false>(z) - 1.0f;
+    // next to 0 the subtraction would cancel: z + z^2/2 + z^3/6, off by z^3/24 relative, 2^-19.7 at -0.03
     const float s = z * fmaf(z, fmaf(z, 0.16666667f, 0.5f), 1.0f);
-    return z < -0.03f ? e : s;
+    return z < -0.03f ? e - 1.0f : s;
 }
 
 // The normal distribution function.  16-bit results: 1 - t(a1 + .. + a5 t^4) exp(-z^2/2) with
@@ -115,7 +121,7 @@ template <bool EXACT> __device__ __forceinline__ float act_phi(float z, float &g
 
 template <int ACT, bool EXACT> __device__ __forceinline__ float act_value(float z) {
     if constexpr (ACT == GATMI_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
-    if constexpr (ACT == GATMI_ACT_ELU) return z > 0.f ? z : act_expm1<EXACT>(z);
+    if constexpr (ACT == GATMI_ACT_ELU) return z > 0.f ? z : act_expm1<EXACT>(z, act_exp_neg<EXACT>(z));
     if constexpr (ACT == GATMI_ACT_SILU) {
         const float d = 1.0f + act_exp<EXACT>(-z);   // +inf for z far below 0: the quotient is -0
         return EXACT ? z / d : z * __builtin_amdgcn_rcpf(d);
@@ -134,9 +140,9 @@ template <int ACT, bool EXACT> __device__ __forceinline__ float act_both(float z
         return z > 0.f ? z : (z != z ? z : 0.f);
     }
     if constexpr (ACT == GATMI_ACT_ELU) {
-        const float e = act_expm1<EXACT>(z);
-        d = z > 0.f ? 1.f : e + 1.f;      // exp(z), to a step of 1
-        return z > 0.f ? z : e;
+        const float e = act_exp_neg<EXACT>(z);
+        d = z > 0.f ? 1.f : e;            // not (exp(z) - 1) + 1, which is good to a step of 1 only
+        return z > 0.f ? z : act_expm1<EXACT>(z, e);
     }
     if constexpr (ACT == GATMI_ACT_SILU) {
         const float q = 1.0f + act_exp<EXACT>(-z);

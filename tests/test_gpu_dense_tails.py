@@ -108,3 +108,46 @@ def test_linear_gradient_past_the_range_of_f16(cuda):
         dx = dy.double() * T.act(x.double() * 0.25 + 1.0, "gelu")[1] * 0.25
         assert float(dx.abs().min()) * 4 > 65520
         T.within(gx, dx, dx.abs() * (T.u(F16) + 2.0 ** -11), "dx")
+
+
+def gradient_of_saturated_units(cuda, dtype, act, m, n, lo=-12.0, hi=-4.0):
+    """W = 1: z = x and dx = dy act'(x), to the type's precision whether z is -4 or -12.  (f16: dy of a size at which
+    these gradients are normal numbers.)"""
+    import gat_amd
+    x, dy = uniform((m, n), dtype, lo, hi, m + n, 1024.0 if dtype == F16 else 1.0)
+    z = x.double()
+    _, d, _, size = T.act(z, act)
+    dx = dy.double() * d
+    edz = dy.double().abs() * (T.own(z, dtype) * size + T.coding(d, dtype)) * 1.01 + 4 * T.U * dx.abs()
+    # f32: three bf16 pieces of dz, of which the last is rounded to a multiple of bf16's smallest number, 2^-133, at
+    # the coarsest: half of that, times W = 1
+    edz = edz + (2.0 ** -134 if dtype == F32 else pieces(dx, dtype))
+    xd = x.to(cuda).requires_grad_(True)
+    y = gat_amd.linear_act(xd, torch.eye(n, dtype=dtype, device=cuda), act=act)
+    (gx,) = torch.autograd.grad(y, xd, dy.to(cuda))
+    T.within(gx, dx, edz + T.u(dtype) * dx.abs(), "dx")
+
+
+SIZES = [(3, 64), (40, 64), (333, 72), (2500, 40), (40, 5), (66000, 128)]
+
+
+@pytest.mark.parametrize("m,n", SIZES)
+def test_elu_slope_of_saturated_units_f32(cuda, m, n):
+    gradient_of_saturated_units(cuda, F32, "elu", m, n)
+    gradient_of_saturated_units(cuda, F32, "elu", m, n, -80.0, -10.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_elu_slope_of_saturated_units_group_norm(cuda, dtype):
+    """one sample, weight 1 and bias far below 0: the bias's gradient is dy act'(z), one term"""
+    import gat_amd
+    for shape in ((1, 64), (1, 1, 64)):
+        b, dy = uniform((64,), dtype, -12.0, -6.0, 3, 1024.0 if dtype == F16 else 1.0)
+        bd = b.to(cuda).requires_grad_(True)
+        w = torch.zeros(64, dtype=dtype, device=cuda)          # z = bias, exactly
+        x = torch.randn(*shape, generator=torch.Generator().manual_seed(1)).to(dtype).to(cuda)
+        y = gat_amd.group_norm_act(x, 4, w, bd, act="elu")
+        (gb,) = torch.autograd.grad(y, bd, dy.to(cuda).view(shape))
+        _, d, _, size = T.act(b.double(), "elu")
+        want = dy.double() * d
+        T.within(gb, want, dy.double().abs() * T.own(b.double(), dtype) * size + (T.u(dtype) + 4 * T.U) * want.abs(), "db")
