@@ -14,12 +14,10 @@ namespace gatmi {
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 
-// V elements as one access.  The address only needs the element's own alignment: rows of odd widths and
-// sliced tensors start anywhere, and a global load or store of up to 16 bytes takes that as it is.
-template <class T, int V> struct __attribute__((packed, aligned(sizeof(T)))) RawVec { T e[V]; };
-
 template <int V> struct VecF { float e[V]; };
 
+// V elements as one access.  The address only needs the element's own alignment: rows of odd widths and
+// sliced tensors start anywhere, and a global load or store of up to 16 bytes takes that as it is.
 template <class T, int V> __device__ __forceinline__ VecF<V> ldv(const T *p) {
     typedef T vec __attribute__((ext_vector_type(V)));
     typedef vec uvec __attribute__((aligned(sizeof(T))));
@@ -67,8 +65,8 @@ __device__ __forceinline__ uint32_t fdiv(const FastDiv &f, uint32_t n) {
 }
 
 // ---- activations: value and derivative at z, f32.  EXACT: the library's expm1 / exp / erf, for f32
-// tensors.  Otherwise (results are rounded to 16 bits) v_exp_f32 forms, whose error of a few 2^-22 is a
-// hundredth of that rounding.
+// tensors.  Otherwise (results are rounded to 16 bits) v_exp_f32 and v_rcp_f32 forms, whose error of at most
+// 2^-17 of the value is small beside that rounding (2^-11 for f16, 2^-8 for bf16), where the value itself is small too.
 template <bool EXACT> __device__ __forceinline__ float act_exp(float v) {
     if constexpr (EXACT) return expf(v);   // of either sign
     return __builtin_amdgcn_exp2f(v * 1.44269502162933349609375f);
@@ -100,22 +98,25 @@ template <bool EXACT> __device__ __forceinline__ float act_expm1(float z, float 
     return z < -0.03f ? e - 1.0f : s;
 }
 
-// The normal distribution function.  16-bit results: 1 - t(a1 + .. + a5 t^4) exp(-z^2/2) with
-// t = 1 / (1 + p |z| / sqrt 2) (Abramowitz and Stegun 7.1.26, absolute error 1.5e-7 of erf); the
-// lower tail is taken from the product itself, not from a difference.  `gauss` = exp(-z^2/2).
+// The normal distribution function, its lower tail relative to itself: from erfc, not as 1 + erf, which is nothing
+// where erf rounds to -1 and has lost half its digits by z = -3.  16-bit results: exp(-z^2/2) times a polynomial in
+// t = 1 / (1 + p |z|), fitted to erfc(a) exp(a^2) / 2 (a = |z| / sqrt 2, up to 10) for the smallest relative error,
+// which is 2^-17.9; v_exp adds z^2 2^-24 of its argument's rounding.  `gauss` = exp(-z^2/2).
 template <bool EXACT> __device__ __forceinline__ float act_phi(float z, float &gauss) {
+    float tail;
     if constexpr (EXACT) {
         gauss = expf(-0.5f * z * z);
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f));
+        tail = 0.5f * erfcf(fabsf(z) * 0.70710678118654752f);
+    } else {
+        gauss = act_exp<false>(-0.5f * z * z);
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.308308125f, fabsf(z), 1.0f));
+        float q = fmaf(t, -0.07528124f, 0.188420862f);
+        q = fmaf(t, q, 0.00836186484f);
+        q = fmaf(t, q, 0.136160269f);
+        q = fmaf(t, q, 0.119097903f);
+        q = fmaf(t, q, 0.123238377f);
+        tail = q * t * gauss;
     }
-    gauss = act_exp<false>(-0.5f * z * z);
-    const float a = fabsf(z) * 0.70710678118654752f;
-    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, a, 1.0f));
-    float q = fmaf(t, 1.061405429f, -1.453152027f);
-    q = fmaf(t, q, 1.421413741f);
-    q = fmaf(t, q, -0.284496736f);
-    q = fmaf(t, q, 0.254829592f);
-    const float tail = 0.5f * q * t * gauss;
     return z > 0.f ? 1.0f - tail : tail;
 }
 

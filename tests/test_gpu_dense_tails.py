@@ -151,3 +151,21 @@ def test_elu_slope_of_saturated_units_group_norm(cuda, dtype):
         _, d, _, size = T.act(b.double(), "elu")
         want = dy.double() * d
         T.within(gb, want, dy.double().abs() * T.own(b.double(), dtype) * size + (T.u(dtype) + 4 * T.U) * want.abs(), "db")
+
+
+@pytest.mark.parametrize("dtype,lo", [(F32, -12.0), (BF16, -12.0), (F16, -5.5)])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("m,n", SIZES)
+def test_values_of_saturated_units(cuda, dtype, lo, act, m, n):
+    """W = 1: y = act(x) where it is small itself"""
+    import gat_amd
+    x, _ = uniform((m, n), dtype, lo, -0.5, m + n)
+    a, _, size, _ = T.act(x.double(), act)
+    y = gat_amd.linear_act(x.to(cuda), torch.eye(n, dtype=dtype, device=cuda), act=act)
+    T.within(y, a, T.own(x.double(), dtype) * size + T.u(dtype) * a.abs(), "y")
+
+
+@pytest.mark.parametrize("m,n", SIZES)
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_slope_of_saturated_units_f32(cuda, act, m, n):
+    gradient_of_saturated_units(cuda, F32, act, m, n)
