@@ -7,8 +7,8 @@
 //    six products p_i q_j with i + j <= 2: what is left out is 2^-25 of a product, less than an f32
 //    multiply rounds, at 16/6 of the f32 MFMA's rate.  A sum that comes out infinite or NaN (an operand
 //    was, or a piece rounded up to infinity next to the largest float) is taken again in plain f32.
-//  * act'(z) is written by the forward when a backward follows: f32 for f32 tensors, for 16-bit ones as a
-//    16-bit fixed-point number of step 2^-15 (0 and 1 are exact).
+//  * act'(z) is written by the forward when a backward follows: f32 for f32 tensors, for 16-bit ones in 16 bits, to
+//    2^-16 and, where a unit is saturated and the slope small, to 2^-11 of itself (see pack_slope).
 //  * dz = dy act'(z) of 16-bit tensors does not fit their type.  It enters the products as two numbers of it,
 //    dz = hi + lo, lo what hi's rounding left: a product more a step, and dx and dW are rounded once, as they
 //    are stored.  (One number: every dz off by up to half a step, and the error of dx and dW larger by sqrt 2.)
@@ -34,15 +34,36 @@ typedef float f32x16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));   // 16 bytes from any element on
 
-// act'(z) in 16 bits: round(d * 2^15) + 2^13, i.e. [-0.25, 1.75); 65535 stands for NaN
-__device__ __forceinline__ uint16_t pack_slope(float d) {
-    return d != d ? (uint16_t)65535 : (uint16_t)(int)rintf(fmaf(d, 32768.f, 8192.f));
+// act'(z), in -0.129 .. 1.129, in 16 bits.  Codes from kSlopeLin on are fixed point of step 2^-15, so that a sum of
+// slopes near 1 loses nothing to speak of.  The codes below are a floating-point number of 1024 codes an octave, for
+// slopes of the sign that the activation's lower tail has (ELU's is positive, SiLU's and GELU's negative) and below
+// 2^-5: a saturated unit's, down to 2^-27 (z = -18 of ELU) to eleven bits, and in steps of 2^-37 from there.  0 and 1
+// are exact, 65535 stands for NaN.
+constexpr uint32_t kSlopeLin = 23 * 1024, kSlopeZero = kSlopeLin + 4300;     // 4300 steps: 0.1312
+constexpr float kSlopeScale = 0x1p99f;                                       // kSlopeLin << 13, as a float, times the scale: 2^-5
+constexpr uint32_t kMagic = 0x4b000000u;                                     // 2^23: the integers from there on end a float's bits
+constexpr bool slope_tail_negative(int act) { return act == GATMI_ACT_SILU || act == GATMI_ACT_GELU; }
+template <bool NEGATIVE> __device__ __forceinline__ uint16_t pack_slope(float d) {
+    // of the other sign, 2^-5 or more (once rounded) or NaN: kSlopeLin or more
+    const uint32_t small = (__float_as_uint((NEGATIVE ? -d : d) * (1.0f / kSlopeScale)) + 0x1000u) >> 13;
+    // v_med3 takes the least of the others for a NaN: the last code
+    constexpr float least = -(65535.f - kSlopeZero) / 32768.f;
+    const float t = __builtin_amdgcn_fmed3f(-d, least, 0.1312f);
+    const uint32_t lin = __float_as_uint(fmaf(t, -32768.f, 8388608.f + kSlopeZero));
+    return (uint16_t)(small < kSlopeLin ? small : lin);
+}
+// scale: kSlopeScale with the tail's sign.  (65535 is left to the caller.)
+__device__ __forceinline__ float unpack_slope(uint32_t code, float scale) {
+    const uint32_t c = kMagic | code;
+    const float lin = fmaf(__uint_as_float(c), 1.0f / 32768.f, -(8388608.f + kSlopeZero) / 32768.f);
+    const float small = __uint_as_float(c << 13) * scale;          // (kMagic's bits leave at the top)
+    return c < kMagic + kSlopeLin ? small : lin;
 }
 template <class T> struct SlopeOf { typedef uint16_t type; };
 template <> struct SlopeOf<float> { typedef float type; };
-template <class T> __device__ __forceinline__ typename SlopeOf<T>::type slope_out(float d) {
+template <class T, int ACT> __device__ __forceinline__ typename SlopeOf<T>::type slope_out(float d) {
     if constexpr (IsF32<T>::value) return d;
-    else return pack_slope(d);
+    else return pack_slope<slope_tail_negative(ACT)>(d);
 }
 
 // What the kernels need to know of an element type
@@ -207,6 +228,7 @@ struct LinArgs {
     const void *bias, *res;
     void *C;                  // [M, N]
     void *slope;              // forward: act'(z) out
+    float slope_scale;        // backward: of the slope's coding
     float *part, *dbpart;     // dW: [splits][N][K] slabs, [splits][N] column sums
     void *dw, *db;            // one split: the gradients themselves instead
     long long M;
@@ -241,7 +263,7 @@ template <class T> __device__ __forceinline__ SlopeGran<T> ld_slope_short(const 
     __builtin_memcpy(s.w, e, sizeof(e));
     return s;
 }
-template <class T> __device__ __forceinline__ VecF<8> with_slope(const Gran<T> &g, const SlopeGran<T> &s) {
+template <class T> __device__ __forceinline__ VecF<8> with_slope(const Gran<T> &g, const SlopeGran<T> &s, float scale) {
     VecF<8> v = gran_values<T>(g);
     if constexpr (IsF32<T>::value) {
 #pragma unroll
@@ -252,8 +274,8 @@ template <class T> __device__ __forceinline__ VecF<8> with_slope(const Gran<T> &
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, s.w[i]));
-            v.e[2 * i] *= fmaf((float)(s.w[i] & 0xffffu), 1.0f / 32768.f, -0.25f);
-            v.e[2 * i + 1] *= fmaf((float)(s.w[i] >> 16), 1.0f / 32768.f, -0.25f);
+            v.e[2 * i] *= unpack_slope(s.w[i] & 0xffffu, scale);
+            v.e[2 * i + 1] *= unpack_slope(s.w[i] >> 16, scale);
         }
         if (top[0] == 65535 || top[1] == 65535)      // a NaN among the eight
             for (int i = 0; i < 8; ++i)
@@ -261,10 +283,11 @@ template <class T> __device__ __forceinline__ VecF<8> with_slope(const Gran<T> &
     }
     return v;
 }
-// one value of A as it enters the products, in f32
-template <class T> __device__ __forceinline__ float one_slope(const typename SlopeOf<T>::type s) {
+
+// one slope
+template <class T> __device__ __forceinline__ float one_slope(const typename SlopeOf<T>::type s, float scale) {
     if constexpr (IsF32<T>::value) return s;
-    else return s == 65535 ? __uint_as_float(0x7fc00000u) : fmaf((float)s, 1.0f / 32768.f, -0.25f);
+    else return s == 65535 ? __uint_as_float(0x7fc00000u) : unpack_slope(s, scale);
 }
 
 // acc (32x32 blocks of a wave) += one contraction step of 16, all pieces
@@ -319,7 +342,7 @@ template <class T, int ACT> __device__ __forceinline__ void epi_values(float (&v
     for (int k = 0; k < 8; ++k) {
         float d;
         v[k] = act_both<ACT, IsF32<T>::value>(v[k] + bias.e[k], d);
-        sl[k] = slope_out<T>(d);
+        sl[k] = slope_out<T, ACT>(d);
     }
 }
 template <class T, bool FWD>
@@ -371,7 +394,7 @@ template <class T, bool FWD> __device__ __forceinline__ float plain_dot(const Li
     const long long step = FWD ? 1 : A.N;
     float s = 0.f;
 #pragma unroll 1
-    for (int k = 0; k < A.K; ++k) s = fmaf(sl ? (float)a[k] * one_slope<T>(sl[k]) : (float)a[k], (float)w[k * step], s);
+    for (int k = 0; k < A.K; ++k) s = fmaf(sl ? (float)a[k] * one_slope<T>(sl[k], A.slope_scale) : (float)a[k], (float)w[k * step], s);
     return s;
 }
 
@@ -517,10 +540,10 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
         for (int i = 0; i < NA; ++i) {
             if constexpr (TWO) {
                 if (end) drop(ga[i], over);
-                TA::put2(la, row + i * RP, g, with_slope<T>(ga[i], gs[i]));
+                TA::put2(la, row + i * RP, g, with_slope<T>(ga[i], gs[i], A.slope_scale));
                 continue;
             } else {
-                if (!FWD && sloped) ga[i] = to_gran<T>(with_slope<T>(ga[i], gs[i]));
+                if (!FWD && sloped) ga[i] = to_gran<T>(with_slope<T>(ga[i], gs[i], A.slope_scale));
                 if (end) {
                     if constexpr (CUT) shift_down<T>(ga[i].w, over);
                     else drop(ga[i], over);
@@ -640,9 +663,11 @@ template <class T, bool FWD> __global__ __launch_bounds__(256) void lin_join_ker
     if ((IsF32<T>::value || (!FWD && A.aslope)) && !(fabsf(v) < INFINITY)) v = plain_dot<T, FWD>(A, m, n);
     if constexpr (FWD) {
         const float z = v + (A.bias ? (float)static_cast<const T *>(A.bias)[n] : 0.f);
-        float d = 1.f;
-        GATMI_WITH_ACT(A.act, v = (act_both<ACT, IsF32<T>::value>(z, d)));
-        if (A.slope) static_cast<typename SlopeOf<T>::type *>(A.slope)[at] = slope_out<T>(d);
+        GATMI_WITH_ACT(A.act, {
+            float d;
+            v = act_both<ACT, IsF32<T>::value>(z, d);
+            if (A.slope) static_cast<typename SlopeOf<T>::type *>(A.slope)[at] = slope_out<T, ACT>(d);
+        });
         if (A.res) v += (float)static_cast<const T *>(A.res)[at];
     }
     static_cast<T *>(A.C)[at] = (T)v;
@@ -786,7 +811,7 @@ template <class T, int BN, bool SHORT, bool TWO> __global__ __launch_bounds__(2 
                 if (sloped) shift_down<T>(gs[i].w, 8);
             }
             if (sloped) {
-                const VecF<8> v = with_slope<T>(ga[i], gs[i]);
+                const VecF<8> v = with_slope<T>(ga[i], gs[i], A.slope_scale);
                 if (sums)
 #pragma unroll
                     for (int k = 0; k < 8; ++k) db.e[k] += v.e[k];     // before the rounding
@@ -863,7 +888,7 @@ template <class T, int BN, bool SHORT, bool TWO> __global__ __launch_bounds__(2 
                     v = 0.f;
                     for (long long m = r0; m < r1; ++m) {
                         float d = (float)pa[m * A.N + n];
-                        if (sloped) d *= one_slope<T>(static_cast<const ST *>(A.aslope)[m * A.N + n]);
+                        if (sloped) d *= one_slope<T>(static_cast<const ST *>(A.aslope)[m * A.N + n], A.slope_scale);
                         v = fmaf(d, (float)pb[m * A.K + k], v);
                     }
                 }
@@ -909,9 +934,12 @@ template <class T, int MR> __global__ __launch_bounds__(256) void lin_rows_kerne
     if (lane >= M) return;
     const long long at = (long long)lane * A.N + n;
     z += A.bias ? (float)static_cast<const T *>(A.bias)[n] : 0.f;
-    float d = 1.f, y = z;
-    GATMI_WITH_ACT(A.act, y = (act_both<ACT, IsF32<T>::value>(z, d)));
-    if (A.slope) static_cast<typename SlopeOf<T>::type *>(A.slope)[at] = slope_out<T>(d);
+    float y = z;
+    GATMI_WITH_ACT(A.act, {
+        float d;
+        y = act_both<ACT, IsF32<T>::value>(z, d);
+        if (A.slope) static_cast<typename SlopeOf<T>::type *>(A.slope)[at] = slope_out<T, ACT>(d);
+    });
     if (A.res) y += (float)static_cast<const T *>(A.res)[at];
     static_cast<T *>(A.C)[at] = (T)y;
 }
@@ -1216,6 +1244,7 @@ extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void
     A.A = grad_y;
     A.aslope = l->act == GATMI_ACT_NONE ? nullptr : slope;
     A.M = l->rows;
+    A.slope_scale = slope_tail_negative(l->act) ? -kSlopeScale : kSlopeScale;
     const bool two = lin_two(l);
     if (grad_x && l->rows > 0) {
         ProfScope ps("linear_dx", st);

@@ -36,13 +36,13 @@ def own(z, dtype):
     return 8 * U * (1 + z * z) if dtype == torch.float32 else 2.0 ** -17 + 4 * U * (1 + z * z)
 
 
-def coding(slope, dtype):
-    """what the slope's way through memory may cost: f32 tensors nothing; 16-bit ones half a step of 11 (bf16) or 12
-    bits (f16), which stop at steps of 2^-39 and 2^-25"""
+def coding(slope, dtype, name):
+    """what the slope's way through memory may cost: f32 tensors nothing; 16-bit ones half a step of 2^-15, and where
+    the slope is below 2^-5 and has the sign of the activation's lower tail half a step of eleven bits, or of 2^-37"""
     if dtype == torch.float32:
         return 0.0 * slope
-    rel, step = (2.0 ** -11, 2.0 ** -39) if dtype == torch.bfloat16 else (2.0 ** -12, 2.0 ** -25)
-    return rel * slope.abs() + step / 2
+    tail = (slope if name == "elu" else -slope) >= 0
+    return torch.where(tail & (slope.abs() < 2.0 ** -5), 2.0 ** -11 * slope.abs() + 2.0 ** -38, 2.0 ** -16)
 
 
 def within(got, want, bound, name):

@@ -33,7 +33,7 @@ def test_linear_dx_is_rounded_once(cuda, dtype, act, m, n):
     z = x.double() * float(w[0, 0])              # exact in f32 too: 8 by 8 or 11 by 11 bits
     _, d, _, size = T.act(z, act)
     dz = dy.double() * d
-    edz = dy.double().abs() * (T.own(z, dtype) * size + T.coding(d, dtype)) * 1.01 + pieces(dz, dtype) + 4 * T.U * dz.abs()
+    edz = dy.double().abs() * (T.own(z, dtype) * size + T.coding(d, dtype, act)) * 1.01 + pieces(dz, dtype) + 4 * T.U * dz.abs()
     dx = dz * float(w[0, 0])
     xd = x.to(cuda).requires_grad_(True)
     y = gat_amd.linear_act(xd, w.to(cuda), act=act)
@@ -55,7 +55,7 @@ def test_linear_dw_is_rounded_once(cuda, dtype, act, m, k, n):
     z = b.double().expand(m, n)
     _, d, _, size = T.act(z, act)
     dz = dy.double() * d
-    edz = dy.double().abs() * (T.own(z, dtype) * size + T.coding(d, dtype)) * 1.01 + pieces(dz, dtype) + 4 * T.U * dz.abs()
+    edz = dy.double().abs() * (T.own(z, dtype) * size + T.coding(d, dtype, act)) * 1.01 + pieces(dz, dtype) + 4 * T.U * dz.abs()
     wd = torch.zeros(n, k, dtype=dtype, device=cuda, requires_grad=True)
     y = gat_amd.linear_act(x.to(cuda), wd, b.to(cuda), act)
     (gw,) = torch.autograd.grad(y, wd, dy.to(cuda))
@@ -118,7 +118,7 @@ def gradient_of_saturated_units(cuda, dtype, act, m, n, lo=-12.0, hi=-4.0):
     z = x.double()
     _, d, _, size = T.act(z, act)
     dx = dy.double() * d
-    edz = dy.double().abs() * (T.own(z, dtype) * size + T.coding(d, dtype)) * 1.01 + 4 * T.U * dx.abs()
+    edz = dy.double().abs() * (T.own(z, dtype) * size + T.coding(d, dtype, act)) * 1.01 + 4 * T.U * dx.abs()
     # f32: three bf16 pieces of dz, of which the last is rounded to a multiple of bf16's smallest number, 2^-133, at
     # the coarsest: half of that, times W = 1
     edz = edz + (2.0 ** -134 if dtype == F32 else pieces(dx, dtype))
@@ -169,3 +169,30 @@ def test_values_of_saturated_units(cuda, dtype, lo, act, m, n):
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 def test_slope_of_saturated_units_f32(cuda, act, m, n):
     gradient_of_saturated_units(cuda, F32, act, m, n)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("act", ["elu", "silu", "gelu"])
+@pytest.mark.parametrize("m,n", SIZES)
+def test_slope_of_saturated_units_16_bit(cuda, dtype, act, m, n):
+    gradient_of_saturated_units(cuda, dtype, act, m, n)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("act", ["relu", "elu"])
+def test_slope_of_special_values(cuda, dtype, act):
+    """0 and 1 are exact slopes, and NaN is one of its own row only"""
+    import gat_amd
+    x = torch.tensor([3.0, 1.0, 200.0, -200.0]).to(dtype).repeat(20, 16)
+    x[:, 7] = 0.0
+    dy = torch.full_like(x, 1.25)
+    x[11, 5] = float("nan")
+    xd = x.to(cuda).requires_grad_(True)
+    y = gat_amd.linear_act(xd, torch.eye(64, dtype=dtype, device=cuda), act=act)
+    (gx,) = torch.autograd.grad(y, xd, dy.to(cuda))
+    want = torch.where(x > 0, 1.25, 0.0).to(dtype)
+    want[:, 7] = 0.0 if act == "relu" else 1.25
+    got = gx.cpu()
+    rows = torch.arange(20) != 11
+    assert torch.equal(got[rows], want[rows])
+    assert bool(torch.isnan(got[11]).all())      # every column of that row's x W^T has NaN among its terms
