@@ -2,6 +2,7 @@
 // C ABI of libgat_mi355.so (include/gat_mi355.h).  In C++ because the smallest of these calls take a few
 // microseconds on the GPU: an autograd node in Python costs ten times that (the engine's thread has to take
 // the interpreter's lock and run the backward there).  gat_amd/dense.py has the documentation.
+#include <ATen/TracerMode.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -44,6 +45,17 @@ void load(const std::string &path) {
 void check(int code, const char *what) {
     TORCH_CHECK(code == 0, what, " failed (code ", code, "): ", api.last_error());
 }
+
+// The kernels run on raw pointers, out of sight of what transforms or records torch's operators: a forward-mode
+// tangent would be dropped, and a trace would hold an empty tensor where the result was.  (vmap and torch.func's
+// wrapped tensors have no pointer and raise by themselves.)
+void plain_call(const char *name, std::initializer_list<const Tensor *> operands) {
+    TORCH_CHECK(!at::tracer::impl::is_dispatch_enabled(), "gat_amd.", name, " cannot be recorded by torch.jit.trace");
+    for (const Tensor *t : operands)
+        TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(0).defined(), "gat_amd.", name,
+                    " has no forward-mode derivative (an operand carries a tangent)");
+}
+const Tensor *maybe(const MaybeTensor &t) { return t ? &*t : nullptr; }
 
 int dtype_code(const char *name, const Tensor &x) {
     TORCH_CHECK(api.loaded, "gat_amd: the library is not loaded");
@@ -159,6 +171,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
 
 Tensor linear_act(const Tensor &x, const Tensor &w, const MaybeTensor &b, int64_t act, const MaybeTensor &r) {
     const char *me = "linear_act";
+    plain_call(me, {&x, &w, maybe(b), maybe(r)});
     const int dtype = dtype_code(me, x);
     same(me, x, w), same(me, x, b), same(me, x, r);
     check_act(me, act);
@@ -254,6 +267,7 @@ struct GroupNormFn : torch::autograd::Function<GroupNormFn> {
 
 Tensor group_norm_act(const Tensor &x, int64_t groups, const Tensor &w, const Tensor &b, double eps, int64_t act) {
     const char *me = "group_norm_act";
+    plain_call(me, {&x, &w, &b});
     const int dtype = dtype_code(me, x);
     same(me, x, w), same(me, x, b);
     check_act(me, act);
@@ -315,6 +329,7 @@ struct EmbeddingFn : torch::autograd::Function<EmbeddingFn> {
 
 Tensor embedding(const Tensor &ids, const Tensor &table, double scale) {
     const char *me = "embedding";
+    plain_call(me, {&table});
     const int dtype = dtype_code(me, table);
     TORCH_CHECK_VALUE(ids.device() == table.device(), me, ": ids on ", ids.device(), ", table on ", table.device());
     TORCH_CHECK_TYPE(ids.scalar_type() == at::kLong, me, ": ids must be int64, got ", ids.scalar_type());
@@ -370,6 +385,7 @@ struct DropoutFn : torch::autograd::Function<DropoutFn> {
 Tensor dropout(const Tensor &x, double p, bool training, uint64_t seed, MaybeTensor seed_dev, int64_t step,
                const MaybeTensor &r) {
     const char *me = "dropout";
+    if ((training && p != 0.0) || r) plain_call(me, {&x, maybe(r)});      // (otherwise x is handed back)
     const int dtype = dtype_code(me, x);
     same(me, x, r);
     TORCH_CHECK_VALUE(p >= 0.0 && p < 1.0 && (float)p < 1.f, me, ": p must be in [0, 1), got ", p);

@@ -7,7 +7,7 @@ made of when it grows a skip connection, a per-node normalisation (no statistics
 combine over the ranks of a partitioned graph) or categorical node features.  Each takes float32, bfloat16
 or float16 tensors (all of one type, any strides), computes in float32 or wider and rounds every result
 once; the same inputs give the same bits.  GPU only.  Gradients are those of one backward pass: a second
-derivative is refused.
+derivative, a forward-mode tangent and a recording by torch.jit.trace are refused.
 
 Checks, outputs, workspaces and the autograd nodes are native (gat_amd/csrc/torch_dense.cpp, built with the
 library as gat_amd/_torch_dense.so) over the same C ABI any other host uses (include/gat_mi355.h).
