@@ -3,9 +3,10 @@
 // on the matrix cores, in f32, bf16 or f16; every sum is kept in f32.
 //
 //  * 16-bit tensors multiply as they are (v_mfma_f32_32x32x16_{bf16,f16}).
-//  * f32 tensors are cut exactly into three bf16 pieces each, v = p0 + p1 + p2, and multiply as the
+//  * f32 tensors are cut into three bf16 pieces each, v = p0 + p1 + p2, and multiply as the
 //    six products p_i q_j with i + j <= 2: what is left out is 2^-25 of a product, less than an f32
-//    multiply rounds, at 16/6 of the f32 MFMA's rate.  A sum that comes out infinite or NaN (an operand
+//    multiply rounds, at 16/6 of the f32 MFMA's rate.  The pieces are exact for |v| from 2^-110 (7.7e-34) on; of a
+//    smaller v they hold the nearest multiple of bf16's smallest number, 2^-133 (the matrix cores keep subnormals).  A sum that comes out infinite or NaN (an operand
 //    was, or a piece rounded up to infinity next to the largest float) is taken again in plain f32.
 //  * act'(z) is written by the forward when a backward follows: f32 for f32 tensors, for 16-bit ones in 16 bits, to
 //    2^-16 and, where a unit is saturated and the slope small, to 2^-11 of itself (see pack_slope).

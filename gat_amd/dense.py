@@ -60,7 +60,8 @@ def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, act: st
                residual: Optional[Tensor] = None) -> Tensor:
     """act(x @ weight.T + bias) + residual in one kernel: x [..., in], weight [out, in], bias [out],
     residual [..., out]; act one of ACTIVATIONS ("gelu" is the exact form).  With `residual=conv(x)` it is
-    the skip connection beside a GAT layer."""
+    the skip connection beside a GAT layer.  float32 operands smaller than 2^-110 (7.7e-34) count as the nearest
+    multiple of 2^-133."""
     return (_native or _load()).linear_act(x, weight, bias, _act("linear_act", act), residual)
 
 

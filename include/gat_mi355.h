@@ -467,8 +467,9 @@ int gatmi_knn_graph_ties(const double *x, int64_t n, int32_t f, int32_t k, int64
 #define GATMI_ACT_SILU 3
 #define GATMI_ACT_GELU 4   /* the exact form, by erf */
 
-/* y = act(x W^T + b) + residual.  f32 tensors multiply on the bf16 matrix cores as three exact bf16 pieces
- * each, at f32 accuracy (csrc/linear.hip). */
+/* y = act(x W^T + b) + residual.  f32 tensors multiply on the bf16 matrix cores as three bf16 pieces each, at
+ * f32 accuracy for operands from 2^-110 (7.7e-34) on; smaller ones count as the nearest multiple of 2^-133
+ * (csrc/linear.hip; up to 16 rows forward are plain f32). */
 typedef struct gatmi_linear {
     int64_t rows;          /* < 2^31 */
     int32_t in_features;   /* 1 .. 65536 */
