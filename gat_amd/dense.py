@@ -74,6 +74,16 @@ def group_norm_act(x: Tensor, groups: int, weight: Tensor, bias: Tensor, eps: fl
     return (_native or _load()).group_norm_act(x, int(groups), weight, bias, float(eps), _act("group_norm_act", act))
 
 
+def stock_group_norm(x: Tensor, norm: torch.nn.GroupNorm) -> Tensor:
+    """norm(x) for x [N, C] in elementary torch operations, any device and type: what the networks' stock paths take.
+    Not F.group_norm: its weight and bias gradients are wrong on this platform for rows without further axes
+    (more than 128 of them)."""
+    v = x.reshape(x.size(0), norm.num_groups, x.size(1) // norm.num_groups)
+    var, mean = torch.var_mean(v, dim=2, unbiased=False, keepdim=True)
+    v = ((v - mean) * torch.rsqrt(var + norm.eps)).view_as(x)
+    return v * norm.weight + norm.bias
+
+
 def embedding(ids: Tensor, table: Tensor, scale: float = 1.0) -> Tensor:
     """scale * table[ids]: ids int64 of any shape, table [entries, dim] -> [..., dim].  An id outside the table
     (-1 for "none") gives a zero row and takes no gradient.  The table's gradient is dense, summed over the

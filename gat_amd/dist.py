@@ -1071,9 +1071,9 @@ class PartitionedGAT(nn.Module):
         """dropout(bn(elu(x))) with the batch statistics of all N rows (model.py:40-42, 43-45); with
         norm="group" dropout(elu(group_norm(x))), row by row"""
         if self.norm == "group":
+            from .dense import dropout, group_norm_act, stock_group_norm
             if not self.fused:
-                return self._drop(torch.nn.functional.elu(bn(x)))
-            from .dense import dropout, group_norm_act
+                return self._drop(torch.nn.functional.elu(stock_group_norm(x, bn)))
             x = group_norm_act(x, bn.num_groups, bn.weight, bn.bias, bn.eps, "elu")
             if not self.training or self.p <= 0.0:
                 return x

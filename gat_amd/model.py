@@ -38,7 +38,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .data import Data, Metrics
-from .dense import dropout, embedding as embed, group_norm_act, linear_act
+from .dense import dropout, embedding as embed, group_norm_act, linear_act, stock_group_norm
 from .glue import elu_bn_dropout, log_softmax_nll
 from .layer import GATConv
 
@@ -179,12 +179,7 @@ class GAT(nn.Module):
         if self.fused_glue:
             x = group_norm_act(x, norm.num_groups, norm.weight, norm.bias, norm.eps, "elu")
             return dropout(x, p, self.training, seed)
-        # not F.group_norm: its weight and bias gradients are wrong on this platform for rows without further
-        # axes (more than 128 of them)
-        v = x.view(x.size(0), norm.num_groups, -1)
-        var, mean = torch.var_mean(v, dim=2, unbiased=False, keepdim=True)
-        v = ((v - mean) * torch.rsqrt(var + norm.eps)).view_as(x)
-        return self.dropout(F.elu(v * norm.weight + norm.bias))
+        return self.dropout(F.elu(stock_group_norm(x, norm)))
 
     def _logits(self, data):
         x, edge_index = self._features(data), data.edge_index
