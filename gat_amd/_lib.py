@@ -157,6 +157,7 @@ SYMBOLS = {
     "gatmi_linear_fwd": (C.c_int, [C.POINTER(Linear), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "gatmi_linear_bwd_workspace_bytes": (C.c_size_t, [C.POINTER(Linear)]),
+    "gatmi_linear_bwd_workspace_bytes_of": (C.c_size_t, [C.POINTER(Linear), C.c_int32, C.c_int32, C.c_int32]),
     "gatmi_linear_bwd": (C.c_int, [C.POINTER(Linear), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                    C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "gatmi_group_norm_workspace_bytes": (C.c_size_t, [C.POINTER(GroupNorm)]),

@@ -873,6 +873,7 @@ template <class T, int BN, bool SHORT, bool TWO> __global__ __launch_bounds__(2 
             else A.dbpart[split * A.N + n0 + threadIdx.x] = s;
         }
     }
+    if (!A.part && !A.dw) return;       // the bias alone
     bool again = IsF32<T>::value;
     if constexpr (TWO) again = redo<T, 2, 2>(acc, pb + r0 * A.K + k0, r1 - r0, A.K, A.K - k0 < BN ? A.K - k0 : BN);
     float *part = A.part + split * (long long)A.N * A.K;
@@ -1050,7 +1051,7 @@ struct LinGeom {
     bool wide;                      // dW's tiles: 256 columns of x, for which dz is made once, instead of 128
     long long per_split;
     int ldf, ldb;                   // row lengths of the weight images, forward and transposed
-    size_t image_f, image_b, slabs, dbpart;     // bytes
+    size_t image_f, image_b, slabs, dbpart;     // bytes; slabs and dbpart are used by more than one split only
     LinSplitK fwd, dx;
     bool image_fwd;                 // the forward takes an image
     bool few;                       // ... or the few-row kernel
@@ -1218,10 +1219,32 @@ extern "C" int gatmi_linear_fwd(const gatmi_linear *l, const void *x, const void
     return GATMI_OK;
 }
 
+// The backward's workspace: [weights' image][slabs][column sums], the sums of a split dx where the slabs follow
+struct LinBwdWs {
+    bool one;               // dW's single split writes the gradients themselves
+    size_t image, slabs, bytes;
+};
+static LinBwdWs lin_bwd_ws(const LinGeom &G, bool x, bool w, bool b) {
+    LinBwdWs W;
+    W.one = G.splits == 1 && w;
+    W.image = x ? G.image_b : 0;
+    W.slabs = w && !W.one ? G.slabs : 0;
+    const size_t dw = W.slabs + (b && !W.one ? G.dbpart : 0), dx = x ? G.dx.bytes : 0;
+    W.bytes = W.image + (dw > dx ? dw : dx);
+    return W;
+}
+
+extern "C" size_t gatmi_linear_bwd_workspace_bytes_of(const gatmi_linear *l, int32_t grad_x, int32_t grad_weight,
+                                                      int32_t grad_bias) {
+    if (lin_check(l)) return 0;
+    return lin_bwd_ws(lin_geom(l), grad_x, grad_weight, grad_bias).bytes;
+}
+
 extern "C" size_t gatmi_linear_bwd_workspace_bytes(const gatmi_linear *l) {
     if (lin_check(l)) return 0;
     const LinGeom G = lin_geom(l);
-    return G.image_b + (G.slabs + G.dbpart > G.dx.bytes ? G.slabs + G.dbpart : G.dx.bytes);
+    const size_t all = lin_bwd_ws(G, true, true, true).bytes, some = lin_bwd_ws(G, true, false, true).bytes;
+    return all > some ? all : some;
 }
 
 extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void *weight, const void *slope,
@@ -1231,14 +1254,14 @@ extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void
     GATMI_REQUIRE(l->rows == 0 || (x && weight && grad_y), "linear_bwd: null argument");
     GATMI_REQUIRE(l->act == GATMI_ACT_NONE || slope || l->rows == 0, "linear_bwd: the activation's slope is missing");
     const LinGeom G = lin_geom(l);
-    const size_t need = gatmi_linear_bwd_workspace_bytes(l);
-    if (!ws || ws_bytes < need) {
-        set_error("linear workspace too small: %zu < %zu", ws_bytes, need);
+    const LinBwdWs W = lin_bwd_ws(G, grad_x, grad_weight, grad_bias);
+    if (ws_bytes < W.bytes || (W.bytes && !ws)) {
+        set_error("linear workspace too small: %zu < %zu", ws_bytes, W.bytes);
         return GATMI_ERR_WS;
     }
     hipStream_t st = static_cast<hipStream_t>(stream);
     char *image = static_cast<char *>(ws);
-    float *slabs = reinterpret_cast<float *>(image + G.image_b), *dbpart = reinterpret_cast<float *>(image + G.image_b + G.slabs);
+    float *slabs = reinterpret_cast<float *>(image + W.image), *dbpart = reinterpret_cast<float *>(image + W.image + W.slabs);
     const int N = l->out_features, K = l->in_features;
     LinArgs A;
     memset(&A, 0, sizeof(A));
@@ -1271,8 +1294,8 @@ extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void
         A.B = x;
         A.N = N;
         A.K = K;
-        A.part = slabs;
-        const bool one = G.splits == 1 && grad_weight;
+        const bool one = W.one;
+        A.part = grad_weight && !one ? slabs : nullptr;
         A.dbpart = grad_bias && !one ? dbpart : nullptr;
         A.dw = one ? grad_weight : nullptr;
         A.db = one ? grad_bias : nullptr;

@@ -23,7 +23,7 @@ struct Api {
 #define ENTRY(name) decltype(&gatmi_##name) name = nullptr;
 #define ENTRIES                                                                           \
     ENTRY(last_error) ENTRY(linear_fwd_workspace_bytes) ENTRY(linear_fwd)                 \
-    ENTRY(linear_bwd_workspace_bytes) ENTRY(linear_bwd) ENTRY(group_norm_workspace_bytes) \
+    ENTRY(linear_bwd_workspace_bytes_of) ENTRY(linear_bwd) ENTRY(group_norm_workspace_bytes) \
     ENTRY(group_norm_fwd) ENTRY(group_norm_bwd) ENTRY(embedding_fwd)                      \
     ENTRY(embedding_bwd_workspace_bytes) ENTRY(embedding_bwd) ENTRY(dropout)
     ENTRIES
@@ -135,7 +135,8 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
                           const MaybeTensor &r_, int64_t dtype, int64_t act, bool keep) {
         const Tensor x = x_.contiguous(), w = w_.contiguous();
         auto [y, slope] = linear_run(x, w, contiguous(b_), contiguous(r_), (int)dtype, act, keep);
-        ctx->save_for_backward({x, w, slope});
+        if (keep) ctx->save_for_backward({x, w, slope});       // (a gradient of the residual alone needs none)
+        else ctx->save_for_backward({Tensor(), Tensor(), Tensor()});
         ctx->saved_data["bias"] = b_.has_value();
         ctx->saved_data["residual"] = r_.has_value();
         ctx->saved_data["dtype"] = dtype;
@@ -159,7 +160,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
             if (nx) out[0] = at::empty(x.sizes(), x.options());
             if (nw) out[1] = at::empty(w.sizes(), w.options());
             if (nb) out[2] = at::empty({w.size(0)}, w.options());
-            const size_t need = api.linear_bwd_workspace_bytes(&d);
+            const size_t need = api.linear_bwd_workspace_bytes_of(&d, nx, nw, nb);
             Tensor ws = bytes_like(need, x);
             check(api.linear_bwd(&d, ptr(x), ptr(w), ptr(slope), ptr(gy), ptr(out[0]), ptr(out[1]), ptr(out[2]), ptr(ws),
                                  need, stream_of(x)),

@@ -486,7 +486,10 @@ int gatmi_linear_fwd(const gatmi_linear *l, const void *x, const void *weight, c
 /*   slope: what the forward wrote (NULL when act == NONE);  grad_y [rows, out]
  *   -> grad_x [rows, in], grad_weight [out, in], grad_bias [out], each NULL to skip.  The residual's
  *   gradient is grad_y itself. */
-size_t gatmi_linear_bwd_workspace_bytes(const gatmi_linear *l);
+size_t gatmi_linear_bwd_workspace_bytes(const gatmi_linear *l);      /* enough for any of them */
+/* of just these (0 / 1); may be 0, then ws may be NULL */
+size_t gatmi_linear_bwd_workspace_bytes_of(const gatmi_linear *l, int32_t grad_x, int32_t grad_weight,
+                                           int32_t grad_bias);
 int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void *weight, const void *slope,
                      const void *grad_y, void *grad_x, void *grad_weight, void *grad_bias, void *ws,
                      size_t ws_bytes, void *stream);
