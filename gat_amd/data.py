@@ -103,11 +103,18 @@ def create_knn_graph(X, k: int = 5, backend: str = "auto", device=None) -> torch
     return _knn_graph_sklearn(values, k)
 
 
-def convert_to_graph(X, y) -> Data:
+def convert_to_graph(X, y, ids=None) -> Data:
+    """ids (not in the reference): categorical codes of the rows for GAT(embedding=...), [N] or [N, K], integers,
+    -1 for none."""
     xv = X.values if hasattr(X, "values") else np.asarray(X)
     yv = y.values if hasattr(y, "values") else np.asarray(y)
+    if ids is not None:
+        codes = ids.values if hasattr(ids, "values") else np.asarray(ids)
+        if codes.ndim not in (1, 2) or codes.shape[0] != xv.shape[0] or codes.dtype.kind not in "iu":
+            raise ValueError(f"ids must be integers, one row for each of the {xv.shape[0]} nodes, got {codes.dtype} {codes.shape}")
+        ids = torch.tensor(codes.astype(np.int64))
     return Data(x=torch.tensor(xv, dtype=torch.float), edge_index=create_knn_graph(X),
-                y=torch.tensor(yv, dtype=torch.long))
+                y=torch.tensor(yv, dtype=torch.long), ids=ids)
 
 
 @dataclass
