@@ -72,11 +72,15 @@ template <bool EXACT> __device__ __forceinline__ float act_exp(float v) {
     return __builtin_amdgcn_exp2f(v * 1.44269502162933349609375f);
 }
 
-// exp(z) for z <= 0, to a few of its own steps however small it is; NaN for NaN
+// exp(z) for z <= 0, to a few of its own steps however small it is: 0 for -inf, NaN for NaN.  EXACT: as exp_fast, whose
+// end at -87 applies to the correction alone here.
 template <bool EXACT> __device__ __forceinline__ float act_exp_neg(float z) {
-    const float e = act_exp<false>(z);
-    if constexpr (EXACT) return z >= -87.0f ? exp_fast(z) : e;      // (exp_fast stops at -87)
-    return e;
+    if constexpr (!EXACT) return act_exp<false>(z);
+    const float L2E = 1.44269502162933349609375f, L2E_LO = 1.925963033500011e-8f;
+    const float c = fmaxf(z, -87.0f);
+    const float r = fmaf(c, L2E_LO, fmaf(c, L2E, -(c * L2E)));
+    const float e = __builtin_amdgcn_exp2f(z * L2E);
+    return fmaf(e, r * 0.693147182464599609375f, e);
 }
 
 // exp(z) - 1 for z <= 0, from exp(z)
