@@ -64,15 +64,15 @@ __device__ __forceinline__ uint32_t fdiv(const FastDiv &f, uint32_t n) {
     return f.s == 0 ? n : (t + ((n - t) >> 1)) >> (f.s - 1);
 }
 
-// ---- activations: value and derivative at z, f32.  EXACT: the library's expm1 / exp / erf, for f32
-// tensors.  Otherwise (results are rounded to 16 bits) v_exp_f32 and v_rcp_f32 forms, whose error of at most
-// 2^-17 of the value is small beside that rounding (2^-11 for f16, 2^-8 for bf16), where the value itself is small too.
+// ---- activations: value and derivative at z, f32.  EXACT: to a few steps of f32, for f32 tensors.  Otherwise
+// (results are rounded to 16 bits) v_exp_f32 and v_rcp_f32 forms, whose error of at most 2^-17 of the value is small
+// beside that rounding (2^-11 for f16, 2^-8 for bf16), where the value itself is small too.
 template <bool EXACT> __device__ __forceinline__ float act_exp(float v) {
     if constexpr (EXACT) return expf(v);   // of either sign
     return __builtin_amdgcn_exp2f(v * 1.44269502162933349609375f);
 }
 
-// exp(z) for z <= 0, to a few of its own steps however small it is: 0 for -inf, NaN for NaN.  EXACT: as exp_fast, whose
+// exp(z) for z <= 0, to a few of its own steps down to the smallest normal number, then 0; NaN for NaN.  EXACT: as exp_fast, whose
 // end at -87 applies to the correction alone here.
 template <bool EXACT> __device__ __forceinline__ float act_exp_neg(float z) {
     if constexpr (!EXACT) return act_exp<false>(z);
@@ -102,15 +102,29 @@ template <bool EXACT> __device__ __forceinline__ float act_expm1(float z, float 
     return z < -0.03f ? e - 1.0f : s;
 }
 
-// The normal distribution function, its lower tail relative to itself: from erfc, not as 1 + erf, which is nothing
-// where erf rounds to -1 and has lost half its digits by z = -3.  16-bit results: exp(-z^2/2) times a polynomial in
-// t = 1 / (1 + p |z|), fitted to erfc(a) exp(a^2) / 2 (a = |z| / sqrt 2, up to 10) for the smallest relative error,
-// which is 2^-17.9; v_exp adds z^2 2^-24 of its argument's rounding.  `gauss` = exp(-z^2/2).
+// The normal distribution function, its lower tail relative to itself, not as 1 + erf, which is nothing where erf
+// rounds to -1 and has lost half its digits by z = -3: exp(-z^2/2) times a polynomial in t = 1 / (1 + p |z|), fitted to
+// erfc(a) exp(a^2) / 2 (a = |z| / sqrt 2, up to 10) for the smallest relative error.  EXACT: degree 9, 2^-25.6, with
+// 1 / (1 + p |z|) corrected by its residual and z^2 by what its rounding left; 8 f32 steps in all (the library's erfc
+// costs twice the arithmetic: group norm with GELU of [100000, 8 x 30] f32 52 us forward).  16-bit results: degree 6,
+// 2^-17.9; v_exp adds z^2 2^-24 of its argument's rounding.  `gauss` = exp(-z^2/2).
 template <bool EXACT> __device__ __forceinline__ float act_phi(float z, float &gauss) {
     float tail;
     if constexpr (EXACT) {
-        gauss = expf(-0.5f * z * z);
-        tail = 0.5f * erfcf(fabsf(z) * 0.70710678118654752f);
+        const float a = fminf(fabsf(z), 20.0f);                 // the tail is 0 from 14.2 on; a^2 stays finite
+        const float h = a * a, e = act_exp_neg<true>(-0.5f * h);
+        gauss = fmaf(-0.5f * fmaf(a, a, -h), e, e);
+        float t = __builtin_amdgcn_rcpf(fmaf(0.26870057f, a, 1.0f));
+        t = fmaf(t, fmaf(-(t * a), 0.26870057f, 1.0f - t), t);
+        float q = fmaf(t, 0.0294948481f, -0.131197944f);
+        q = fmaf(t, q, 0.18205376f);
+        q = fmaf(t, q, -0.0808761716f);
+        q = fmaf(t, q, 0.115118489f);
+        q = fmaf(t, q, 0.0692774951f);
+        q = fmaf(t, q, 0.101966202f);
+        q = fmaf(t, q, 0.106957726f);
+        q = fmaf(t, q, 0.1072056f);
+        tail = q * t * gauss;
     } else {
         gauss = act_exp<false>(-0.5f * z * z);
         const float t = __builtin_amdgcn_rcpf(fmaf(0.308308125f, fabsf(z), 1.0f));

@@ -196,3 +196,31 @@ def test_slope_of_special_values(cuda, dtype, act):
     rows = torch.arange(20) != 11
     assert torch.equal(got[rows], want[rows])
     assert bool(torch.isnan(got[11]).all())      # every column of that row's x W^T has NaN among its terms
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("act", ["elu", "silu", "gelu"])
+def test_activations_at_the_ends_of_their_range(cuda, dtype, act):
+    """W = 0 and z the bias: far beyond any exponential's range values and slopes are those of the limit, infinities
+    and NaN as z * factor gives them"""
+    import gat_amd
+    inf, nan, top = float("inf"), float("nan"), torch.finfo(dtype).max
+    far = [top, -top, top / 3, -top / 3, 100.0, -100.0, 89.0, -89.0, 30.0, -30.0, 20.5, -20.5, 0.0, -0.0]
+    b = torch.tensor(far + [inf, -inf, nan] + [1.0] * 7).to(dtype)
+    for m in (1, 20):
+        x, w = torch.zeros(m, 8, dtype=dtype, device=cuda), torch.zeros(24, 8, dtype=dtype, device=cuda)
+        bd = b.to(cuda).requires_grad_(True)
+        y = gat_amd.linear_act(x, w, bd, act)
+        (db,) = torch.autograd.grad(y, bd, torch.tensor([1.0] + [0.0] * (m - 1), dtype=dtype, device=cuda)[:, None].expand(m, 24))
+        n = len(far)
+        z = b[:n].double()
+        a, d, size, dsize = T.act(z, act)
+        # v_exp_f32 gives 0 for a subnormal result: exp(-89) = 2.2e-39 and what it multiplies, |z| <= 89, are within that
+        # many times the smallest normal f32 number of 0
+        flushed = 90 * torch.finfo(F32).smallest_normal
+        T.within(y[0, :n], a, T.own(z.clamp(-20, 20), dtype) * size + T.u(dtype) * a.abs() + flushed, "y")
+        T.within(db[:n], d, T.own(z.clamp(-20, 20), dtype) * dsize + T.coding(d, dtype, act) + T.u(dtype) * d.abs() + flushed, "slope")
+        y = y.detach().cpu()
+        assert float(y[0, n]) == inf and bool(torch.isnan(y[0, n + 2])) and bool(torch.isnan(db[n + 2]))
+        assert float(y[0, n + 1]) == -1.0 if act == "elu" else bool(torch.isnan(y[0, n + 1]))
+        assert bool(torch.isfinite(y[0, n + 3:]).all())
