@@ -14,10 +14,10 @@
 // No sum is made with atomics: the same inputs give the same bits.
 //
 // Memory bounds all of it.  [100000, 8 x 30] f32: forward with the statistics kept 36 us for 193 MB (5.3 TB/s),
-// backward 52 us for 289 MB (5.6 TB/s) and 10 us for the parameter sums.  [3, 169343, 256] bf16: statistics 65 us
-// (260 MB), applying them 84 (520 MB), the backward's sums 140 (520 MB), dx 140 (780 MB, 5.6 TB/s); the sums'
+// backward 49 us for 289 MB (5.9 TB/s) and 10 us for the parameter sums.  [3, 169343, 256] bf16: statistics 67 us
+// (260 MB), applying them 85 (520 MB), the backward's sums 136 (520 MB), dx 139 (780 MB, 5.6 TB/s); the sums'
 // pass is the one that its arithmetic holds back (SiLU and its derivative for two bytes read of x), and x and dy
-// are read twice because a sample of 43 MB fits no block's memory.
+// are read twice because a sample of 87 MB fits no block's memory.
 #include "attn_device.h"
 #include "common.h"
 #include "dense_device.h"
