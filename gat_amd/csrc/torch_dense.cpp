@@ -203,6 +203,7 @@ gatmi_group_norm group_norm_desc(const Tensor &x, const Tensor &w, const Tensor 
     d.batch = x.size(0);
     d.length = 1;
     for (int64_t i = 1; i + 1 < x.dim(); ++i) d.length *= x.size(i);
+    if (d.length == 0) d.length = 1;       // no samples either (checked)
     d.groups = (int32_t)groups;
     d.width = (int32_t)(x.size(-1) / groups);
     d.dtype = dtype;
