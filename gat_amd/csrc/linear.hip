@@ -6,15 +6,17 @@
 //  * f32 tensors are cut into three bf16 pieces each, v = p0 + p1 + p2, and multiply as the
 //    six products p_i q_j with i + j <= 2: what is left out is 2^-25 of a product, less than an f32
 //    multiply rounds, at 16/6 of the f32 MFMA's rate.  The pieces are exact for |v| from 2^-110 (7.7e-34) on; of a
-//    smaller v they hold the nearest multiple of bf16's smallest number, 2^-133 (the matrix cores keep subnormals).  A sum that comes out infinite or NaN (an operand
-//    was, or a piece rounded up to infinity next to the largest float) is taken again in plain f32.
+//    smaller v they hold the nearest multiple of bf16's smallest number, 2^-133 (the matrix cores keep subnormals).
+//    A sum that comes out infinite or NaN (an operand was, or a piece rounded up to infinity next to the largest
+//    float) is taken again in plain f32.
 //  * act'(z) is written by the forward when a backward follows: f32 for f32 tensors, for 16-bit ones in 16 bits, to
 //    2^-16 and, where a unit is saturated and the slope small, to 2^-11 of itself (see pack_slope).
 //  * dz = dy act'(z) of 16-bit tensors does not fit their type.  It enters the products as two numbers of it,
 //    dz = hi + lo, lo what hi's rounding left: a product more a step, and dx and dW are rounded once, as they
 //    are stored.  (One number: every dz off by up to half a step, and the error of dx and dW larger by sqrt 2.)
 //    ReLU's slopes are 0 and 1, dz is dy or nothing, and one number is enough.  An infinite or NaN factor on the
-//    other side would meet a zero lo or one of the other sign: see `redo`.
+//    other side would meet a lo of zero, or of the other sign than hi: such sums are made with hi for lo, twice the
+//    sum of the rounded dz (dx: where lin_image_kernel has seen such weights; dW: in a second pass, see `redo`).
 //
 // What bounds it (times of the kernels alone under the profiler, whose clock varies by a few percent from run to run).
 // The forward of layers of a few hundred columns is bound by memory for 16-bit types: [2449029, 256] x [256, 256] bf16
@@ -172,8 +174,8 @@ template <class T> __device__ __forceinline__ Gran<T> to_gran(const VecF<8> &v) 
 }
 
 // v = hi + lo, both of the tensor's type.  hi stays finite, so that lo is v - hi for every v: infinite where v is
-// (v_med3), NaN where v is.
-template <class T> __device__ __forceinline__ void split2(const VecF<8> &v, Gran<T> &hi, Gran<T> &lo) {
+// (v_med3), NaN where v is.  twice: hi again for a finite lo.
+template <class T> __device__ __forceinline__ void split2(const VecF<8> &v, Gran<T> &hi, Gran<T> &lo, bool twice) {
     const float top = std::is_same<T, f16_t>::value ? 65504.f : 3.3895313892515355e38f;
     VecF<8> h, l;
 #pragma unroll
@@ -182,6 +184,9 @@ template <class T> __device__ __forceinline__ void split2(const VecF<8> &v, Gran
     h = gran_values<T>(hi);
 #pragma unroll
     for (int i = 0; i < 8; ++i) l.e[i] = v.e[i] - h.e[i];
+    if (twice)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) l.e[i] = fabsf(l.e[i]) < INFINITY ? h.e[i] : l.e[i];
     lo = to_gran<T>(l);
 }
 
@@ -208,10 +213,10 @@ template <class T, int R, int PIECES = Mul<T>::PIECES> struct Tile {
                 *reinterpret_cast<u32x4 *>(lds + p * PLANE + at(row, g)) = u32x4{q[p][0], q[p][1], q[p][2], q[p][3]};
         }
     }
-    static __device__ __forceinline__ void put2(char *lds, int row, int g, const VecF<8> &v) {
+    static __device__ __forceinline__ void put2(char *lds, int row, int g, const VecF<8> &v, bool twice) {
         static_assert(P == 2, "a tile of halves");
         Gran<T> q[2];
-        split2<T>(v, q[0], q[1]);
+        split2<T>(v, q[0], q[1], twice);
 #pragma unroll
         for (int p = 0; p < 2; ++p)
             *reinterpret_cast<u32x4 *>(lds + p * PLANE + at(row, g)) = u32x4{q[p].w[0], q[p].w[1], q[p].w[2], q[p].w[3]};
@@ -221,13 +226,14 @@ template <class T, int R, int PIECES = Mul<T>::PIECES> struct Tile {
     }
 };
 
-
 constexpr int kBM = 128;      // rows of dW's tiles
 
 struct LinArgs {
     const void *A, *B;        // [M, K] and [N, K], rows of K elements (B: of ldb)
     const void *plain;        // f32: the weights as they are ([N, K], or [K, N] when A is dy)
     const void *aslope;       // A is multiplied by this slope on its way in (dz = dy act'(z))
+    const uint8_t *bad;       // TWO: [rows of B / 32][bad_cols], whether 32 x 32 of B are all finite (0) or not
+    int bad_cols;
     const void *bias, *res;
     void *C;                  // [M, N]
     void *slope;              // forward: act'(z) out
@@ -287,12 +293,6 @@ template <class T> __device__ __forceinline__ VecF<8> with_slope(const Gran<T> &
     return v;
 }
 
-// one slope
-template <class T> __device__ __forceinline__ float one_slope(const typename SlopeOf<T>::type s, float scale) {
-    if constexpr (IsF32<T>::value) return s;
-    else return s == 65535 ? __uint_as_float(0x7fc00000u) : unpack_slope(s, scale);
-}
-
 // acc (32x32 blocks of a wave) += one contraction step of 16, all pieces
 template <class T, int PA, int MI, int NI>
 __device__ __forceinline__ void mma_pieces(const u32x4 (&a)[MI][PA], const u32x4 (&b)[NI][Mul<T>::PIECES],
@@ -320,7 +320,9 @@ template <class T, class TA, class TB, int MI, int NI>
 __device__ __forceinline__ void tile_mma(const char *la, const char *lb, int ra, int rb, int lane,
                                          f32x16v (&acc)[MI][NI]) {
     const int r = lane & 31, half = lane >> 5;
-#pragma unroll
+    // (two numbers of f16, unrolled whole: registers go to scratch memory)
+    constexpr int kUnroll = std::is_same<T, f16_t>::value && TA::P == 2 ? 2 : TA::BK / 16;
+#pragma unroll kUnroll
     for (int s = 0; s < TA::BK / 16; ++s) {
         u32x4 a[MI][TA::P], b[NI][TB::P];
 #pragma unroll
@@ -388,36 +390,16 @@ __device__ __forceinline__ void epi_piece(const LinArgs &A, long long m, int n, 
     }
 }
 
-// the sum in plain f32, an element at a time: what the pieces cannot say
-template <class T, bool FWD> __device__ __forceinline__ float plain_dot(const LinArgs &A, long long m, int n) {
-    typedef typename SlopeOf<T>::type ST;
-    const T *a = static_cast<const T *>(A.A) + m * A.K;
-    const ST *sl = FWD || !A.aslope ? nullptr : static_cast<const ST *>(A.aslope) + m * A.K;
-    const T *w = static_cast<const T *>(A.plain) + (FWD ? (long long)n * A.K : n);
+// the sum in plain f32, an element at a time: what the pieces cannot say (f32 only)
+template <bool FWD> __device__ __forceinline__ float plain_dot(const LinArgs &A, long long m, int n) {
+    const float *a = static_cast<const float *>(A.A) + m * A.K;
+    const float *sl = FWD || !A.aslope ? nullptr : static_cast<const float *>(A.aslope) + m * A.K;
+    const float *w = static_cast<const float *>(A.plain) + (FWD ? (long long)n * A.K : n);
     const long long step = FWD ? 1 : A.N;
     float s = 0.f;
 #pragma unroll 1
-    for (int k = 0; k < A.K; ++k) s = fmaf(sl ? (float)a[k] * one_slope<T>(sl[k], A.slope_scale) : (float)a[k], (float)w[k * step], s);
+    for (int k = 0; k < A.K; ++k) s = fmaf(sl ? a[k] * sl[k] : a[k], w[k * step], s);
     return s;
-}
-
-// Whether this block's sums need the plain ones after all, where dz is two numbers: some sum is not finite, and so
-// is some factor of the other side among `rows` rows (`stride` apart) of `cols` columns.  An infinity of dz alone
-// comes out right.
-template <class T, int MI, int NI>
-__device__ __forceinline__ bool redo(const f32x16v (&acc)[MI][NI], const T *b, long long rows, long long stride, int cols) {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j)
-#pragma unroll
-            for (int q = 0; q < 16; ++q) s = fmaf(acc[i][j][q], 0.f, s);       // NaN once one is not finite
-    if (!__syncthreads_or(s != 0.f)) return false;
-    bool bad = false;
-    for (long long r = 0; r < rows; ++r)
-        for (int c = threadIdx.x; c < cols; c += blockDim.x) bad = bad || !(fabsf((float)b[r * stride + c]) < INFINITY);
-    return __syncthreads_or(bad);
 }
 
 // One block a tile, through registers into one LDS buffer: the next step's loads are on their way while this
@@ -533,7 +515,17 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
         for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
-    fetch(k_first);
+    bool twice = false;
+    if constexpr (TWO) {        // (in front of the first loads, which take as long)
+        const int groups = (A.N - n0 < BN ? A.N - n0 + 31 : BN) / 32;
+        const uint8_t *bad = A.bad + (long long)(n0 / 32) * A.bad_cols;
+        uint32_t any = 0;
+        for (int i = threadIdx.x; i < groups * A.bad_cols; i += THREADS) any |= bad[i];
+        fetch(k_first);
+        twice = __builtin_amdgcn_readfirstlane(__syncthreads_or(any)) != 0;
+    } else {
+        fetch(k_first);
+    }
     for (int k0 = k_first; k0 < k_end; k0 += TA::BK) {
         // the row's last, partial step: what a granule holds of the one before it is dropped.  An image has
         // zeros behind K instead of a step back, in its place: A must line up, so it is moved down there.
@@ -543,7 +535,7 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
         for (int i = 0; i < NA; ++i) {
             if constexpr (TWO) {
                 if (end) drop(ga[i], over);
-                TA::put2(la, row + i * RP, g, with_slope<T>(ga[i], gs[i], A.slope_scale));
+                TA::put2(la, row + i * RP, g, with_slope<T>(ga[i], gs[i], A.slope_scale), twice);
                 continue;
             } else {
                 if (!FWD && sloped) ga[i] = to_gran<T>(with_slope<T>(ga[i], gs[i], A.slope_scale));
@@ -571,6 +563,13 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
         tile_mma<T, TA, TB, MI, NI>(la, lb, wm, wn, lane, acc);
         __syncthreads();
     }
+    if (TWO && twice)
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) acc[i][j][q] *= 0.5f;
     if constexpr (PART) {
         float *part = A.part + split * A.M * A.N;
 #pragma unroll
@@ -585,9 +584,6 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
                 }
         return;
     }
-    bool again = IsF32<T>::value;
-    if constexpr (TWO)
-        again = redo<T, MI, NI>(acc, reinterpret_cast<const T *>(bb), A.N - n0 < BN ? A.N - n0 : BN, A.ldb, A.K);
     // epilogue: a wave turns its blocks 16 rows at a time through LDS of its own into row pieces of 8
     float *le = reinterpret_cast<float *>(smem) + wave * 16 * LD;
     constexpr int PR = NI * 4, RI = 64 / PR;        // pieces a row, rows at once
@@ -634,7 +630,7 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
                 float v[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[k] = le[(p * RI + rr) * LD + c8 + k];
-                if (again) {        // see the head of this file
+                if constexpr (IsF32<T>::value) {        // see the head of this file
                     bool fine = true;
 #pragma unroll
                     for (int k = 0; k < 8; ++k) fine = fine && fabsf(v[k]) < INFINITY;
@@ -642,7 +638,7 @@ __global__ __launch_bounds__(WM * WN * 64, FWD && !IsF32<T>::value ? 4 : 3) void
                         float *row = le + (p * RI + rr) * LD + c8;      // this lane's own eight
 #pragma unroll 1
                         for (int k = 0; k < 8; ++k)
-                            if (k < have && !(fabsf(row[k]) < INFINITY)) row[k] = plain_dot<T, FWD>(A, m, n + k);
+                            if (k < have && !(fabsf(row[k]) < INFINITY)) row[k] = plain_dot<FWD>(A, m, n + k);
 #pragma unroll
                         for (int k = 0; k < 8; ++k) v[k] = row[k];
                     }
@@ -663,7 +659,7 @@ template <class T, bool FWD> __global__ __launch_bounds__(256) void lin_join_ker
     for (int q = 0; q < A.splits; ++q) v += A.part[q * size + at];
     const long long m = at / A.N;
     const int n = (int)(at - m * A.N);
-    if ((IsF32<T>::value || (!FWD && A.aslope)) && !(fabsf(v) < INFINITY)) v = plain_dot<T, FWD>(A, m, n);
+    if (IsF32<T>::value && !(fabsf(v) < INFINITY)) v = plain_dot<FWD>(A, m, n);
     if constexpr (FWD) {
         const float z = v + (A.bias ? (float)static_cast<const T *>(A.bias)[n] : 0.f);
         GATMI_WITH_ACT(A.act, {
@@ -699,10 +695,10 @@ template <class T, int C, int PIECES = Mul<T>::PIECES> struct TileT {
                 *reinterpret_cast<u32x4 *>(to + p * PLANE) = u32x4{q[p][0], q[p][1], q[p][2], q[p][3]};
         }
     }
-    static __device__ __forceinline__ void put2(char *lds, int row, int col, const VecF<8> &v) {
+    static __device__ __forceinline__ void put2(char *lds, int row, int col, const VecF<8> &v, bool twice) {
         static_assert(P == 2, "a tile of halves");
         Gran<T> q[2];
-        split2<T>(v, q[0], q[1]);
+        split2<T>(v, q[0], q[1], twice);
 #pragma unroll
         for (int p = 0; p < 2; ++p)
             *reinterpret_cast<u32x4 *>(lds + p * PLANE + at(row, col)) = u32x4{q[p].w[0], q[p].w[1], q[p].w[2], q[p].w[3]};
@@ -718,6 +714,31 @@ template <class T, int C, int PIECES = Mul<T>::PIECES> struct TileT {
         return __builtin_bit_cast(u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
     }
 };
+
+// Whether this block's sums have to be taken again, where dz is two numbers: some sum is not finite, and so is some
+// factor of the other side among `rows` rows (`stride` apart) of `cols` columns, which met a lo of 0 or of the other
+// sign than hi.  (An infinity of dz alone comes out right.)  They are, by a second pass with hi for lo: twice the sum
+// of the rounded dz, whose infinities and NaN are those of the formula; what was finite stays as it is.
+template <class T>
+__device__ __forceinline__ bool redo(const f32x16v (&acc)[2][2], const T *b, long long rows, long long stride, int cols) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) s = fmaf(acc[i][j][q], 0.f, s);       // NaN once one is not finite
+    if (!__syncthreads_or(s != 0.f)) return false;
+    // as many rows at once as fit the block side by side
+    const int threads = blockDim.x, wide = cols < threads ? cols : threads, high = threads / wide;
+    const int c0 = threadIdx.x % wide, r0 = threadIdx.x / wide;
+    bool bad = false;
+    if (r0 < high)
+        for (int c = c0; c < cols; c += wide)
+#pragma unroll 8
+            for (long long r = r0; r < rows; r += high) bad |= !(fabsf((float)b[r * stride + c]) < INFINITY);
+    return __syncthreads_or(bad);
+}
 
 // The wide form is 512 threads and one block a CU (its registers), so nothing but its own loads in flight hides
 // the memory: two steps' for 16-bit types, 0.82 -> 0.71 ms for [2449029, 256] x [2449029, 256] bf16 together with
@@ -793,13 +814,7 @@ template <class T, int BN, bool SHORT, bool TWO> __global__ __launch_bounds__(2 
         }
     };
     f32x16v acc[2][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
-    auto step = [&](auto set, long long r) {
+    auto step = [&](auto set, long long r, bool twice) __attribute__((always_inline)) {
         Gran<T>(&ga)[NA] = ga_[decltype(set)::value], (&gb)[NB] = gb_[decltype(set)::value];
         SlopeGran<T>(&gs)[NA] = gs_[decltype(set)::value];
         const bool end = r + TA::BK > r1;
@@ -815,11 +830,11 @@ template <class T, int BN, bool SHORT, bool TWO> __global__ __launch_bounds__(2 
             }
             if (sloped) {
                 const VecF<8> v = with_slope<T>(ga[i], gs[i], A.slope_scale);
-                if (sums)
+                if (sums && !twice)
 #pragma unroll
                     for (int k = 0; k < 8; ++k) db.e[k] += v.e[k];     // before the rounding
                 if constexpr (TWO) {
-                    TA::put2(la, ta + i * RA, ja, v);
+                    TA::put2(la, ta + i * RA, ja, v, twice);
                     continue;
                 }
                 ga[i] = to_gran<T>(v);
@@ -852,17 +867,25 @@ template <class T, int BN, bool SHORT, bool TWO> __global__ __launch_bounds__(2 
         }
         __syncthreads();
     };
-    if (r0 < r1) {
+    auto sweep = [&](bool twice) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
+        if (r0 >= r1) return;
         typedef std::integral_constant<int, 0> First;
         typedef std::integral_constant<int, SETS - 1> Second;
         fetch(First{}, r0);
         if constexpr (SETS == 2) fetch(Second{}, r0 + TA::BK);
         for (long long r = r0; r < r1; r += SETS * TA::BK) {
-            step(First{}, r);
+            step(First{}, r, twice);
             if constexpr (SETS == 2)
-                if (r + TA::BK < r1) step(Second{}, r + TA::BK);
+                if (r + TA::BK < r1) step(Second{}, r + TA::BK, twice);
         }
-    }
+    };
+    sweep(false);
     if (sums) {      // [RA][128] partial sums, added in order
         float *red = reinterpret_cast<float *>(smem);
 #pragma unroll
@@ -876,29 +899,44 @@ template <class T, int BN, bool SHORT, bool TWO> __global__ __launch_bounds__(2 
         }
     }
     if (!A.part && !A.dw) return;       // the bias alone
-    bool again = IsF32<T>::value;
-    if constexpr (TWO) again = redo<T, 2, 2>(acc, pb + r0 * A.K + k0, r1 - r0, A.K, A.K - k0 < BN ? A.K - k0 : BN);
     float *part = A.part + split * (long long)A.N * A.K;
+    // f(element's place in dW, its sum)
+    auto each = [&](auto f) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
-                const int n = n0 + wm + i * 32 + acc_row(q, lane >> 5), k = k0 + wn + j * 32 + (lane & 31);
-                if (n >= A.N || k >= A.K) continue;
-                float v = acc[i][j][q];
-                if (again && !(fabsf(v) < INFINITY)) {
-                    v = 0.f;
-                    for (long long m = r0; m < r1; ++m) {
-                        float d = (float)pa[m * A.N + n];
-                        if (sloped) d *= one_slope<T>(static_cast<const ST *>(A.aslope)[m * A.N + n], A.slope_scale);
-                        v = fmaf(d, (float)pb[m * A.K + k], v);
-                    }
+                for (int q = 0; q < 16; ++q) {
+                    const int n = n0 + wm + i * 32 + acc_row(q, lane >> 5), k = k0 + wn + j * 32 + (lane & 31);
+                    if (n < A.N && k < A.K) f(n, k, acc[i][j][q]);
                 }
-                if (A.dw) static_cast<T *>(A.dw)[(long long)n * A.K + k] = (T)v;
-                else part[(long long)n * A.K + k] = v;
+    };
+    each([&](int n, int k, float v) {
+        if (IsF32<T>::value && !(fabsf(v) < INFINITY)) {
+            v = 0.f;
+            for (long long m = r0; m < r1; ++m) {
+                float d = (float)pa[m * A.N + n];
+                if (sloped) d *= static_cast<const float *>(A.aslope)[m * A.N + n];
+                v = fmaf(d, (float)pb[m * A.K + k], v);
             }
+        }
+        if (A.dw) static_cast<T *>(A.dw)[(long long)n * A.K + k] = (T)v;
+        else part[(long long)n * A.K + k] = v;
+    });
+    if constexpr (TWO)
+        if (redo<T>(acc, pb + r0 * A.K + k0, r1 - r0, A.K, A.K - k0 < BN ? A.K - k0 : BN)) {
+            sweep(true);
+            each([&](int n, int k, float v) {
+                const long long at = (long long)n * A.K + k;
+                if (A.dw) {
+                    T *o = static_cast<T *>(A.dw) + at;
+                    if (!(fabsf((float)*o) < INFINITY)) *o = (T)v;
+                } else if (!(fabsf(part[at]) < INFINITY)) {
+                    part[at] = v;
+                }
+            });
+        }
 }
 
 // A few rows (serving): one wave a column of y, lanes along the contraction, f32 multiply-adds whatever the
@@ -980,16 +1018,22 @@ template <class T> __global__ __launch_bounds__(256) void lin_slabs_kernel(const
 }
 
 // The weights as the products take them: rows of `ld` (a multiple of 8, zeros behind the end), the matrix
-// itself (TR: transposed, out[k][n] = w[n][k]), f32 as three planes of bf16 pieces
-template <class T, bool TR> __global__ __launch_bounds__(256) void lin_image_kernel(const T *w, int N, int K, int ld, void *out) {
+// itself (TR: transposed, out[k][n] = w[n][k]), f32 as three planes of bf16 pieces.  bad (or null): a byte a block,
+// whether its 32 x 32 hold an infinity or NaN.
+template <class T, bool TR> __global__ __launch_bounds__(256) void lin_image_kernel(const T *w, int N, int K, int ld, void *out,
+                                                                                        uint8_t *bad) {
     __shared__ T t[32][33];
     const int R = TR ? K : N, S = TR ? N : K;       // rows and columns of the image
     const int s0 = blockIdx.x * 32, r0 = blockIdx.y * 32, x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    int odd = 0;
     for (int i = y; i < 32; i += 8) {
         const int n = TR ? s0 + i : r0 + i, k = TR ? r0 + x : s0 + x;
-        t[TR ? x : i][TR ? i : x] = n < N && k < K ? w[(long long)n * K + k] : (T)0.f;
+        const T v = n < N && k < K ? w[(long long)n * K + k] : (T)0.f;
+        t[TR ? x : i][TR ? i : x] = v;
+        if (!(fabsf((float)v) < INFINITY)) odd = 1;
     }
-    __syncthreads();
+    const int any = __syncthreads_or(odd);
+    if (bad && threadIdx.x == 0) bad[(long long)blockIdx.y * gridDim.x + blockIdx.x] = (uint8_t)(any != 0);
     for (int i = y; i < 32; i += 8) {
         if (r0 + i >= R || s0 + x >= ld) continue;
         const long long at = (long long)(r0 + i) * ld + s0 + x;
@@ -1054,6 +1098,7 @@ struct LinGeom {
     long long per_split;
     int ldf, ldb;                   // row lengths of the weight images, forward and transposed
     size_t image_f, image_b, slabs, dbpart;     // bytes; slabs and dbpart are used by more than one split only
+    size_t bad_b;                   // of image_b, behind the image: a byte for every 32 x 32 (dz as two numbers)
     LinSplitK fwd, dx;
     bool image_fwd;                 // the forward takes an image
     bool few;                       // ... or the few-row kernel
@@ -1103,7 +1148,8 @@ static LinGeom lin_geom(const gatmi_linear *l) {
     if (G.few) G.fwd = {1, l->in_features, 0};
     G.dx = lin_split_k(l->rows, l->in_features, l->out_features, l->dtype);
     G.image_f = G.image_fwd ? align_up((size_t)l->out_features * G.ldf * el) : 0;
-    G.image_b = align_up((size_t)l->in_features * G.ldb * el);
+    G.bad_b = lin_two(l) ? align_up((size_t)((l->in_features + 31) / 32) * ((G.ldb + 31) / 32)) : 0;
+    G.image_b = align_up((size_t)l->in_features * G.ldb * el) + G.bad_b;
     G.slabs = align_up((size_t)G.splits * l->in_features * l->out_features * 4);
     G.dbpart = align_up((size_t)G.splits * l->out_features * 4);
     return G;
@@ -1210,7 +1256,7 @@ extern "C" int gatmi_linear_fwd(const gatmi_linear *l, const void *x, const void
         });
     } else if (G.image_fwd) {
         hipLaunchKernelGGL((lin_image_kernel<float, false>), dim3((G.ldf + 31) / 32, (A.N + 31) / 32), dim3(256), 0, st,
-                           static_cast<const float *>(weight), A.N, A.K, G.ldf, ws);
+                           static_cast<const float *>(weight), A.N, A.K, G.ldf, ws, nullptr);
         A.B = ws;
         A.ldb = G.ldf;
         lin_launch_nt<float, true, true, false>(A, G.fwd, st);
@@ -1281,9 +1327,12 @@ extern "C" int gatmi_linear_bwd(const gatmi_linear *l, const void *x, const void
         A.N = K;
         A.K = N;
         A.ldb = G.ldb;
+        uint8_t *bad = reinterpret_cast<uint8_t *>(image) + (W.image - G.bad_b);
+        A.bad = bad;
+        A.bad_cols = (G.ldb + 31) / 32;
         GATMI_WITH_TYPE(l->dtype, {
             hipLaunchKernelGGL((lin_image_kernel<T, true>), dim3((G.ldb + 31) / 32, (K + 31) / 32), dim3(256), 0, st,
-                               static_cast<const T *>(weight), N, K, G.ldb, ws);
+                               static_cast<const T *>(weight), N, K, G.ldb, ws, two ? bad : nullptr);
             constexpr bool cut = IsF32<T>::value;
             if (two) lin_launch_nt<T, false, cut, !cut>(A, G.dx, st);
             else lin_launch_nt<T, false, cut, false>(A, G.dx, st);

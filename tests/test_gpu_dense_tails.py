@@ -224,3 +224,46 @@ def test_activations_at_the_ends_of_their_range(cuda, dtype, act):
         assert float(y[0, n]) == inf and bool(torch.isnan(y[0, n + 2])) and bool(torch.isnan(db[n + 2]))
         assert float(y[0, n + 1]) == -1.0 if act == "elu" else bool(torch.isnan(y[0, n + 1]))
         assert bool(torch.isfinite(y[0, n + 3:]).all())
+
+
+@pytest.mark.parametrize("act", ["gelu", "elu"])
+def test_linear_gradients_not_finite_cost_no_plain_sums(cuda, act):
+    """an infinity in x or W sends no element through a sum of its own: the step stays within a few times an ordinary one
+    (it was three hundred times), and what does not meet the infinity keeps the ordinary precision"""
+    import gat_amd
+    m = 400000
+    g = torch.Generator().manual_seed(1)
+    x, w = torch.randn(m, 256, generator=g).to(BF16).to(cuda), (torch.randn(256, 256, generator=g) / 16).to(BF16).to(cuda)
+    dy = torch.randn(m, 256, generator=g).to(BF16).to(cuda)
+
+    def step(x, w):
+        xd, wd = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        y = gat_amd.linear_act(xd, wd, act=act)
+        first, last = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        torch.autograd.grad(y, (xd, wd), dy, retain_graph=True)
+        first.record()
+        got = torch.autograd.grad(y, (xd, wd), dy)
+        last.record()
+        torch.cuda.synchronize()
+        return first.elapsed_time(last), got
+
+    ms, plain = step(x, w)
+    for which, at in ((0, (77, 3)), (1, (3, 200))):
+        xs = [x.clone(), w.clone()]
+        xs[which][at] = float("inf")
+        slow, got = step(*xs)
+        assert slow < 20 * ms + 1.0, (slow, ms)
+        dx, dw = got
+        rows, cols = torch.arange(m, device=cuda) != 77, torch.arange(256, device=cuda)
+        # z is infinite in row 77, or in column 3.  The slope there is 0 or 1 for ELU, and inf * 0, NaN, for GELU.
+        if which == 0:
+            assert torch.equal(dx[rows], plain[0][rows])
+            assert not bool(torch.isfinite(dw[:, 3]).any())
+            assert bool(torch.isfinite(dw[:, cols != 3]).all() if act == "elu" else torch.isnan(dw).all())
+            assert bool(torch.isfinite(dx[77]).all() if act == "elu" else torch.isnan(dx[77]).all())
+        else:
+            assert torch.equal(dw[cols != 3], plain[1][cols != 3])
+            if act == "elu":
+                assert bool(torch.isfinite(dx[:, cols != 200]).all()) and not bool(torch.isfinite(dx[:, 200]).any())
+            else:
+                assert bool(torch.isnan(dx).all()) and bool(torch.isnan(dw[3]).all())
