@@ -21,12 +21,12 @@
 // What bounds it (times of the kernels alone under the profiler, whose clock varies by a few percent from run to run).
 // The forward of layers of a few hundred columns is bound by memory for 16-bit types: [2449029, 256] x [256, 256] bf16
 // with GELU and residual takes 1.14 ms (5.0 GB, 4.4 TB/s), where a copy runs at 4.9 TB/s.  Its gradients carry two
-// products for one and the slope's decoding: dx 0.98 ms (3.8 GB, 3.8 TB/s), dW 1.12 ms (3.8 GB, 3.4 TB/s; with dz in one
+// products for one and the slope's decoding: dx 1.01 ms (3.8 GB, 3.7 TB/s), dW 1.14 ms (3.8 GB, 3.3 TB/s; with dz in one
 // number they took 0.85 and 0.71).  Wide layers are bound by what feeds the matrix cores: [65537, 1024] x [1024, 1001]
-// f16 in 0.176 ms, 760 TFLOP/s, with the matrix cores, LDS and the vector units busy for a third of it each.  f32 is
-// between the two: [100000, 240] x [240, 240] takes 0.143 ms forward, of which the matrix cores are busy for 0.031, the
-// vector units (cutting the operands, the activation) for 0.037, and 384 MB at the copy's rate are 0.078; dx 0.122, dW
-// 0.108.  Launched one behind the other the three take 0.35 ms.
+// f16 in 0.177 ms, 760 TFLOP/s, with the matrix cores, LDS and the vector units busy for a third of it each.  f32 is
+// between the two: [100000, 240] x [240, 240] takes 0.145 ms forward, of which the matrix cores are busy for 0.031, the
+// vector units (cutting the operands, the activation) for 0.037, and 384 MB at the copy's rate are 0.078; dx 0.124, dW
+// 0.105.  Launched one behind the other the three take 0.36 ms.
 #include "attn_device.h"
 #include "common.h"
 #include "dense_device.h"
