@@ -92,7 +92,7 @@ def embedding(ids: Tensor, table: Tensor, scale: float = 1.0) -> Tensor:
 
 
 def dropout(x: Tensor, p: float, training: bool = True, seed=None, residual: Optional[Tensor] = None) -> Tensor:
-    """x / (1 - p) where a counter-based draw of (seed, row, column) keeps it, else 0; plus `residual`.  No
+    """x / (1 - p) where a counter-based draw of (seed, row, column) keeps it, else 0; plus `residual`; 0 <= p < 1.  No
     mask is stored: the backward draws it again.  Rows are x flattened to [rows, x.size(-1)], and the mask is
     `gat_amd.glue.dropout_mask(rows, cols, p, seed)`.  `seed`: an int; None draws one from torch's generator;
     a one-element int64 CUDA tensor is advanced in place on the device and read there, so the call can be
